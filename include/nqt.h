@@ -56,6 +56,8 @@ extern "C" {
 #define NQT_BF16 0
 #define NQT_F16 1
 #define NQT_F32 2
+#define NQT_I8 3   /* two's-complement int8 codes of a KV cache, in [-127, 127] */
+#define NQT_E4M3 4 /* float8 e4m3 codes of a KV cache */
 
 /* Version of this ABI; bumped on any signature change. */
 int nqt_abi_version(void);
@@ -548,6 +550,65 @@ int nqt_step_finish(const int32_t* row_slot, int rows, int slots, const int64_t*
                     int32_t* slot_step, const int32_t* slot_max_tokens, const int32_t* slot_eos_from,
                     int64_t* slot_offset, int64_t offset_stride, uint8_t* terminal, int32_t* n_terminal,
                     int32_t* status, void* stream);
+
+/*
+ * 8-bit paged KV cache.  A layer is `layer_cache`, contiguous one-byte codes
+ * [total_pages, 2, page_size, num_kv_heads, head_dim] (kind 0 = K, 1 = V), and
+ * `layer_scales`, contiguous f32 [total_pages, 2, page_size / 16, num_kv_heads]:
+ * one scale for every block of 16 tokens of a page, kind and KV head.  An
+ * element stands for code * scale; `code` is NQT_I8 or NQT_E4M3.  page_size is a
+ * multiple of 16 up to 256, head_dim 64 or 128, num_kv_heads <= 256; the cache
+ * is 16-byte aligned.
+ *
+ * nqt_qk_norm_rope_paged_cache8: the step's QK RMSNorm + RoPE with the quantised
+ * K/V write, the 8-bit counterpart of nqt_qk_norm_rope_paged_kv_write (bf16
+ * inputs, fp32 in between).  q leaves rotated through q_out (bf16, which may not
+ * overlap q); k and v are only read.  The tokens of one call that follow one
+ * another in the token order with one page, one block and rising offsets form a
+ * group with one scale: need = largest magnitude / top code (127 or 448).  A
+ * group whose first offset in its block is 0 starts the block with scale need.
+ * Any other keeps the block's scale s, or doubles it until it is >= need (s = 0:
+ * need), and then the codes at lower offsets are rounded again to code * s / s'.
+ * Codes behind the group are left as they are.  A call's tokens of one block
+ * must form one group: two groups of one block in a call race on its scale.
+ * Infinities count as the largest finite number, NaN becomes code 0 (NQT_I8) or
+ * the NaN code (NQT_E4M3).  A page or offset outside the pool sets
+ * NQT_DEV_BAD_PAGE and writes nothing.
+ *
+ * nqt_read_paged_cache8: pages i64 [count] of a layer as bf16
+ * [count, 2, page_size, num_kv_heads, head_dim] (out 16-byte aligned, contiguous).
+ */
+int nqt_qk_norm_rope_paged_cache8(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+    const void* k, int64_t k_stride_tok, int64_t k_stride_head,
+    const void* v, int64_t v_stride_tok, int64_t v_stride_head,
+    const void* q_weight, const void* k_weight,
+    const int64_t* position_ids, const int64_t* write_pages, const int64_t* write_offsets,
+    void* q_out, int64_t out_stride_tok, int64_t out_stride_head,
+    void* layer_cache, float* layer_scales, int total_pages, int page_size,
+    int tokens, int num_qo_heads, int num_kv_heads, int head_dim,
+    float eps, float rope_theta, int code, int32_t* status, void* stream);
+int nqt_read_paged_cache8(const void* layer_cache, const float* layer_scales, int total_pages, int page_size,
+                          int num_kv_heads, int head_dim, int code, const int64_t* pages, int count, void* out,
+                          int32_t* status, void* stream);
+
+/*
+ * Paged GQA decode attention over an 8-bit layer: nqt_decode_attention_ex's
+ * contract (bf16 q and out, num_qo_heads / num_kv_heads <= 8, its flags) without
+ * a plan: the split is computed inside the launch from kv_indptr and
+ * last_page_len.  batch <= 8192; rows without pages give zeros.  The workspace
+ * (16-byte aligned, nqt_decode8_workspace_bytes) must be zero before its first
+ * use and belongs to this entry point: every launch leaves its tickets at zero.
+ * One launch at a time per workspace; any shape within its capacity.
+ */
+size_t nqt_decode8_workspace_bytes(int batch_capacity, int num_qo_heads, int head_dim);
+int nqt_decode_attention8(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+    const void* layer_cache, const float* layer_scales, int total_pages, int page_size,
+    const int32_t* kv_indptr, const int32_t* kv_indices, const int32_t* last_page_len,
+    int batch, int batch_capacity, int num_qo_heads, int num_kv_heads, int head_dim,
+    float sm_scale, int code, void* out, int64_t out_stride_tok, int64_t out_stride_head,
+    void* workspace, size_t workspace_bytes, int flags, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,7 +14,9 @@ from .kernels import (
     decode_attn_nhd_short_cache,
     paired_qk_norm_rope_,
     paired_qk_norm_rope_dense_cache_,
+    paired_qk_norm_rope_paged_cache8,
     paired_qk_norm_rope_paged_cache_,
+    read_paged_cache8,
 )
 from .planner import DevicePagePlanner, KVAllocationError
 from .sampling import (
@@ -29,8 +31,10 @@ from .talker_kv import (
     B200TalkerBinding,
     TalkerAttentionMetadata,
     batch_decode_paged,
+    batch_decode_paged8,
     batch_prefill_paged,
     binding_factory,
+    decode_paged8_workspace,
 )
 
 __all__ = [
@@ -42,16 +46,20 @@ __all__ = [
     "RequestSampling",
     "TalkerAttentionMetadata",
     "batch_decode_paged",
+    "batch_decode_paged8",
     "batch_prefill_paged",
     "binding_factory",
     "cp_decode_attention_",
     "decode_attn_nhd_short_cache",
+    "decode_paged8_workspace",
     "kernels",
     "lib",
     "paired_qk_norm_rope_",
     "paired_qk_norm_rope_dense_cache_",
+    "paired_qk_norm_rope_paged_cache8",
     "paired_qk_norm_rope_paged_cache_",
     "planner",
+    "read_paged_cache8",
     "sample_code_predictor_cuda_graph",
     "sample_logits_cuda_graph",
     "sample_logits_stateless",

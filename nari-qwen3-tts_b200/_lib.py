@@ -32,6 +32,8 @@ NQT_DEV_BAD_TOKEN = 0x40
 NQT_BF16 = 0
 NQT_F16 = 1
 NQT_F32 = 2
+NQT_I8 = 3
+NQT_E4M3 = 4
 
 P = c_void_p
 I = c_int
@@ -104,6 +106,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "nqt_gemm_fp8_pack_weight": (I, [P, L, I, I, I, P, P]),
     "nqt_gemm_fp8_workspace_bytes": (I, [I, I, I, I, P]),
     "nqt_gemm_fp8": (I, [P, L, P, L, P, P, P, L, I, I, I, I, I, I, P, L, P, P]),
+    "nqt_qk_norm_rope_paged_cache8": (
+        I,
+        [P, L, L, P, L, L, P, L, L, P, P, P, P, P, P, L, L, P, P, I, I, I, I, I, I, F, F, I, P, P],
+    ),
+    "nqt_read_paged_cache8": (I, [P, P, I, I, I, I, I, P, I, P, P, P]),
+    "nqt_decode8_workspace_bytes": (Z, [I, I, I]),
+    "nqt_decode_attention8": (
+        I,
+        [P, L, L, P, P, I, I, P, P, P, I, I, I, I, I, F, I, P, L, L, P, Z, I, P, P],
+    ),
     "nqt_step_stage": (I, [P, I, I, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P]),
     "nqt_talker_logits_mask": (I, [P, I, L, I, I, I, I, P, P]),
     "nqt_step_finish": (I, [P, I, I, P, I, P, P, P, P, L, P, P, P, P]),
@@ -192,6 +204,15 @@ def call(name: str, *args) -> int:
     return rc
 
 
+def call_on(device: torch.device, name: str, *args) -> int:
+    """``call`` with ``device`` current: a launch goes to the device of its tensors whichever is current."""
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(device):
+        return call(name, *args)
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -212,6 +233,16 @@ def dtype_code(dtype: torch.dtype) -> int:
     if dtype == torch.float32:
         return NQT_F32
     raise TypeError(f"unsupported element type {dtype}")
+
+
+def cache_code(dtype: torch.dtype) -> int:
+    """Code of an 8-bit KV cache's element type."""
+
+    if dtype == torch.int8:
+        return NQT_I8
+    if dtype == torch.float8_e4m3fn:
+        return NQT_E4M3
+    raise TypeError(f"an 8-bit KV cache holds int8 or float8_e4m3fn, not {dtype}")
 
 
 def require_cuda(*tensors: torch.Tensor | None) -> torch.device:

@@ -1,0 +1,716 @@
+// Paged GQA decode attention over an 8-bit KV cache (layout and codes: cache8.cuh).
+//
+//   out[b, h] = softmax(q[b, h] . K[b, :, h / G]^T * sm_scale) V[b, :, h / G]
+//
+// over the (n_pages - 1) * P + last_page_len tokens of row b, one query per row.
+//
+// Mathematics.  With codes k_t, v_t and block scales a, c (16 tokens each):
+//   s_t = a * (q . k_t) * sm_scale,   O = sum_t 2^(s_t - m) c v_t / sum_t 2^(s_t - m)
+// in one pass with a running reference m and fp32 sums.  q . k and p . v are
+// fp16 tensor-core tiles with fp32 accumulation: codes are exact in fp16; q is
+// brought to [1, 2) by the power of two of its row maximum, which is exact for
+// every element above 2^-14 of it; p is rounded to fp16's 11 bits and kept
+// between 2^-32 and 2^7 of the reference, so m only moves when a score exceeds
+// it by more than 7 (in log2) and the accumulators are rarely rescaled.  The
+// scale c multiplies the tile's fp32 product, so no rounding depends on it.
+//
+// Work split.  The KV of one KV-head group is a flat list of 16-token tiles;
+// CTA c of n streams tiles [T c / n, T (c + 1) / n) across sequence borders, so
+// every CTA moves the same bytes whatever the lengths are.  The tile prefix is
+// computed by every CTA from the row lengths (one read and a scan, which costs
+// no more than reading a prefix that a plan kernel left), so the call is one
+// launch.  A sequence that several CTAs cover is finished by the warp that
+// completes its ticket, from fp32 partials in the workspace, in CTA order: the
+// result does not depend on which one that is.  No CTA waits for another.
+//
+// Data path.  A producer warp keeps STAGES tiles in flight with TMA boxes
+// {D bytes, 1 head, 16 tokens, K and V}; each consumer warp owns one KV head.
+// Rows of 128 (64) bytes use the 128-byte (64-byte) swizzle, so ldmatrix reads
+// eight rows without bank conflicts.  ldmatrix moves 16-bit units: as an A
+// operand K's bytes 4t..4t+3 of a row become two fp16 pairs, and since a dot
+// product does not mind the order of its terms q's fragments are loaded in that
+// order; for V the transposing form delivers bytes (token, token + 1) x (dim,
+// dim + 1), and one byte permutation sorts them into the fragments of two dims.
+// P goes from the accumulator layout to the B layout with movmatrix.
+#include "cache8.cuh"
+
+namespace nqt {
+namespace {
+
+using namespace c8;
+
+constexpr int kMaxCtas = 1184;     // split CTAs per head group (8 per SM on 148 SMs)
+constexpr int kMaxRows8 = 8192;    // rows whose prefix a CTA holds in shared memory
+constexpr int kPageWindow = 1024;  // page ids of one CTA's tile range staged in shared memory
+
+constexpr size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+struct Ws8 {
+  size_t lse, o, total;  // tickets i32 [batch_cap * hq] come first, zero between launches
+};
+
+constexpr Ws8 ws8_layout(int batch_cap, int hq, int d) {
+  Ws8 w{};
+  w.lse = up256(4 * static_cast<size_t>(batch_cap) * hq);
+  w.o = up256(w.lse + 4 * static_cast<size_t>(2 * kMaxCtas) * hq);
+  w.total = up256(w.o + 4 * static_cast<size_t>(2 * kMaxCtas) * hq * d);
+  return w;
+}
+
+struct Decode8Args {
+  const __nv_bfloat16* q;
+  int64_t q_st, q_sh;
+  __nv_bfloat16* out;
+  int64_t o_st, o_sh;
+  const float* scales;
+  const int32_t *indptr, *indices, *last_len;
+  int32_t* tickets;
+  float *part_lse, *part_o;
+  int32_t* status;
+  int batch, hq, hkv, group, page_size, total_pages, n_ctas;
+  int early;  // NQT_DECODE_OVERLAP_KV_WRITE
+  float scale_log2;
+  uint64_t wait_ns;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Transpose of an 8 x 8 matrix of 16-bit elements held one row per quad.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+__device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int head, int tok, int pk,
+                                         uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(0), "r"(head), "r"(tok), "r"(pk), "l"(policy)
+      : "memory");
+}
+
+// Bounded pipeline wait; with NQT_DECODE_SHORT_WAIT (limit 0) one look at the barrier that does not suspend.
+__device__ __forceinline__ bool pipe_wait(uint64_t* bar, uint32_t parity, const Decode8Args& p) {
+  if (p.wait_ns != 0) return mbar_wait_ns(bar, parity, p.status, p.wait_ns);
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  if (!ok) report(p.status, NQT_DEV_TIMEOUT);
+  return ok != 0;
+}
+
+__device__ __forceinline__ int atomic_inc_acq_rel(int32_t* addr) {
+  int32_t old;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(addr) : "memory");
+  return old;
+}
+
+// First tile of CTA c of n, and the CTA that owns tile t.
+__device__ __forceinline__ int64_t first_tile(int64_t total, int c, int n) { return total * c / n; }
+__device__ __forceinline__ int tile_owner(int64_t total, int n, int64_t t) {
+  return static_cast<int>(((t + 1) * n + total - 1) / total) - 1;
+}
+
+// Row that owns flat tile t: the last b with prefix[b] <= t.
+__device__ __forceinline__ int row_of_tile(const int32_t* prefix, int batch, int64_t t) {
+  int lo = 0, hi = batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// out = sum_i 2^(lse_i - M) O_i / sum_i 2^(lse_i - M) over the CTAs c0..c1 that cover `row`, for the query heads
+// of one KV head, by one warp; lane l owns the float4 columns l, l + 32, ...  A CTA's part is in slot 2c when the
+// row starts inside its range, else in 2c + 1.
+template <int D>
+__device__ __forceinline__ void combine_row(const Decode8Args& p, int row, int kvh, int64_t total, int n, int c0,
+                                            int c1, int64_t row_t0, int lane) {
+  constexpr int QD = D / 4;
+  constexpr int kBatch = 4;
+  const float NEG_INF = -__int_as_float(0x7f800000);
+  for (int f = lane; f < p.group * QD; f += 32) {
+    const int head = kvh * p.group + f / QD;
+    float m = NEG_INF, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int cb = c0; cb <= c1; cb += kBatch) {
+      float lse[kBatch];
+      float4 v[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int cc = cb + k;
+        lse[k] = NEG_INF;
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (cc <= c1) {
+          const int slot = first_tile(total, cc, n) >= row_t0 ? 2 * cc : 2 * cc + 1;
+          const int64_t r = static_cast<int64_t>(slot) * p.hq + head;
+          lse[k] = __ldcg(p.part_lse + r);
+          v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D) + f % QD);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (cb + k > c1) continue;
+        const float nm = fmaxf(m, lse[k]);
+        const float ref = nm == NEG_INF ? 0.f : nm;
+        const float a = exp2f(m - ref), w = exp2f(lse[k] - ref);
+        sum = sum * a + w;
+        acc.x = acc.x * a + w * v[k].x;
+        acc.y = acc.y * a + w * v[k].y;
+        acc.z = acc.z * a + w * v[k].z;
+        acc.w = acc.w * a + w * v[k].w;
+        m = nm;
+      }
+    }
+    const float inv = 1.f / sum;
+    __nv_bfloat16* dst = p.out + row * p.o_st + static_cast<int64_t>(head) * p.o_sh + (f % QD) * 4;
+    *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+    *reinterpret_cast<__nv_bfloat162*>(dst + 2) = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+  }
+}
+
+template <int D, int HPC, int STAGES>
+struct Cfg8 {
+  static constexpr int kBox = 2 * kBlock * D;  // K then V of 16 tokens of one head
+  static constexpr int kStage = HPC * kBox;
+  static constexpr int kThreads = (HPC + 1) * 32;
+  static constexpr int kBars = 2 * STAGES * 8;
+  static __host__ __device__ constexpr int smem(int batch) {
+    return STAGES * kStage + 1024 + kBars + 4 * kPageWindow + 4 * (2 * (batch + 1)) + (batch + 3) / 4 * 4;
+  }
+};
+
+template <int D, int HPC, int STAGES, bool E4M3>
+__global__ void __launch_bounds__((HPC + 1) * 32) decode8_kernel(const __grid_constant__ CUtensorMap tmap,
+                                                                 const __grid_constant__ Decode8Args p) {
+  using Cfg = Cfg8<D, HPC, STAGES>;
+  constexpr int CH = D / 16;  // 16-byte chunks of a row
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::kStage);
+  uint64_t* empty = full + STAGES;
+  int32_t* s_pages = reinterpret_cast<int32_t*>(empty + STAGES);
+  int32_t* s_prefix = s_pages + kPageWindow;      // [batch + 1] first tile of every row
+  int32_t* s_base = s_prefix + p.batch + 1;       // [batch + 1] kv_indptr
+  uint8_t* s_valid = reinterpret_cast<uint8_t*>(s_base + p.batch + 1);  // [batch] tokens of the row's last tile
+  __shared__ int s_warp_sum[HPC + 1];
+  __shared__ int s_issued;
+  __shared__ int s_progress[HPC];
+
+  // see nqt_decode_attention_ex: by default everything waits for the previous grid; with `early` only q, each
+  // row's last tile and its scales, the workspace and all writes do
+  if (!p.early) grid_dependency_wait();
+  grid_dependents_launch();
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int tpp = p.page_size / kBlock;
+
+  // tile prefix of the batch: exclusive scan of the rows' tile counts
+  int carry = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += Cfg::kThreads) {
+    const int b = b0 + threadIdx.x;
+    int tiles = 0;
+    if (b < p.batch) {
+      const int i0 = p.indptr[b], np = p.indptr[b + 1] - i0;
+      int valid = 0;
+      if (np > 0) {
+        int ll = p.last_len[b];
+        ll = ll < 1 ? 1 : (ll > p.page_size ? p.page_size : ll);
+        tiles = (np - 1) * tpp + (ll + kBlock - 1) / kBlock;
+        valid = ll - (ll - 1) / kBlock * kBlock;
+      }
+      s_base[b] = i0;
+      s_valid[b] = static_cast<uint8_t>(valid);
+    }
+    int incl = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(kFull, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_warp_sum[warp] = incl;
+    __syncthreads();
+    int before = carry, sum = 0;
+#pragma unroll
+    for (int w = 0; w < HPC + 1; ++w) {
+      if (w < warp) before += s_warp_sum[w];
+      sum += s_warp_sum[w];
+    }
+    if (b < p.batch) s_prefix[b] = before + incl - tiles;
+    carry += sum;
+    __syncthreads();
+  }
+  const int64_t total = carry;
+  if (threadIdx.x == 0) {
+    s_prefix[p.batch] = carry;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], HPC);
+    }
+    fence_barrier_init();
+  }
+  __syncthreads();
+
+  const int c = blockIdx.x;
+  const int kv0 = blockIdx.y * HPC;
+  // rows without a page are zeros (this CTA's heads of rows c, c + n_ctas, ...)
+  for (int b = c; b < p.batch; b += p.n_ctas) {
+    if (s_valid[b] != 0) continue;
+    if (p.early) grid_dependency_wait();
+    for (int i = threadIdx.x; i < HPC * p.group * D; i += Cfg::kThreads)
+      p.out[b * p.o_st + static_cast<int64_t>(kv0 * p.group + i / D) * p.o_sh + i % D] = __float2bfloat16_rn(0.f);
+  }
+  // fewer tiles than CTAs: one tile each and the rest idle, so every range is non-empty
+  const int n = total < p.n_ctas ? static_cast<int>(total) : p.n_ctas;
+  if (c >= n) return;  // uniform over the block
+  const int64_t t_begin = first_tile(total, c, n);
+  const int64_t t_end = first_tile(total, c + 1, n);
+  const int n_tiles = static_cast<int>(t_end - t_begin);
+
+  if (warp == HPC) {
+    // ---------------------------------------------------------- producer
+    const int row_a = row_of_tile(s_prefix, p.batch, t_begin);
+    const int row_b = row_of_tile(s_prefix, p.batch, t_end - 1);
+    // the range's tiles read one contiguous window of kv_indices: bring it in with all lanes
+    const int win0 = s_base[row_a] + static_cast<int>(t_begin - s_prefix[row_a]) / tpp;
+    const int win1 = s_base[row_b] + static_cast<int>(t_end - 1 - s_prefix[row_b]) / tpp + 1;
+    const bool windowed = win1 - win0 <= kPageWindow;
+    if (windowed)
+      for (int i = lane; i < win1 - win0; i += 32) s_pages[i] = p.indices[win0 + i];
+    __syncwarp();
+    if (lane == 0) prefetch_tensormap(&tmap);
+    uint64_t evict_first;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(evict_first));
+    int row = row_a;
+    bool met = !p.early;
+    int issued = 0;
+    for (int i = 0; i < n_tiles; ++i) {
+      const int64_t t = t_begin + i;
+      while (t >= s_prefix[row + 1]) ++row;
+      if (!met && t == s_prefix[row + 1] - 1) {  // a row's last tile may come from the previous grid
+        grid_dependency_wait();
+        met = true;
+      }
+      const int s = i % STAGES;
+      const bool ready = i < STAGES || pipe_wait(&empty[s], ((i / STAGES) - 1) & 1, p);
+      if (!__all_sync(kFull, ready)) break;
+      const int in_row = static_cast<int>(t - s_prefix[row]);
+      const int pl = in_row / tpp;
+      const int pos = s_base[row] + pl;
+      int page = windowed ? s_pages[pos - win0] : p.indices[pos];
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.total_pages)) {
+        if (lane == 0) report(p.status, NQT_DEV_BAD_PAGE);
+        page = p.total_pages;  // a box outside the map: TMA fills zeros
+      }
+      if (lane == 0) mbar_arrive_expect_tx(&full[s], Cfg::kStage);
+      __syncwarp();
+      if (lane < HPC)
+        tma_tile(smem + s * Cfg::kStage + lane * Cfg::kBox, &tmap, &full[s], kv0 + lane, (in_row - pl * tpp) * kBlock,
+                 page * 2, evict_first);
+      issued = i + 1;
+    }
+    if (lane == 0) s_issued = issued;
+  } else {
+    // ------------------------------------------------------------ consumers
+    const int kvh = kv0 + warp;
+    const int g = lane >> 2, t4 = lane & 3;
+    const int lm_j = lane >> 3, lm_r = lane & 7;
+    const int group = p.group;
+    const float NEG_INF = -__int_as_float(0x7f800000);
+
+    uint32_t qf[CH][2];
+    float o[CH][4];
+    float m0 = NEG_INF, m1 = NEG_INF, l0 = 0.f, l1 = 0.f;  // references and sums of heads 2 t4, 2 t4 + 1
+    float f0 = 0.f, f1 = 0.f;                              // their score factors: 2^e of q, sm_scale, log2 e
+
+    // scales of up to 32 tiles ahead, one per lane; the page ids are a chunk further ahead
+    auto tile_page = [&](int i) -> int {  // page of this lane's tile i, -1 past the range
+      if (i >= n_tiles) return -1;
+      const int r = row_of_tile(s_prefix, p.batch, t_begin + i);
+      return p.indices[s_base[r] + static_cast<int>(t_begin + i - s_prefix[r]) / tpp];
+    };
+    auto tile_scales = [&](int i, int page, float& ks, float& vs) {
+      ks = vs = 0.f;
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.total_pages)) return;
+      const int r = row_of_tile(s_prefix, p.batch, t_begin + i);
+      const int blk = static_cast<int>(t_begin + i - s_prefix[r]) % tpp;
+      const float* sp = p.scales + (static_cast<int64_t>(page) * 2 * tpp + blk) * p.hkv + kvh;
+      ks = __ldcg(sp);  // from L2: the previous grid may have written neighbouring scales
+      vs = __ldcg(sp + static_cast<int64_t>(tpp) * p.hkv);
+    };
+    int page_nx = tile_page(lane);
+    float ks_c = 0.f, vs_c = 0.f, ks_n, vs_n;
+    if (p.early) grid_dependency_wait();  // q, the last tiles' scales, the partials and tickets of the last launch
+    tile_scales(lane, page_nx, ks_n, vs_n);
+    page_nx = tile_page(32 + lane);
+
+    int row = row_of_tile(s_prefix, p.batch, t_begin);
+    int row_t0 = s_prefix[row], row_t1 = s_prefix[row + 1];
+    bool open = false;
+    int fix_a = -1, fix_b = -1;  // split rows whose ticket this warp completed
+    int stop = n_tiles;          // first tile that was not consumed
+
+    for (int i = 0; i < n_tiles; ++i) {
+      if ((i & 31) == 0) {  // the next 32 tiles' scales have arrived; start on those after them
+        ks_c = ks_n;
+        vs_c = vs_n;
+        tile_scales(i + 32 + lane, page_nx, ks_n, vs_n);
+        page_nx = tile_page(i + 64 + lane);
+      }
+      const int64_t t = t_begin + i;
+      while (t >= row_t1) {
+        ++row;
+        row_t0 = row_t1;
+        row_t1 = s_prefix[row + 1];
+      }
+      if (!open) {
+        // a new row: its query heads of the group, as B fragments in K's byte order, scaled to a maximum in [1, 2)
+        const __nv_bfloat16* qrow = p.q + row * p.q_st + static_cast<int64_t>(kvh * group + g) * p.q_sh;
+        uint32_t raw[CH][2];
+        float amax = 0.f;
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) {
+          raw[ch][0] = raw[ch][1] = 0u;
+          if (g < group) {
+            raw[ch][0] = *reinterpret_cast<const uint32_t*>(qrow + ch * 16 + 4 * t4);
+            raw[ch][1] = *reinterpret_cast<const uint32_t*>(qrow + ch * 16 + 4 * t4 + 2);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ch][h]));
+            amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 2));
+        int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+        e = (amax == 0.f || e > 127) ? 0 : min(max(e, -126), 126);
+        const float down = fp8::exp2_int(-e);
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ch][h]));
+            qf[ch][h] = pack_f16x2(v.x * down, v.y * down);
+          }
+        f0 = fp8::exp2_int(__shfl_sync(kFull, e, 8 * t4)) * p.scale_log2;
+        f1 = fp8::exp2_int(__shfl_sync(kFull, e, 8 * t4 + 4)) * p.scale_log2;
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) o[ch][0] = o[ch][1] = o[ch][2] = o[ch][3] = 0.f;
+        m0 = m1 = NEG_INF;
+        l0 = l1 = 0.f;
+        open = true;
+      }
+      const bool last_tile = t == row_t1 - 1;
+      const int valid = last_tile ? s_valid[row] : kBlock;
+      const float ks = __shfl_sync(kFull, ks_c, i & 31), vs = __shfl_sync(kFull, vs_c, i & 31);
+
+      const int s = i % STAGES;
+      if (!__all_sync(kFull, pipe_wait(&full[s], (i / STAGES) & 1, p))) {
+        stop = i;
+        break;
+      }
+      const uint32_t box = smem_addr(smem + s * Cfg::kStage + warp * Cfg::kBox);
+      const int tok = ((lm_j & 1) << 3) + lm_r;  // ldmatrix row of this lane
+      const uint32_t krow = box + tok * D, vrow = krow + kBlock * D;
+      const int sw = D == 128 ? (tok & 7) : ((tok >> 1) & 3);
+
+      // S^T[tok][head] = sum_d K[tok][d] Q[head][d], in two chains
+      float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int cc = 0; cc < CH; cc += 2) {
+        uint32_t r0, r1, r2, r3;
+        ldmatrix_x4(r0, r1, r2, r3, krow + (((cc + (lm_j >> 1)) ^ sw) << 4));
+        uint32_t a0, a1, a2, a3;
+        codes_to_f16_rows<E4M3>(r0, a0, a2);
+        codes_to_f16_rows<E4M3>(r1, a1, a3);
+        mma_f16_16816(sa, a0, a1, a2, a3, qf[cc][0], qf[cc][1]);
+        codes_to_f16_rows<E4M3>(r2, a0, a2);
+        codes_to_f16_rows<E4M3>(r3, a1, a3);
+        mma_f16_16816(sb, a0, a1, a2, a3, qf[cc + 1][0], qf[cc + 1][1]);
+      }
+      // online softmax (log2): the lane holds heads 2 t4 (0, 2) and 2 t4 + 1 (1, 3) of tokens g and g + 8
+      const bool lo = g < valid, hi = g + 8 < valid;
+      const float c0 = ks * f0, c1 = ks * f1;
+      const float s0 = lo ? (sa[0] + sb[0]) * c0 : NEG_INF;
+      const float s1 = lo ? (sa[1] + sb[1]) * c1 : NEG_INF;
+      const float s2 = hi ? (sa[2] + sb[2]) * c0 : NEG_INF;
+      const float s3 = hi ? (sa[3] + sb[3]) * c1 : NEG_INF;
+      float x0 = fmaxf(s0, s2), x1 = fmaxf(s1, s3);
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(kFull, x0, off));
+        x1 = fmaxf(x1, __shfl_xor_sync(kFull, x1, off));
+      }
+      if (__any_sync(kFull, x0 > m0 + 7.f || x1 > m1 + 7.f)) {  // always on a row's first tile (m = -inf)
+        const float n0 = x0 > m0 + 7.f ? x0 : m0, n1 = x1 > m1 + 7.f ? x1 : m1;
+        const float a0 = n0 == m0 ? 1.f : ex2(m0 - n0), a1 = n1 == m1 ? 1.f : ex2(m1 - n1);
+        l0 *= a0;
+        l1 *= a1;
+        m0 = n0;
+        m1 = n1;
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) {
+          o[ch][0] *= a0;
+          o[ch][1] *= a1;
+          o[ch][2] *= a0;
+          o[ch][3] *= a1;
+        }
+      }
+      // p is held 2^8 above its value: fp16 then reaches down to 2^-32 of the reference
+      const float r0 = m0 - 8.f, r1 = m1 - 8.f;
+      const float p0 = ex2(s0 - r0), p1 = ex2(s1 - r1), p2 = ex2(s2 - r0), p3 = ex2(s3 - r1);
+      l0 += p0 + p2;
+      l1 += p1 + p3;
+      const uint32_t b0 = movmatrix_trans(pack_f16x2(p0, p1)), b1 = movmatrix_trans(pack_f16x2(p2, p3));
+      // e4m3 codes behind the row's end may be NaN codes: they count as zeros
+      uint32_t k0 = 0xffffffffu, k1 = 0xffffffffu;
+      if (E4M3) {
+        k0 = (2 * t4 < valid ? 0xffffu : 0u) | (2 * t4 + 1 < valid ? 0xffff0000u : 0u);
+        k1 = (2 * t4 + 8 < valid ? 0xffffu : 0u) | (2 * t4 + 9 < valid ? 0xffff0000u : 0u);
+      }
+      // O^T[d][head] += c * sum_tok V[tok][d] P[head][tok]; rows g and g + 8 of a chunk are its dims 2g and 2g + 1
+#pragma unroll
+      for (int cc = 0; cc < CH; cc += 2) {
+        uint32_t v0, v1, v2, v3;
+        ldmatrix_x4_trans(v0, v1, v2, v3, vrow + (((cc + (lm_j >> 1)) ^ sw) << 4));
+        uint32_t a0, a1, a2, a3;
+        float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
+        codes_to_f16_cols<E4M3>(v0, a0, a1);
+        codes_to_f16_cols<E4M3>(v1, a2, a3);
+        mma_f16_16816(d, a0 & k0, a1 & k0, a2 & k1, a3 & k1, b0, b1);
+        codes_to_f16_cols<E4M3>(v2, a0, a1);
+        codes_to_f16_cols<E4M3>(v3, a2, a3);
+        mma_f16_16816(e, a0 & k0, a1 & k0, a2 & k1, a3 & k1, b0, b1);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          o[cc][x] = fmaf(vs, d[x], o[cc][x]);
+          o[cc + 1][x] = fmaf(vs, e[x], o[cc + 1][x]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+
+      if (last_tile || i == n_tiles - 1) {
+        float t0 = l0, t1 = l1;
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          t0 += __shfl_xor_sync(kFull, t0, off);
+          t1 += __shfl_xor_sync(kFull, t1, off);
+        }
+        const float i0 = 1.f / t0, i1 = 1.f / t1;
+        const int ha = kvh * group + 2 * t4;
+        const bool has0 = 2 * t4 < group, has1 = 2 * t4 + 1 < group;
+        if (t_begin <= row_t0 && t_end >= row_t1) {
+          __nv_bfloat16* ob = p.out + row * p.o_st + static_cast<int64_t>(ha) * p.o_sh + 2 * g;
+#pragma unroll
+          for (int ch = 0; ch < CH; ++ch) {
+            if (has0)
+              *reinterpret_cast<__nv_bfloat162*>(ob + ch * 16) = __floats2bfloat162_rn(o[ch][0] * i0, o[ch][2] * i0);
+            if (has1)
+              *reinterpret_cast<__nv_bfloat162*>(ob + p.o_sh + ch * 16) =
+                  __floats2bfloat162_rn(o[ch][1] * i1, o[ch][3] * i1);
+          }
+        } else {
+          const int slot = t_begin >= row_t0 ? 2 * c : 2 * c + 1;
+          float* po = p.part_o + (static_cast<int64_t>(slot) * p.hq + ha) * D + 2 * g;
+          float* pl = p.part_lse + static_cast<int64_t>(slot) * p.hq + ha;
+#pragma unroll
+          for (int ch = 0; ch < CH; ++ch) {
+            if (has0) *reinterpret_cast<float2*>(po + ch * 16) = make_float2(o[ch][0] * i0, o[ch][2] * i0);
+            if (has1) *reinterpret_cast<float2*>(po + D + ch * 16) = make_float2(o[ch][1] * i1, o[ch][3] * i1);
+          }
+          if (g == 0) {
+            if (has0) pl[0] = m0 + log2f(t0);
+            if (has1) pl[1] = m1 + log2f(t1);
+          }
+          __syncwarp();
+          const int ca = tile_owner(total, n, row_t0), cb = tile_owner(total, n, row_t1 - 1);
+          int32_t* ticket = p.tickets + static_cast<int64_t>(row) * p.hq + kvh;
+          int arrived = 0;
+          if (lane == 0) arrived = atomic_inc_acq_rel(ticket);
+          arrived = __shfl_sync(kFull, arrived, 0);
+          if (arrived == cb - ca) {
+            if (lane == 0) *ticket = 0;  // ready for the next launch
+            if (fix_a < 0) fix_a = row;  // only a range's first and last rows can be split
+            else fix_b = row;
+          }
+        }
+        open = false;
+      }
+    }
+
+    if (stop < n_tiles) {
+      // A wait gave up (NQT_DEV_TIMEOUT is set, the output is undefined).  The split rows that this warp did not
+      // finish still count in on their tickets, so that each returns to zero for the next launch.
+      const int last = row_of_tile(s_prefix, p.batch, t_end - 1);
+      for (int r = row; r <= last; r = r == row && last != row ? last : last + 1) {
+        const int r0 = s_prefix[r], r1 = s_prefix[r + 1];
+        if (t_begin <= r0 && t_end >= r1) continue;
+        const int ca = tile_owner(total, n, r0), cb = tile_owner(total, n, r1 - 1);
+        int32_t* ticket = p.tickets + static_cast<int64_t>(r) * p.hq + kvh;
+        if (lane == 0 && atomic_inc_acq_rel(ticket) == cb - ca) *ticket = 0;
+      }
+    }
+    __syncwarp();
+    for (int f = 0; f < 2; ++f) {
+      const int r = f == 0 ? fix_a : fix_b;
+      if (r < 0) continue;
+      const int r0 = s_prefix[r], r1 = s_prefix[r + 1];
+      combine_row<D>(p, r, kvh, total, n, tile_owner(total, n, r0), tile_owner(total, n, r1 - 1), r0, lane);
+    }
+    if (lane == 0) s_progress[warp] = stop;
+  }
+  // When a wait gave up, copies that were issued but not consumed may still land: wait for them before leaving.
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int lo = n_tiles;
+    for (int w = 0; w < HPC; ++w) lo = s_progress[w] < lo ? s_progress[w] : lo;
+    for (int j = lo; j < s_issued; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, p.status);
+  }
+}
+
+int encode_tiles(CUtensorMap* map, const void* layer, int total_pages, int page_size, int hkv, int d) {
+  auto encode = c8::get_encode();
+  if (encode == nullptr) return NQT_ERR_CUDA;
+  const cuuint64_t D = static_cast<cuuint64_t>(d);
+  cuuint64_t dims[4] = {D, static_cast<cuuint64_t>(hkv), static_cast<cuuint64_t>(page_size),
+                        static_cast<cuuint64_t>(total_pages) * 2};
+  cuuint64_t strides[3] = {D, static_cast<cuuint64_t>(hkv) * D, static_cast<cuuint64_t>(page_size) * hkv * D};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(d), 1, kBlock, 2};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r =
+      encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(layer), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? NQT_OK : NQT_ERR_CUDA;
+}
+
+template <int D, int HPC, int STAGES, bool E4M3>
+int launch8(const CUtensorMap& map, Decode8Args a, cudaStream_t s) {
+  using Cfg = Cfg8<D, HPC, STAGES>;
+  constexpr int kMaxSmem = Cfg::smem(kMaxRows8);
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaFuncSetAttribute(decode8_kernel<D, HPC, STAGES, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  });
+  const int smem = Cfg::smem(a.batch);
+  int occ = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, decode8_kernel<D, HPC, STAGES, E4M3>, Cfg::kThreads, smem) !=
+          cudaSuccess ||
+      occ < 1)
+    occ = 1;
+  const int groups = a.hkv / HPC;
+  int n = num_sms() * occ / groups;
+  n = n < 1 ? 1 : (n > kMaxCtas ? kMaxCtas : n);
+  a.n_ctas = n;
+  const cudaError_t err = launch_pdl(decode8_kernel<D, HPC, STAGES, E4M3>, dim3(n, groups), dim3(Cfg::kThreads), smem,
+                                     s, map, a);
+  if (err != cudaSuccess) {
+    set_last_error("decode_attention8", err);
+    return NQT_ERR_CUDA;
+  }
+  return NQT_OK;
+}
+
+template <int D, bool E4M3>
+int dispatch8(const CUtensorMap& map, const Decode8Args& a, cudaStream_t s) {
+  if (a.hkv % 4 == 0) return launch8<D, 4, 5, E4M3>(map, a, s);
+  if (a.hkv % 2 == 0) return launch8<D, 2, 6, E4M3>(map, a, s);
+  return launch8<D, 1, 8, E4M3>(map, a, s);
+}
+
+}  // namespace
+}  // namespace nqt
+
+using namespace nqt;
+
+extern "C" size_t nqt_decode8_workspace_bytes(int batch_capacity, int num_qo_heads, int head_dim) {
+  if (batch_capacity < 1 || num_qo_heads < 1 || head_dim < 1) return 0;
+  return ws8_layout(batch_capacity, num_qo_heads, head_dim).total;
+}
+
+extern "C" int nqt_decode_attention8(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                     const void* layer_cache, const float* layer_scales, int total_pages,
+                                     int page_size, const int32_t* kv_indptr, const int32_t* kv_indices,
+                                     const int32_t* last_page_len, int batch, int batch_capacity, int num_qo_heads,
+                                     int num_kv_heads, int head_dim, float sm_scale, int code, void* out,
+                                     int64_t out_stride_tok, int64_t out_stride_head, void* workspace,
+                                     size_t workspace_bytes, int flags, int32_t* status, void* stream) {
+  int rc = c8::check_layer(layer_cache, layer_scales, total_pages, page_size, num_kv_heads, head_dim, code);
+  if (rc != NQT_OK) return rc;
+  if (!q || !kv_indptr || !kv_indices || !last_page_len || !out || !workspace) return NQT_ERR_ARG;
+  if (batch < 0 || batch > batch_capacity || num_qo_heads < 1 || num_qo_heads % num_kv_heads) return NQT_ERR_ARG;
+  if (num_qo_heads / num_kv_heads > 8) return NQT_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(q) & 3) || (reinterpret_cast<uintptr_t>(out) & 3)) return NQT_ERR_ARG;
+  if ((q_stride_tok & 1) || (q_stride_head & 1) || (out_stride_tok & 1) || (out_stride_head & 1)) return NQT_ERR_ARG;
+  if (flags & ~(NQT_DECODE_OVERLAP_KV_WRITE | NQT_DECODE_SHORT_WAIT)) return NQT_ERR_ARG;
+  if (batch > kMaxRows8) return NQT_ERR_CAPACITY;
+  const Ws8 w = ws8_layout(batch_capacity, num_qo_heads, head_dim);
+  if (workspace_bytes < w.total) return NQT_ERR_CAPACITY;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return NQT_ERR_ARG;
+  if (batch == 0) return NQT_OK;
+  CUtensorMap map;
+  rc = encode_tiles(&map, layer_cache, total_pages, page_size, num_kv_heads, head_dim);
+  if (rc != NQT_OK) {
+    set_last_message("decode_attention8: cuTensorMapEncodeTiled failed");
+    return rc;
+  }
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  Decode8Args a{};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.q_st = q_stride_tok;
+  a.q_sh = q_stride_head;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.o_st = out_stride_tok;
+  a.o_sh = out_stride_head;
+  a.scales = layer_scales;
+  a.indptr = kv_indptr;
+  a.indices = kv_indices;
+  a.last_len = last_page_len;
+  a.tickets = reinterpret_cast<int32_t*>(base);
+  a.part_lse = reinterpret_cast<float*>(base + w.lse);
+  a.part_o = reinterpret_cast<float*>(base + w.o);
+  a.status = status;
+  a.batch = batch;
+  a.hq = num_qo_heads;
+  a.hkv = num_kv_heads;
+  a.group = num_qo_heads / num_kv_heads;
+  a.page_size = page_size;
+  a.total_pages = total_pages;
+  a.early = (flags & NQT_DECODE_OVERLAP_KV_WRITE) ? 1 : 0;
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.wait_ns = (flags & NQT_DECODE_SHORT_WAIT) ? 0 : kWaitLimitNs;
+  cudaStream_t s = as_stream(stream);
+  if (head_dim == 128)
+    return code == NQT_E4M3 ? dispatch8<128, true>(map, a, s) : dispatch8<128, false>(map, a, s);
+  return code == NQT_E4M3 ? dispatch8<64, true>(map, a, s) : dispatch8<64, false>(map, a, s);
+}

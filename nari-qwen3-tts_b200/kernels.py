@@ -290,7 +290,128 @@ def cp_decode_attention_(
     return output
 
 
+# ---------------------------------------------------------------- 8-bit paged KV cache
+CACHE_BLOCK = 16  # tokens of a page that share a scale
+
+
+def check_cache8(layer_cache: torch.Tensor, layer_scales: torch.Tensor, key_heads: int, head_dim: int) -> int:
+    """Validate one layer of an 8-bit paged cache: codes [pages, 2, P, Hkv, D] (int8 or float8_e4m3fn) and
+    scales float32 [pages, 2, P / 16, Hkv], both contiguous.  Returns the code type."""
+
+    code = _lib.cache_code(layer_cache.dtype)
+    if layer_cache.ndim != 5 or layer_cache.shape[1] != 2 or layer_cache.shape[3:] != (key_heads, head_dim):
+        raise ValueError("8-bit paged cache must be [pages, 2, page_size, kv_heads, head_dim]")
+    pages, _, page_size, _, _ = layer_cache.shape
+    if page_size % CACHE_BLOCK or not CACHE_BLOCK <= page_size <= 256:
+        raise ValueError("8-bit paged cache needs a page size that is a multiple of 16 up to 256")
+    if head_dim not in (64, 128):
+        raise ValueError("8-bit paged cache needs head_dim 64 or 128")
+    if layer_scales.dtype != torch.float32:
+        raise TypeError("8-bit paged cache scales must be float32")
+    if layer_scales.shape != (pages, 2, page_size // CACHE_BLOCK, key_heads):
+        raise ValueError("8-bit paged cache scales must be [pages, 2, page_size / 16, kv_heads]")
+    if not layer_cache.is_contiguous() or not layer_scales.is_contiguous():
+        raise ValueError("8-bit paged cache and its scales must be contiguous")
+    return code
+
+
+def paired_qk_norm_rope_paged_cache8(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    query_weight: torch.Tensor,
+    key_weight: torch.Tensor,
+    position_ids: torch.Tensor,
+    epsilon: float,
+    rope_theta: float,
+    layer_cache: torch.Tensor,
+    layer_scales: torch.Tensor,
+    write_pages: torch.Tensor,
+    write_offsets: torch.Tensor,
+    *,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """QK RMSNorm + RoPE with the quantised K/V write into an 8-bit paged cache; returns the rotated query.
+
+    The 8-bit counterpart of ``paired_qk_norm_rope_paged_cache_``: fp32 from the bf16 inputs to the codes and to
+    the bf16 query (no rounding between norm and rotation; angles exact at any position); query, key and value
+    are only read.  K and V are stored as code * scale with one scale per 16-token block, kind and head.  The
+    call's tokens of one block share its scale: their largest magnitude / the largest code (127 or 448) when
+    they start the block, else the block's scale, doubled until they fit, with the earlier tokens' codes rounded
+    again.  The tokens of one block have to follow one another in the call, at rising offsets, which is the
+    planner's order."""
+
+    if query.ndim != 3 or key.ndim != 3 or value.ndim != 3:
+        raise ValueError("Qwen3-TTS QKV tensors must have rank three")
+    tokens, query_heads, head_dim = query.shape
+    if key.shape != value.shape or key.shape[0] != tokens or key.shape[2] != head_dim:
+        raise ValueError("Qwen3-TTS QKV shapes are incompatible")
+    key_heads = key.shape[1]
+    if not (query.dtype == key.dtype == value.dtype == torch.bfloat16):
+        raise TypeError("8-bit paged staging takes bf16 query, key and value")
+    code = check_cache8(layer_cache, layer_scales, key_heads, head_dim)
+    if query_weight.shape != (head_dim,) or key_weight.shape != (head_dim,):
+        raise ValueError("QK norm weights must match the head dimension")
+    if position_ids.shape != (tokens,) or write_pages.shape != (tokens,) or write_offsets.shape != (tokens,):
+        raise ValueError("paged QKV metadata must contain one entry per token")
+    if query.stride(2) != 1 or key.stride(2) != 1 or value.stride(2) != 1:
+        raise ValueError("QKV must be contiguous per head")
+    for t in (position_ids, write_pages, write_offsets):
+        if t.dtype != torch.long or not t.is_contiguous():
+            raise TypeError("paged QKV metadata must be contiguous int64")
+    if out is not None and (out.shape != query.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1):
+        raise ValueError("the rotated query must be bf16 of the query's shape, contiguous per head")
+    device = _lib.require_cuda(query, key, value, query_weight, key_weight, position_ids, layer_cache, layer_scales,
+                               write_pages, write_offsets, out)
+    if out is None:
+        out = torch.empty((tokens, query_heads, head_dim), dtype=torch.bfloat16, device=device)
+    if tokens == 0:
+        return out
+    if query_weight.dtype != torch.bfloat16 or not query_weight.is_contiguous():
+        query_weight = query_weight.to(torch.bfloat16).contiguous()
+    if key_weight.dtype != torch.bfloat16 or not key_weight.is_contiguous():
+        key_weight = key_weight.to(torch.bfloat16).contiguous()
+    _lib.call_on(
+        device, "nqt_qk_norm_rope_paged_cache8",
+        query.data_ptr(), query.stride(0), query.stride(1),
+        key.data_ptr(), key.stride(0), key.stride(1),
+        value.data_ptr(), value.stride(0), value.stride(1),
+        query_weight.data_ptr(), key_weight.data_ptr(),
+        position_ids.data_ptr(), write_pages.data_ptr(), write_offsets.data_ptr(),
+        out.data_ptr(), out.stride(0), out.stride(1),
+        layer_cache.data_ptr(), layer_scales.data_ptr(), layer_cache.shape[0], layer_cache.shape[2],
+        tokens, query_heads, key_heads, head_dim,
+        float(epsilon), float(rope_theta), code, device_status(device).data_ptr(), _lib.stream_handle(device),
+    )
+    return out
+
+
+def read_paged_cache8(layer_cache: torch.Tensor, layer_scales: torch.Tensor, pages: torch.Tensor, *,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """Pages of an 8-bit cache layer as bf16 [n, 2, P, Hkv, D] (a bf16 pool's layout): to move a request's KV to
+    a bf16 pool or off the device.  ``pages``: int64 [n] page ids."""
+
+    if layer_cache.ndim != 5:
+        raise ValueError("8-bit paged cache must be [pages, 2, page_size, kv_heads, head_dim]")
+    code = check_cache8(layer_cache, layer_scales, layer_cache.shape[3], layer_cache.shape[4])
+    if pages.ndim != 1 or pages.dtype != torch.long or not pages.is_contiguous():
+        raise TypeError("page ids must be contiguous int64 [n]")
+    shape = (pages.shape[0], *layer_cache.shape[1:])
+    if out is not None and (out.shape != shape or out.dtype != torch.bfloat16 or not out.is_contiguous()):
+        raise ValueError("read_paged_cache8 output must be contiguous bf16 [n, 2, page_size, kv_heads, head_dim]")
+    device = _lib.require_cuda(layer_cache, layer_scales, pages, out)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    if pages.shape[0]:
+        _lib.call_on(device, "nqt_read_paged_cache8", layer_cache.data_ptr(), layer_scales.data_ptr(),
+                     layer_cache.shape[0], layer_cache.shape[2], layer_cache.shape[3], layer_cache.shape[4], code,
+                     pages.data_ptr(), pages.shape[0], out.data_ptr(), device_status(device).data_ptr(),
+                     _lib.stream_handle(device))
+    return out
+
+
 __all__ = [
+    "CACHE_BLOCK",
     "Fp8BlockWeight",
     "PackedWeight",
     "clear_status",
@@ -306,8 +427,10 @@ __all__ = [
     "fused_add_rmsnorm_fp8_",
     "linear",
     "linear_fp8",
+    "paired_qk_norm_rope_paged_cache8",
     "paired_qk_norm_rope_paged_cache_",
     "quantize_fp8_weight_blocks",
+    "read_paged_cache8",
     "read_status",
     "rmsnorm",
     "silu_and_mul",

@@ -38,7 +38,7 @@ import torch
 
 from . import _lib
 from ._lib import call, ptr
-from .kernels import device_status, paired_qk_norm_rope_paged_cache_
+from .kernels import check_cache8, device_status, paired_qk_norm_rope_paged_cache_
 
 # nqt_decode_attention_ex flags (include/nqt.h NQT_DECODE_OVERLAP_KV_WRITE, NQT_DECODE_SHORT_WAIT)
 DECODE_OVERLAP_KV_WRITE = 0x1
@@ -174,6 +174,85 @@ def batch_prefill_paged(
         float(sm_scale if sm_scale is not None else d**-0.5),
         ptr(out), out.stride(0), out.stride(1),
         ptr(device_status(device)), _lib.stream_handle(device),
+    )
+    return out
+
+
+def _check_paged8(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, rows, out):
+    if query.ndim != 3 or layer_cache.ndim != 5:
+        raise ValueError("8-bit paged attention takes query [tokens, heads, head_dim] and a rank-five cache")
+    _, hq, d = query.shape
+    hkv = layer_cache.shape[3]
+    if hq % hkv or hq // hkv > 8:
+        raise ValueError("8-bit paged attention needs 1 to 8 query heads per KV head")
+    if query.dtype != torch.bfloat16:
+        raise TypeError("8-bit paged attention runs on a bf16 query")
+    code = check_cache8(layer_cache, layer_scales, hkv, d)
+    if query.stride(2) != 1:
+        raise ValueError("query must be contiguous per head")
+    for t in (kv_indptr, kv_indices, last_page_len):
+        if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous():
+            raise TypeError("paged KV metadata must be contiguous int32")
+    if kv_indptr.shape[0] < rows + 1 or last_page_len.shape[0] < rows:
+        raise ValueError("paged KV metadata must cover every row")
+    if out is not None and (out.shape != query.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1):
+        raise ValueError("attention output must be bf16 of the query's shape, contiguous per head")
+    return code
+
+
+def decode_paged8_workspace(batch_capacity: int, num_qo_heads: int, head_dim: int,
+                            device: torch.device) -> torch.Tensor:
+    """The zeroed workspace of ``batch_decode_paged8`` for up to ``batch_capacity`` rows: make it once, outside
+    graph capture, and use it for one launch at a time."""
+
+    nbytes = _lib.lib().nqt_decode8_workspace_bytes(batch_capacity, num_qo_heads, head_dim)
+    if nbytes == 0:
+        raise ValueError("workspace dimensions must be positive")
+    return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+
+def batch_decode_paged8(
+    query: torch.Tensor,
+    layer_cache: torch.Tensor,
+    layer_scales: torch.Tensor,
+    kv_indptr: torch.Tensor,
+    kv_indices: torch.Tensor,
+    last_page_len: torch.Tensor,
+    workspace: torch.Tensor,
+    *,
+    batch_capacity: int | None = None,
+    sm_scale: float | None = None,
+    out: torch.Tensor | None = None,
+    overlap_kv_write: bool = False,
+    short_wait: bool = False,
+) -> torch.Tensor:
+    """``batch_decode_paged`` over an 8-bit cache (codes int8 or float8_e4m3fn with one fp32 scale per 16-token
+    block, kind and KV head; see kernels.paired_qk_norm_rope_paged_cache8).
+
+    There is no plan: the launch splits the batch itself.  ``workspace`` comes from ``decode_paged8_workspace``
+    for ``batch_capacity`` rows (default: this call's) and serves one launch at a time.  ``overlap_kv_write`` and
+    ``short_wait`` as in ``batch_decode_paged``; the scales of each row's last 16-token block count as its last
+    tile."""
+
+    rows = query.shape[0]
+    code = _check_paged8(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, rows, out)
+    device = _lib.require_cuda(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, workspace, out)
+    if out is None:
+        out = torch.empty(query.shape, dtype=torch.bfloat16, device=device)
+    if rows == 0:
+        return out
+    _, hq, d = query.shape
+    _lib.call_on(
+        device, "nqt_decode_attention8",
+        query.data_ptr(), query.stride(0), query.stride(1),
+        layer_cache.data_ptr(), layer_scales.data_ptr(), layer_cache.shape[0], layer_cache.shape[2],
+        kv_indptr.data_ptr(), kv_indices.data_ptr(), last_page_len.data_ptr(),
+        rows, batch_capacity or rows, hq, layer_cache.shape[3], d,
+        d**-0.5 if sm_scale is None else float(sm_scale), code,
+        out.data_ptr(), out.stride(0), out.stride(1),
+        workspace.data_ptr(), workspace.nbytes,
+        (DECODE_OVERLAP_KV_WRITE if overlap_kv_write else 0) | (DECODE_SHORT_WAIT if short_wait else 0),
+        device_status(device).data_ptr(), _lib.stream_handle(device),
     )
     return out
 
@@ -377,6 +456,8 @@ __all__ = [
     "TalkerAttentionContext",
     "TalkerAttentionMetadata",
     "batch_decode_paged",
+    "batch_decode_paged8",
     "batch_prefill_paged",
     "binding_factory",
+    "decode_paged8_workspace",
 ]
