@@ -610,6 +610,33 @@ int nqt_decode_attention8(
     float sm_scale, int code, void* out, int64_t out_stride_tok, int64_t out_stride_head,
     void* workspace, size_t workspace_bytes, int flags, int32_t* status, void* stream);
 
+/*
+ * W8A8 integer projection.  nqt_int8_quantize_rows: per row of bf16 x [m, k],
+ * scale = amax / 127 and q = round(x * 127 / amax) (a row of zeros has scale 0; a
+ * NaN or an infinity makes the row's scale NaN or infinite).  It serves tokens
+ * and, over a weight [n, k], output channels.  Any alignment and any k.
+ *
+ * nqt_gemm_int8: y[t, j] = (xq[t] . w[j]) * xscale[t] * wscale[j], int32 sums:
+ *   epilogue 0  y = bf16(.)          [m, cols], cols == n
+ *   epilogue 1  y = bf16(. + bias[j])
+ *   epilogue 2  w's rows in groups [16 gate | 16 up] (n a multiple of 32):
+ *               y[t, 16 g + i] = bf16(silu(gate) * up), the first cols <= n / 2
+ *               columns of it.
+ * Any m, n >= 1 and 1 <= k <= 131072; xq and w 16-byte aligned with row pitches
+ * (bytes) that are multiples of 16; y any row pitch.  No workspace.
+ *
+ * nqt_linear_int8: both for bf16 x, with xq [m, ldxq] and xscale [m] as scratch.
+ * Launched with programmatic stream serialization.
+ */
+int nqt_int8_quantize_rows(const void* x, int64_t ldx, int m, int k, void* q, int64_t ldq, float* scale,
+                           void* stream);
+int nqt_gemm_int8(const void* xq, int64_t ldxq, const float* xscale, const void* w, int64_t ldw, const float* wscale,
+                  const void* bias, void* y, int64_t ldy, int m, int n, int cols, int k, int epilogue,
+                  int32_t* status, void* stream);
+int nqt_linear_int8(const void* x, int64_t ldx, void* xq, int64_t ldxq, float* xscale, const void* w, int64_t ldw,
+                    const float* wscale, const void* bias, void* y, int64_t ldy, int m, int n, int cols, int k,
+                    int epilogue, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -116,6 +116,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         I,
         [P, L, L, P, P, I, I, P, P, P, I, I, I, I, I, F, I, P, L, L, P, Z, I, P, P],
     ),
+    "nqt_int8_quantize_rows": (I, [P, L, I, I, P, L, P, P]),
+    "nqt_gemm_int8": (I, [P, L, P, P, L, P, P, P, L, I, I, I, I, I, P, P]),
+    "nqt_linear_int8": (I, [P, L, P, L, P, P, L, P, P, P, L, I, I, I, I, I, P, P]),
     "nqt_step_stage": (I, [P, I, I, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P]),
     "nqt_talker_logits_mask": (I, [P, I, L, I, I, I, I, P, P]),
     "nqt_step_finish": (I, [P, I, I, P, I, P, P, P, P, L, P, P, P, P]),
@@ -170,6 +173,7 @@ def exported_symbols() -> list[str]:
 # kernels each entry point launches (nqt_plan_step adds the split-KV plan when given a workspace)
 KERNELS_PER_CALL = {
     "nqt_decode_attention_noalloc": 2,
+    "nqt_linear_int8": 2,
 }
 _launches = 0
 

@@ -1,0 +1,489 @@
+// W8A8 integer projections (sm_100a, tcgen05 kind::i8 + TMA): the quantiser of
+// activations and weights, and the product with its scales.
+//
+//   xs[t] = amax(x[t]) / 127,   xq[t] = round(x[t] * 127 / amax)       (per token)
+//   y[t, j] = (xq[t] . wq[j]) * xs[t] * ws[j] (+ bias[j])              (int32 sums, exact)
+// and for a gate_up weight y[t, j] = silu(g) * u with g, u the two halves'
+// columns, in fp32 up to the one rounding to bf16.  127^2 K < 2^31 holds up to
+// K = 131072, so no sum overflows.
+//
+// Quantiser.  A row's magnitudes are compared as integers (bf16 without its sign
+// bit orders like its value, and NaN above infinity), two per instruction; a NaN
+// makes the row's scale NaN, so it is not lost.
+//
+// Product.  A CTA computes 128 tokens x TN weight rows: one warp keeps a ring of
+// {128 bytes of K} TMA boxes of both operands full (128-byte swizzle; what lies
+// outside the matrices arrives as zeros, so any M, N and K work), one thread
+// issues tcgen05.mma with int32 accumulators in TMEM, four warps drain finished
+// tiles.  The grid is persistent and the accumulator double-buffered, so a tile's
+// epilogue runs under the next tile's products.  Tokens are the MMA's rows: an
+// epilogue thread owns one token, its scale is one register, the weights' scales
+// are broadcast from shared memory, and gate and up columns (interleaved in groups
+// of 16 rows when the weight is laid out) meet in the same thread.
+#include <mutex>
+
+#include "common.cuh"
+#include "gemm_common.cuh"
+#include "tcgen05.cuh"
+
+namespace nqt {
+namespace {
+
+using namespace gemm_detail;
+
+// ------------------------------------------------------------------ quantiser
+// One row by TPR threads; up to 4 vectors of 8 elements per thread stay in registers between the two passes,
+// longer rows are read again (from L2).
+template <int TPR, bool VEC>
+__global__ void __launch_bounds__(256) int8_quantize_rows_kernel(const __nv_bfloat16* x, int64_t ldx, int m, int k,
+                                                                 int8_t* q, int64_t ldq, float* scale) {
+  constexpr int kRows = 256 / TPR;
+  constexpr int kKeep = 4;
+  __shared__ uint32_t s_max[8];
+  grid_dependents_launch();
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
+  const int lt = threadIdx.x % TPR;
+  const bool live = row < m;
+  const __nv_bfloat16* src = x + (live ? row : 0) * ldx;
+  const int vecs = live ? (k + 7) / 8 : 0;
+
+  auto load = [&](int v) -> uint4 {
+    if (VEC) return *reinterpret_cast<const uint4*>(src + v * 8);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(src) + v * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (v * 8 + i < k) w[i / 2] |= static_cast<uint32_t>(e[i]) << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  auto magnitude = [](uint4 v, uint32_t m2) {
+    m2 = __vmaxu2(m2, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
+    return __vmaxu2(m2, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+  };
+  uint4 keep[kKeep];
+  uint32_t m2 = 0;
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int v = lt + i * TPR;
+    keep[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (v < vecs) keep[i] = load(v);
+    m2 = magnitude(keep[i], m2);
+  }
+  for (int v = lt + kKeep * TPR; v < vecs; v += TPR) m2 = magnitude(load(v), m2);
+  uint32_t mx = max(m2 & 0xffffu, m2 >> 16);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(kFull, mx, o));
+  if (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) mx = max(mx, s_max[w]);
+  }
+  if (!live) return;
+  const float amax = __uint_as_float(mx << 16);
+  const float s = __fdiv_rn(amax, 127.f);
+  const float f = amax == 0.f ? 0.f : __fdiv_rn(127.f, amax);
+  const bool tiny = f > 3.0e38f;  // 127 / amax overflows: divide by the (subnormal) scale instead
+  if (lt == 0) scale[row] = s;
+  auto code = [&](uint32_t bf16_bits) -> uint32_t {
+    const float v = __uint_as_float(bf16_bits << 16);
+    const float t = tiny ? fminf(fmaxf(__fdiv_rn(v, s), -127.f), 127.f) : v * f;
+    return static_cast<uint32_t>(__float2int_rn(t)) & 0xffu;
+  };
+  auto store = [&](int v, uint4 w) {
+    uint32_t lo = code(w.x & 0xffffu) | (code(w.x >> 16) << 8) | (code(w.y & 0xffffu) << 16) | (code(w.y >> 16) << 24);
+    uint32_t hi = code(w.z & 0xffffu) | (code(w.z >> 16) << 8) | (code(w.w & 0xffffu) << 16) | (code(w.w >> 16) << 24);
+    int8_t* dst = q + row * ldq + v * 8;
+    if (VEC) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (v * 8 + i < k) dst[i] = static_cast<int8_t>(((i < 4 ? lo : hi) >> (8 * (i & 3))) & 0xffu);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i)
+    if (lt + i * TPR < vecs) store(lt + i * TPR, keep[i]);
+  for (int v = lt + kKeep * TPR; v < vecs; v += TPR) store(v, load(v));
+}
+
+// ------------------------------------------------------------------ product
+constexpr int kTileM = 128;   // tokens per tile (MMA M)
+constexpr int kBlockK = 128;  // bytes of K per stage
+constexpr int kThreads = 6 * 32;
+constexpr int kABytes = kTileM * kBlockK;
+
+enum Epilogue : int { kPlain = 0, kBias = 1, kSiluMul = 2 };  // the numbering of nqt_gemm_bf16
+
+struct Int8Args {
+  const float *xscale, *wscale;
+  const __nv_bfloat16* bias;
+  __nv_bfloat16* y;
+  int64_t ldy;
+  int32_t* status;
+  int m, n, cols, kb;  // cols: output columns; kb: K blocks
+  int m_tiles, tiles;
+  int epilogue;
+  int early;  // the weights may be read before the previous kernel has finished
+  int vec16;  // y rows allow 16-byte stores
+};
+
+template <int TN>
+struct CfgI8 {
+  static constexpr int kBBytes = TN * kBlockK;
+  static constexpr int kStage = kABytes + kBBytes;
+  static constexpr int kStages = TN == 256 ? 4 : (TN == 128 ? 6 : 8);
+  static constexpr uint32_t kTmemCols = 2 * TN < 32 ? 32 : 2 * TN;
+  static constexpr int kSmem = 1024 + kStages * kStage + 2 * TN * 4 * 2 + (2 * kStages + 4) * 8 + 32;
+};
+
+__device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor, kind::i8: s32 accumulate (bits 4-5 = 2), s8 A and B (bits 7-9 and 10-12 = 1), K-major.
+__host__ __device__ constexpr uint32_t idesc_s8_s32(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+// 32 accumulators of one token -> outputs, stored at column `col` of row y (plain, bias) or col / 2 (gate and up
+// columns in groups of 16).  `sw`, `sb`: the columns' scales and biases in shared memory.
+__device__ __forceinline__ void finish_32(const Int8Args& a, const uint32_t (&r)[32], float sx, const float* sw,
+                                          const float* sb, __nv_bfloat16* yrow, int col) {
+  float v[32];
+#pragma unroll
+  for (int e = 0; e < 32; e += 4) {
+    const float4 w = *reinterpret_cast<const float4*>(sw + e);
+    v[e] = static_cast<float>(static_cast<int32_t>(r[e])) * (sx * w.x);
+    v[e + 1] = static_cast<float>(static_cast<int32_t>(r[e + 1])) * (sx * w.y);
+    v[e + 2] = static_cast<float>(static_cast<int32_t>(r[e + 2])) * (sx * w.z);
+    v[e + 3] = static_cast<float>(static_cast<int32_t>(r[e + 3])) * (sx * w.w);
+  }
+  int count = 32, out0 = col;
+  if (a.epilogue == kBias) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] += sb[e];
+  } else if (a.epilogue == kSiluMul) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = silu_mul(v[e], v[e + 16]);
+    count = 16;
+    out0 = col / 2;
+  }
+  const int left = a.cols - out0;
+  if (a.vec16 && left >= count) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 8) {
+      if (e >= count) break;
+      *reinterpret_cast<uint4*>(yrow + out0 + e) =
+          make_uint4(pack_bf16x2(v[e], v[e + 1]), pack_bf16x2(v[e + 2], v[e + 3]), pack_bf16x2(v[e + 4], v[e + 5]),
+                     pack_bf16x2(v[e + 6], v[e + 7]));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (e < count && e < left) yrow[out0 + e] = __float2bfloat16_rn(v[e]);
+  }
+}
+
+template <int TN>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_int8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, Int8Args a) {
+  using Cfg = CfgI8<TN>;
+  constexpr int ST = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* s_sw = reinterpret_cast<float*>(smem + ST * Cfg::kStage);  // [2][TN] scales, then [2][TN] biases
+  float* s_sb = s_sw + 2 * TN;
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_sb + 2 * TN);
+  uint64_t* empty = full + ST;
+  uint64_t* accf = empty + ST;  // [2] accumulator complete
+  uint64_t* acce = accf + 2;    // [2] accumulator read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acce + 2);
+  volatile int* s_issued = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* s_consumed = s_issued + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accf[b], 1);
+      mbar_init(&acce[b], 4);
+    }
+    fence_barrier_init();
+    *s_issued = 0;
+    *s_consumed = 0;
+    prefetch_tensormap(&xmap);
+    prefetch_tensormap(&wmap);
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependents_launch();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      // the first stages' weights do not depend on the previous kernel when the caller says so
+      int ahead = 0;
+      if (a.early && blockIdx.x < a.tiles) {
+        const int n0 = static_cast<int>(blockIdx.x) / a.m_tiles * TN;
+        ahead = a.kb < ST ? a.kb : ST;
+        for (int i = 0; i < ahead; ++i) {
+          mbar_arrive_expect_tx(&full[i], Cfg::kStage);
+          tma_load_2d(smem + i * Cfg::kStage + kABytes, &wmap, &full[i], i * kBlockK, n0);
+        }
+      }
+      grid_dependency_wait();
+      for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
+        const int m0 = tile % a.m_tiles * kTileM, n0 = tile / a.m_tiles * TN;
+        for (int kb = 0; kb < a.kb; ++kb, ++it) {
+          const int s = it % ST;
+          if (it >= ST && !mbar_wait(&empty[s], ((it / ST) - 1) & 1, a.status)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * Cfg::kStage;
+          if (it >= ahead) {
+            mbar_arrive_expect_tx(&full[s], Cfg::kStage);
+            tma_load_2d(st + kABytes, &wmap, &full[s], kb * kBlockK, n0);
+          }
+          tma_load_2d(st, &xmap, &full[s], kb * kBlockK, m0);
+          *s_issued = it + 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_s8_s32(kTileM, TN);
+      const uint64_t a_desc = tc::smem_desc_sw128(smem_addr(smem), 16, 1024);
+      const uint64_t b_desc = tc::smem_desc_sw128(smem_addr(smem + kABytes), 16, 1024);
+      int it = 0, t = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, ++t) {
+        const int buf = t & 1;
+        if (t >= 2 && !mbar_wait(&acce[buf], ((t >> 1) - 1) & 1, a.status)) break;
+        tc::fence_after_sync();
+        for (int kb = 0; kb < a.kb; ++kb, ++it) {
+          const int s = it % ST;
+          if (!mbar_wait(&full[s], (it / ST) & 1, a.status)) {
+            ok = false;
+            break;
+          }
+          *s_consumed = it + 1;
+          tc::fence_after_sync();
+          const uint32_t off = static_cast<uint32_t>(s * Cfg::kStage) >> 4;
+#pragma unroll
+          for (int kk = 0; kk < kBlockK / 32; ++kk)
+            mma_i8_ss(tmem + buf * TN, a_desc + off + kk * 2, b_desc + off + kk * 2, idesc, (kb | kk) ? 1u : 0u);
+          tc::commit(&empty[s]);
+        }
+        if (ok) tc::commit(&accf[buf]);
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    const int et = threadIdx.x - 64;
+    grid_dependency_wait();  // the tokens' scales, and y, which the previous kernel may still read
+    int t = 0;
+    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++t) {
+      const int buf = t & 1;
+      const int m0 = tile % a.m_tiles * kTileM, n0 = tile / a.m_tiles * TN;
+      float* sw = s_sw + buf * TN;
+      float* sb = s_sb + buf * TN;
+      for (int i = et; i < TN; i += 128) {
+        sw[i] = n0 + i < a.n ? __ldg(a.wscale + n0 + i) : 0.f;
+        if (a.epilogue == kBias) sb[i] = n0 + i < a.n ? __bfloat162float(a.bias[n0 + i]) : 0.f;
+      }
+      const int tok = m0 + quarter * 32 + lane;
+      const float sx = tok < a.m ? a.xscale[tok] : 0.f;
+      epi_bar();  // also: everybody is done with this buffer's scales of two tiles ago
+      if (!mbar_wait(&accf[buf], (t >> 1) & 1, a.status)) break;
+      tc::fence_after_sync();
+      const uint32_t src = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * TN;
+      __nv_bfloat16* yrow = a.y + static_cast<int64_t>(tok) * a.ldy;
+      const bool live_warp = m0 + quarter * 32 < a.m;
+#pragma unroll 1
+      for (int c = 0; c < TN; c += 32) {
+        uint32_t r[32];
+        if (live_warp) {
+          tc::ld_32x32b_x32(src + c, r);
+          tc::wait_ld();
+        }
+        if (c + 32 >= TN) {
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acce[buf]);
+        }
+        if (tok < a.m && n0 + c < a.n) finish_32(a, r, sx, sw + c, sb + c, yrow, n0 + c);
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (threadIdx.x == 0)  // after a wait that gave up: copies still in flight land before the CTA leaves
+    for (int i = *s_consumed; i < *s_issued; ++i) mbar_wait(&full[i % ST], (i / ST) & 1, a.status);
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, Cfg::kTmemCols);
+  }
+}
+
+// An int8 matrix [rows, k] (row pitch ld bytes) in boxes of {128 bytes, box_rows}, 128-byte swizzle, zeros outside.
+int encode_i8(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t ld, int box_rows) {
+  auto encode = get_encode();
+  if (encode == nullptr) return NQT_ERR_CUDA;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+  cuuint32_t box[2] = {kBlockK, static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? NQT_OK : NQT_ERR_CUDA;
+}
+
+template <int TN>
+int launch_i8(const void* xq, int64_t ldxq, const void* w, int64_t ldw, int k, Int8Args a, cudaStream_t s) {
+  using Cfg = CfgI8<TN>;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaFuncSetAttribute(gemm_int8_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+  });
+  CUtensorMap xmap, wmap;
+  if (encode_i8(&xmap, xq, a.m, k, ldxq, kTileM) != NQT_OK || encode_i8(&wmap, w, a.n, k, ldw, TN) != NQT_OK) {
+    set_last_message("gemm_int8: cuTensorMapEncodeTiled failed");
+    return NQT_ERR_CUDA;
+  }
+  a.m_tiles = (a.m + kTileM - 1) / kTileM;
+  const int64_t tiles = static_cast<int64_t>(a.m_tiles) * ((a.n + TN - 1) / TN);
+  if (tiles > 0x3fffffff) return NQT_ERR_UNSUPPORTED;
+  a.tiles = static_cast<int>(tiles);
+  const int sms = num_sms();
+  // one CTA per SM: the shared memory of two would fit for small TN, but TMEM and the ring are sized for one
+  const int grid = a.tiles < sms ? a.tiles : sms;
+  const cudaError_t err = launch_pdl(gemm_int8_kernel<TN>, dim3(grid), dim3(kThreads), Cfg::kSmem, s, xmap, wmap, a);
+  if (err != cudaSuccess) {
+    set_last_error("gemm_int8", err);
+    return NQT_ERR_CUDA;
+  }
+  return NQT_OK;
+}
+
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+int check_gemm(const void* xq, int64_t ldxq, const float* xscale, const void* w, int64_t ldw, const float* wscale,
+               const void* bias, const void* y, int64_t ldy, int m, int n, int cols, int k, int epilogue) {
+  if (!w || !wscale || !y || m < 0 || n < 1 || k < 1 || cols < 1) return NQT_ERR_ARG;
+  if (epilogue != kPlain && epilogue != kBias && epilogue != kSiluMul) return NQT_ERR_ARG;
+  if (epilogue == kBias && !bias) return NQT_ERR_ARG;
+  if (epilogue == kSiluMul ? (n % 32 != 0 || cols > n / 2) : cols != n) return NQT_ERR_ARG;
+  if (k > 131072) return NQT_ERR_UNSUPPORTED;  // the int32 sums could overflow
+  if (!xq || !xscale || !aligned(xq, 16) || ldxq % 16 || ldxq < k) return NQT_ERR_ARG;
+  if (!aligned(w, 16) || ldw % 16 || ldw < k || ldy < cols || !aligned(y, 2)) return NQT_ERR_ARG;
+  return NQT_OK;
+}
+
+int run_gemm(const void* xq, int64_t ldxq, const float* xscale, const void* w, int64_t ldw, const float* wscale,
+             const void* bias, void* y, int64_t ldy, int m, int n, int cols, int k, int epilogue, int early,
+             int32_t* status, cudaStream_t s) {
+  Int8Args a{};
+  a.xscale = xscale;
+  a.wscale = wscale;
+  a.bias = static_cast<const __nv_bfloat16*>(bias);
+  a.y = static_cast<__nv_bfloat16*>(y);
+  a.ldy = ldy;
+  a.status = status;
+  a.m = m;
+  a.n = n;
+  a.cols = cols;
+  a.kb = (k + kBlockK - 1) / kBlockK;
+  a.epilogue = epilogue;
+  a.early = early;
+  a.vec16 = aligned(y, 16) && ldy % 8 == 0;
+  // the widest tile that still gives every SM one
+  const int64_t m_tiles = (m + kTileM - 1) / kTileM;
+  const int64_t sms = num_sms();
+  auto tiles = [&](int tn) { return m_tiles * ((n + tn - 1) / tn); };
+  if (tiles(256) >= sms) return launch_i8<256>(xq, ldxq, w, ldw, k, a, s);
+  if (tiles(128) >= sms) return launch_i8<128>(xq, ldxq, w, ldw, k, a, s);
+  if (tiles(64) >= sms) return launch_i8<64>(xq, ldxq, w, ldw, k, a, s);
+  return launch_i8<32>(xq, ldxq, w, ldw, k, a, s);
+}
+
+int run_quantize(const void* x, int64_t ldx, int m, int k, void* q, int64_t ldq, float* scale, cudaStream_t s) {
+  const bool vec = aligned(x, 16) && ldx % 8 == 0 && k % 8 == 0 && aligned(q, 8) && ldq % 8 == 0;
+  const __nv_bfloat16* xp = static_cast<const __nv_bfloat16*>(x);
+  int8_t* qp = static_cast<int8_t*>(q);
+  // a warp per row keeps rows of up to 1024 elements in registers; longer rows get a whole CTA
+  if (k <= 1024) {
+    const unsigned grid = (static_cast<unsigned>(m) + 7) / 8;
+    if (vec) int8_quantize_rows_kernel<32, true><<<grid, 256, 0, s>>>(xp, ldx, m, k, qp, ldq, scale);
+    else int8_quantize_rows_kernel<32, false><<<grid, 256, 0, s>>>(xp, ldx, m, k, qp, ldq, scale);
+  } else {
+    if (vec) int8_quantize_rows_kernel<256, true><<<m, 256, 0, s>>>(xp, ldx, m, k, qp, ldq, scale);
+    else int8_quantize_rows_kernel<256, false><<<m, 256, 0, s>>>(xp, ldx, m, k, qp, ldq, scale);
+  }
+  return check_launch("int8_quantize_rows");
+}
+
+}  // namespace
+}  // namespace nqt
+
+using namespace nqt;
+
+extern "C" int nqt_int8_quantize_rows(const void* x, int64_t ldx, int m, int k, void* q, int64_t ldq, float* scale,
+                                      void* stream) {
+  if (!x || !q || !scale || m < 0 || k < 1 || ldx < k || ldq < k || !aligned(x, 2) || !aligned(scale, 4))
+    return NQT_ERR_ARG;
+  if (m == 0) return NQT_OK;
+  return run_quantize(x, ldx, m, k, q, ldq, scale, as_stream(stream));
+}
+
+extern "C" int nqt_gemm_int8(const void* xq, int64_t ldxq, const float* xscale, const void* w, int64_t ldw,
+                             const float* wscale, const void* bias, void* y, int64_t ldy, int m, int n, int cols,
+                             int k, int epilogue, int32_t* status, void* stream) {
+  const int rc = check_gemm(xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue);
+  if (rc != NQT_OK) return rc;
+  if (m == 0) return NQT_OK;
+  return run_gemm(xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue, 0, status,
+                  as_stream(stream));
+}
+
+extern "C" int nqt_linear_int8(const void* x, int64_t ldx, void* xq, int64_t ldxq, float* xscale, const void* w,
+                               int64_t ldw, const float* wscale, const void* bias, void* y, int64_t ldy, int m, int n,
+                               int cols, int k, int epilogue, int32_t* status, void* stream) {
+  const int rc = check_gemm(xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue);
+  if (rc != NQT_OK) return rc;
+  if (!x || ldx < k || !aligned(x, 2)) return NQT_ERR_ARG;
+  if (m == 0) return NQT_OK;
+  cudaStream_t s = as_stream(stream);
+  const int rq = run_quantize(x, ldx, m, k, xq, ldxq, xscale, s);
+  if (rq != NQT_OK) return rq;
+  // the quantiser is an ordinary launch: what came before it has finished, so the weights can be read at once
+  return run_gemm(xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue, 1, status, s);
+}

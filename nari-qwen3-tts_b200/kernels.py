@@ -413,6 +413,7 @@ def read_paged_cache8(layer_cache: torch.Tensor, layer_scales: torch.Tensor, pag
 __all__ = [
     "CACHE_BLOCK",
     "Fp8BlockWeight",
+    "Int8Weight",
     "PackedWeight",
     "clear_status",
     "cp_codec_step",
@@ -425,8 +426,10 @@ __all__ = [
     "fp8_quantize_rows",
     "fused_add_rmsnorm_",
     "fused_add_rmsnorm_fp8_",
+    "int8_quantize_rows",
     "linear",
     "linear_fp8",
+    "linear_int8",
     "paired_qk_norm_rope_paged_cache8",
     "paired_qk_norm_rope_paged_cache_",
     "quantize_fp8_weight_blocks",
@@ -694,4 +697,139 @@ def linear_fp8(xq: torch.Tensor, xscale: torch.Tensor, weight: Fp8BlockWeight, *
          ptr(out), out.stride(0), m, weight.n, weight.k, epilogue, 1 if weight.gate_up else 0, int(split),
          ptr(workspace), 0 if workspace is None else workspace.numel(), ptr(device_status(xq.device)),
          _lib.stream_handle(xq.device))
+    return out
+
+
+# ---------------------------------------------------------------- W8A8 integer projections
+def int8_quantize_rows(x: torch.Tensor, *, out: torch.Tensor | None = None,
+                       scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per row of bf16 x [m, k]: scale = amax / 127, q = round(x * 127 / amax) - the tokens' rule and, over a
+    weight [n, k], the output channels'.  Returns (q int8 [m, k] with a row pitch that is a multiple of 16,
+    scale float32 [m]).  A NaN or an infinity in a row shows in its scale."""
+
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError("int8_quantize_rows takes bf16 [m, k] with unit stride along k")
+    m, k = x.shape
+    if k < 1:
+        raise ValueError("int8_quantize_rows needs k >= 1")
+    if out is not None and (out.shape != (m, k) or out.dtype != torch.int8 or out.stride(1) != 1):
+        raise ValueError("int8_quantize_rows output must be int8 [m, k] with unit column stride")
+    if scale is not None and (scale.shape != (m,) or scale.dtype != torch.float32 or not scale.is_contiguous()):
+        raise ValueError("int8_quantize_rows scale must be contiguous float32 [m]")
+    device = _lib.require_cuda(x, out, scale)
+    if out is None:
+        out = torch.empty((m, (k + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :k]
+    if scale is None:
+        scale = torch.empty(m, dtype=torch.float32, device=device)
+    _lib.call_on(device, "nqt_int8_quantize_rows", x.data_ptr(), _row_pitch(x), m, k, out.data_ptr(), _row_pitch(out),
+                 scale.data_ptr(), _lib.stream_handle(device))
+    return out, scale
+
+
+def _row_pitch(t: torch.Tensor) -> int:
+    """Row stride of a matrix in elements; a single row's stride says nothing."""
+
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), (t.shape[1] + 15) // 16 * 16)
+
+
+class Int8Weight:
+    """A weight [n, k] in int8 with one scale per output channel, laid out once for linear_int8.
+
+    From a bf16 weight the rule is int8_quantize_rows's; ``from_quantized`` takes codes and scales that exist.
+    ``q`` [n, k] and ``scale`` [n] keep the channel order.  With ``gate_up`` the rows are [gate | up] halves: the
+    copy that the product reads interleaves them in groups of 16, each half padded to a multiple of 16 rows."""
+
+    def __init__(self, weight: torch.Tensor, *, gate_up: bool = False) -> None:
+        if weight.dim() != 2 or weight.dtype != torch.bfloat16:
+            raise ValueError("an int8 weight is made from a bf16 [n, k] matrix")
+        self._lay_out(*int8_quantize_rows(weight), gate_up)
+
+    @classmethod
+    def from_quantized(cls, q: torch.Tensor, scale: torch.Tensor, *, gate_up: bool = False) -> Int8Weight:
+        if q.dim() != 2 or q.dtype != torch.int8:
+            raise ValueError("quantised weights are int8 [n, k]")
+        if scale.shape != (q.shape[0],) or scale.dtype != torch.float32:
+            raise ValueError("quantised weights need a float32 scale per row")
+        _lib.require_cuda(q, scale)
+        self = cls.__new__(cls)
+        self._lay_out(q, scale, gate_up)
+        return self
+
+    def _lay_out(self, q: torch.Tensor, scale: torch.Tensor, gate_up: bool) -> None:
+        n, k = q.shape
+        if n < 1 or not 1 <= k <= 131072:
+            raise ValueError("int8 weights need n >= 1 and 1 <= k <= 131072 (int32 sums)")
+        if gate_up and n % 2:
+            raise ValueError("a gate_up weight has an even number of rows")
+        self.q, self.scale = q, scale
+        self.n, self.k, self.gate_up = n, k, gate_up
+        self.cols = n // 2 if gate_up else n
+        pitch = (k + 15) // 16 * 16
+        if gate_up:
+            half = n // 2
+            groups = (half + 15) // 16
+            data = torch.zeros((2, groups * 16, pitch), dtype=torch.int8, device=q.device)
+            data[:, :half, :k] = q.view(2, half, k) if q.is_contiguous() else torch.stack([q[:half], q[half:]])
+            self.data = data.view(2, groups, 16, pitch).transpose(0, 1).reshape(-1, pitch)
+            scales = torch.zeros((2, groups * 16), dtype=torch.float32, device=q.device)
+            scales[:, :half] = scale.view(2, half)
+            self.data_scale = scales.view(2, groups, 16).transpose(0, 1).reshape(-1)
+        elif q.stride(1) == 1 and _row_pitch(q) % 16 == 0 and _row_pitch(q) >= k and q.data_ptr() % 16 == 0:
+            self.data, self.data_scale = q, scale.contiguous()
+        else:
+            self.data = torch.zeros((n, pitch), dtype=torch.int8, device=q.device)
+            self.data[:, :k] = q
+            self.data_scale = scale.contiguous()
+        self.rows, self.pitch = self.data.shape[0], _row_pitch(self.data)
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return (self.n, self.k)
+
+
+def linear_int8(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None = None, *,
+                xscale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """W8A8 projection: (xq . wq^T) * xscale[t] * wscale[j] (+ bias) with exact int32 sums, bf16 out [m, n]; a
+    ``gate_up`` weight gives silu(gate) * up, [m, n / 2].
+
+    ``x``: bf16 [m, k], quantised per token on the way (the int8_quantize_rows rule), or int8 codes with their
+    ``xscale`` (float32 [m]) and a row pitch that is a multiple of 16."""
+
+    if not isinstance(weight, Int8Weight):
+        raise TypeError("linear_int8 takes an Int8Weight")
+    if x.dim() != 2 or x.shape[1] != weight.k or (x.stride(1) != 1 and weight.k > 1):
+        raise ValueError("linear_int8 needs x [m, k] matching the weight, with unit stride along k")
+    m, k = x.shape
+    if bias is not None:
+        if weight.gate_up:
+            raise ValueError("the silu_mul epilogue takes no bias")
+        if bias.dtype != torch.bfloat16 or bias.shape != (weight.n,) or not bias.is_contiguous():
+            raise ValueError("linear_int8 bias must be contiguous bf16 [n]")
+    if out is not None and (out.shape != (m, weight.cols) or out.dtype != torch.bfloat16
+                            or (out.stride(1) != 1 and weight.cols > 1)):
+        raise ValueError("linear_int8 output must be bf16 [m, n] with unit column stride")
+    epilogue = GEMM_SILU_MUL if weight.gate_up else (GEMM_PLAIN if bias is None else GEMM_BIAS)
+    device = _lib.require_cuda(x, weight.data, bias, xscale, out)
+    if out is None:
+        out = torch.empty((m, weight.cols), dtype=torch.bfloat16, device=device)
+    if m == 0:
+        return out
+    tail = (weight.data.data_ptr(), weight.pitch, weight.data_scale.data_ptr(), ptr(bias), out.data_ptr(),
+            _row_pitch(out), m, weight.rows, weight.cols, k, epilogue, device_status(device).data_ptr(),
+            _lib.stream_handle(device))
+    if x.dtype == torch.bfloat16:
+        if xscale is not None:
+            raise ValueError("xscale belongs to int8 codes")
+        pitch = (k + 15) // 16 * 16
+        scratch = torch.empty(m * (pitch + 4), dtype=torch.uint8, device=device)
+        codes = scratch.data_ptr()
+        _lib.call_on(device, "nqt_linear_int8", x.data_ptr(), _row_pitch(x), codes, pitch, codes + m * pitch, *tail)
+        return out
+    if x.dtype != torch.int8 or xscale is None:
+        raise TypeError("linear_int8 takes bf16 rows, or int8 codes with their xscale")
+    if xscale.dtype != torch.float32 or xscale.shape != (m,) or not xscale.is_contiguous():
+        raise ValueError("linear_int8 xscale must be contiguous float32 [m]")
+    if _row_pitch(x) % 16 or x.data_ptr() % 16:
+        raise ValueError("linear_int8 codes need 16-byte aligned rows")
+    _lib.call_on(device, "nqt_gemm_int8", x.data_ptr(), _row_pitch(x), xscale.data_ptr(), *tail)
     return out
