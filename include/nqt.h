@@ -611,6 +611,24 @@ int nqt_decode_attention8(
     void* workspace, size_t workspace_bytes, int flags, int32_t* status, void* stream);
 
 /*
+ * Ragged causal prefill attention over an 8-bit layer: nqt_prefill_attention's
+ * contract for head_dim 64 and 128, any num_qo_heads / num_kv_heads <= 8 and
+ * sm_scale >= 0.  q 16-byte aligned with strides that are multiples of 8; out any
+ * alignment (16-byte aligned rows leave faster).  Queries that see no key, and
+ * rows without pages, give zeros; tokens behind qo_indptr[batch] are left as
+ * they are.  No workspace: when the query tiles do not fill the GPU, clusters
+ * of CTAs share the keys of one tile and join in shared memory.
+ */
+int nqt_prefill_attention8(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+    const void* layer_cache, const float* layer_scales, int total_pages, int page_size,
+    const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+    const int32_t* last_page_len,
+    int batch, int total_q_tokens, int num_qo_heads, int num_kv_heads, int head_dim,
+    float sm_scale, int code, void* out, int64_t out_stride_tok, int64_t out_stride_head,
+    int32_t* status, void* stream);
+
+/*
  * W8A8 integer projection.  nqt_int8_quantize_rows: per row of bf16 x [m, k],
  * scale = amax / 127 and q = round(x * 127 / amax) (a row of zeros has scale 0; a
  * NaN or an infinity makes the row's scale NaN or infinite).  It serves tokens

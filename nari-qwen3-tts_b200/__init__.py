@@ -33,6 +33,7 @@ from .talker_kv import (
     batch_decode_paged,
     batch_decode_paged8,
     batch_prefill_paged,
+    batch_prefill_paged8,
     binding_factory,
     decode_paged8_workspace,
 )
@@ -48,6 +49,7 @@ __all__ = [
     "batch_decode_paged",
     "batch_decode_paged8",
     "batch_prefill_paged",
+    "batch_prefill_paged8",
     "binding_factory",
     "cp_decode_attention_",
     "decode_attn_nhd_short_cache",

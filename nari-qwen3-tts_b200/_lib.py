@@ -116,6 +116,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         I,
         [P, L, L, P, P, I, I, P, P, P, I, I, I, I, I, F, I, P, L, L, P, Z, I, P, P],
     ),
+    "nqt_prefill_attention8": (
+        I,
+        [P, L, L, P, P, I, I, P, P, P, P, I, I, I, I, I, F, I, P, L, L, P, P],
+    ),
     "nqt_int8_quantize_rows": (I, [P, L, I, I, P, L, P, P]),
     "nqt_gemm_int8": (I, [P, L, P, P, L, P, P, P, L, I, I, I, I, I, P, P]),
     "nqt_linear_int8": (I, [P, L, P, L, P, P, L, P, P, P, L, I, I, I, I, I, P, P]),

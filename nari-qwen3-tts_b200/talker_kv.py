@@ -200,6 +200,11 @@ def _check_paged8(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_
     return code
 
 
+def _table_ptr(kv_indices: torch.Tensor, kv_indptr: torch.Tensor) -> int:
+    # no row has a page: the empty table has no address, and nothing reads one
+    return kv_indices.data_ptr() if kv_indices.numel() else kv_indptr.data_ptr()
+
+
 def decode_paged8_workspace(batch_capacity: int, num_qo_heads: int, head_dim: int,
                             device: torch.device) -> torch.Tensor:
     """The zeroed workspace of ``batch_decode_paged8`` for up to ``batch_capacity`` rows: make it once, outside
@@ -246,12 +251,58 @@ def batch_decode_paged8(
         device, "nqt_decode_attention8",
         query.data_ptr(), query.stride(0), query.stride(1),
         layer_cache.data_ptr(), layer_scales.data_ptr(), layer_cache.shape[0], layer_cache.shape[2],
-        kv_indptr.data_ptr(), kv_indices.data_ptr(), last_page_len.data_ptr(),
+        kv_indptr.data_ptr(), _table_ptr(kv_indices, kv_indptr), last_page_len.data_ptr(),
         rows, batch_capacity or rows, hq, layer_cache.shape[3], d,
         d**-0.5 if sm_scale is None else float(sm_scale), code,
         out.data_ptr(), out.stride(0), out.stride(1),
         workspace.data_ptr(), workspace.nbytes,
         (DECODE_OVERLAP_KV_WRITE if overlap_kv_write else 0) | (DECODE_SHORT_WAIT if short_wait else 0),
+        device_status(device).data_ptr(), _lib.stream_handle(device),
+    )
+    return out
+
+
+def batch_prefill_paged8(
+    query: torch.Tensor,
+    layer_cache: torch.Tensor,
+    layer_scales: torch.Tensor,
+    qo_indptr: torch.Tensor,
+    kv_indptr: torch.Tensor,
+    kv_indices: torch.Tensor,
+    last_page_len: torch.Tensor,
+    *,
+    batch: int | None = None,
+    sm_scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``batch_prefill_paged`` over an 8-bit cache: ragged causal chunks, query i of a chunk of n sees the keys up
+    to kv_len - n + i.  Queries that see no key give zeros; tokens behind ``qo_indptr[batch]`` are not written.  A
+    query whose rows are not 16-byte aligned is copied first."""
+
+    rows = batch if batch is not None else qo_indptr.shape[0] - 1
+    code = _check_paged8(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, rows, out)
+    if qo_indptr.dtype != torch.int32 or qo_indptr.ndim != 1 or not qo_indptr.is_contiguous():
+        raise TypeError("paged KV metadata must be contiguous int32")
+    if qo_indptr.shape[0] < rows + 1:
+        raise ValueError("paged KV metadata must cover every row")
+    if sm_scale is not None and not sm_scale >= 0:
+        raise ValueError("prefill attention needs sm_scale >= 0")
+    device = _lib.require_cuda(query, layer_cache, layer_scales, qo_indptr, kv_indptr, kv_indices, last_page_len, out)
+    if out is None:
+        out = torch.empty(query.shape, dtype=torch.bfloat16, device=device)
+    tokens, hq, d = query.shape
+    if tokens == 0 or rows == 0:
+        return out
+    if query.data_ptr() % 16 or query.stride(0) % 8 or query.stride(1) % 8:
+        query = query.clone(memory_format=torch.contiguous_format)
+    _lib.call_on(
+        device, "nqt_prefill_attention8",
+        query.data_ptr(), query.stride(0), query.stride(1),
+        layer_cache.data_ptr(), layer_scales.data_ptr(), layer_cache.shape[0], layer_cache.shape[2],
+        qo_indptr.data_ptr(), kv_indptr.data_ptr(), _table_ptr(kv_indices, kv_indptr), last_page_len.data_ptr(),
+        rows, tokens, hq, layer_cache.shape[3], d,
+        d**-0.5 if sm_scale is None else float(sm_scale), code,
+        out.data_ptr(), out.stride(0), out.stride(1),
         device_status(device).data_ptr(), _lib.stream_handle(device),
     )
     return out
@@ -458,6 +509,7 @@ __all__ = [
     "batch_decode_paged",
     "batch_decode_paged8",
     "batch_prefill_paged",
+    "batch_prefill_paged8",
     "binding_factory",
     "decode_paged8_workspace",
 ]

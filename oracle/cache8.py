@@ -81,9 +81,10 @@ def values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 def attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, indptr, indices, last, qo_indptr=None,
               sm_scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Causal attention of ragged query rows (one per row without ``qo_indptr``) over the cached tokens.  Returns
-    (out, err), float64 [T, Hq, D]: err is the same average of |v| plus 2^-24 of the plain sum of the visible |v|,
-    so that 2^-9 err bounds what rounding every probability p to p (1 +- 2^-9) or, where it is tiny beside the
-    largest, to p +- 2^-33 of the largest does to the output (the largest is at most the sum they are divided by)."""
+    (out, err), float64 [T, Hq, D]: err is the same average of |v| plus 2^-22 of (largest visible scale of v) times
+    the sum of the visible |codes|, so that 2^-11 err bounds what it costs to round every weight p c (probability
+    times value scale) to 11 bits or, where it is tiny, to a multiple of 2^-32 of a weight that occurs: 2^-33 of it
+    for each code, divided by a sum of probabilities that is at least that weight's."""
 
     tokens, hq, d = q.shape
     hkv, page_size = codes.shape[3], codes.shape[2]
@@ -97,6 +98,8 @@ def attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, indptr
             continue
         n = (len(ids) - 1) * page_size + min(max(int(last[r]), 1), page_size)
         kv = values(codes[ids], scales[ids]).transpose(0, 1).reshape(2, -1, hkv, d)[:, :n]
+        raw = codes[ids][:, 1].reshape(-1, hkv, d)[:n].abs()
+        top = scales[ids][:, 1].repeat_interleave(BLOCK, dim=1).reshape(-1, hkv)[:n].amax(0)
         lim = n - (q1 - q0) + torch.arange(q1 - q0)
         hidden = torch.arange(n)[None] > lim[:, None]
         for h in range(hq):
@@ -104,5 +107,6 @@ def attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, indptr
             s = (q[q0:q1, h].double() @ k.t() * scale).masked_fill(hidden, -math.inf)
             p = torch.nan_to_num(s.softmax(-1)) if bool((lim < 0).any()) else s.softmax(-1)
             out[q0:q1, h] = p @ v
-            mag[q0:q1, h] = p @ v.abs() + 2.0**-24 * ((~hidden).double() @ v.abs())
+            g = h // (hq // hkv)
+            mag[q0:q1, h] = p @ v.abs() + 2.0**-22 * top[g] * ((~hidden).double() @ raw[:, g])
     return out, mag

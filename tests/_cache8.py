@@ -61,9 +61,8 @@ def poison_dead_tokens(codes, scales, indptr, indices, last):
 
 
 def attention_tolerance(want, mag):
-    """One rounding to bf16 (2^-8 of the value), and under the average: probabilities rounded to 8 bits at least
-    (2^-9 relative, or 2^-33 of the largest where the decode kernel's fp16 ends: p is held 2^8 above its value
-    against a reference that the largest score never falls below, fp16 rounds what is under 2^-14 by up to 2^-25,
-    and the sum is at least 2^8) with fp32 scores, exponentials and sums (2^-18)."""
+    """One rounding to bf16 (2^-8 of the value), and under the average: weights rounded to fp16 (finfo.eps / 2 =
+    2^-11 each; both kernels hold them 2^8 above their value against a reference that some weight reaches, and fp16
+    rounds what is under 2^-14 by up to 2^-25) with fp32 scores, exponentials and sums (2^-18)."""
 
-    return 2.0**-8 * want.abs() + (2.0**-9 + 2.0**-18) * mag + 1e-30
+    return 2.0**-8 * want.abs() + (2.0**-11 + 2.0**-18) * mag + 1e-30

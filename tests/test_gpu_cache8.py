@@ -50,7 +50,7 @@ def _decode(nqt, cuda, lens, *, kind="int8", page_size=16, hq=16, hkv=8, d=128, 
 
 
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
-@pytest.mark.parametrize("lens", [[1], [1, 15, 16, 17, 31, 32, 33], [0, 5, 0, 0, 40, 0], [2048, 1, 700, 64, 3, 1999],
+@pytest.mark.parametrize("lens", [[1], [1, 15, 16, 17, 31, 32, 33], [0, 5, 0, 0, 40, 0], [0, 0], [2048, 1, 700, 64, 3, 1999],
                                   [5000]])
 def test_decode_lengths(nqt, cuda, kind, lens):
     out = _decode(nqt, cuda, lens, kind=kind)
