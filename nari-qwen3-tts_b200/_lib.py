@@ -212,13 +212,33 @@ def call(name: str, *args) -> int:
     return rc
 
 
-def call_on(device: torch.device, name: str, *args) -> int:
-    """``call`` with ``device`` current: a launch goes to the device of its tensors whichever is current."""
+def call_on(index: int, name: str, *args) -> int:
+    """``call`` with CUDA device ``index`` current: a launch goes to the device of its tensors, whichever is
+    current.  (torch._C is asked directly: the public forms cost more than the launch.)"""
 
-    if device.index is None or device.index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         return call(name, *args)
-    with torch.cuda.device(device):
+    with torch.cuda.device(index):
         return call(name, *args)
+
+
+def cuda_index(*tensors: torch.Tensor | None) -> int:
+    """Device index shared by the given CUDA tensors (ValueError otherwise)."""
+
+    index = -1
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if i < 0 or (i != index and index >= 0):
+                raise ValueError("libnqt kernels require CUDA tensors on one device")
+            index = i
+    return index
+
+
+def raw_stream(index: int) -> int:
+    """Raw cudaStream_t of torch's current stream on device ``index``."""
+
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

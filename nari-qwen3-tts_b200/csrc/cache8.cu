@@ -30,6 +30,7 @@
 
 #include <float.h>
 #include <math.h>
+#include <string.h>
 
 namespace nqt {
 namespace {
@@ -279,6 +280,25 @@ __global__ void __launch_bounds__(256) read8_kernel(const uint8_t* cache, const 
   dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
+// The rotation's turns per position.  The table depends on (head_dim, theta) alone and costs tens of microseconds to
+// make, so the thread's last one is kept.
+void turn_table(uint64_t* out, int head_dim, float theta) {
+  static thread_local float last_theta = 0.f;
+  static thread_local int last_dim = 0;
+  static thread_local uint64_t last[64];
+  if (last_dim != head_dim || last_theta != theta) {
+    const long double ln_theta = logl(static_cast<long double>(theta));
+    const long double full = 18446744073709551616.0L;  // 2^64
+    for (int i = 0; i < head_dim / 2; ++i) {
+      const long double f = expl(-ln_theta * (2.0L * i / head_dim)) / 6.283185307179586476925286766559L * full;
+      last[i] = static_cast<uint64_t>(fmodl(roundl(f), full));
+    }
+    last_dim = head_dim;
+    last_theta = theta;
+  }
+  memcpy(out, last, sizeof(uint64_t) * (head_dim / 2));
+}
+
 bool pairs_aligned(const void* p, int64_t st, int64_t sh) {
   return (reinterpret_cast<uintptr_t>(p) & 3) == 0 && st % 2 == 0 && sh % 2 == 0;
 }
@@ -333,12 +353,7 @@ extern "C" int nqt_qk_norm_rope_paged_cache8(
   a.vec = pairs_aligned(q, q_stride_tok, q_stride_head) && pairs_aligned(k, k_stride_tok, k_stride_head) &&
           pairs_aligned(v, v_stride_tok, v_stride_head) && pairs_aligned(q_out, out_stride_tok, out_stride_head) &&
           pairs_aligned(q_weight, 0, 0) && pairs_aligned(k_weight, 0, 0);
-  const long double ln_theta = logl(static_cast<long double>(rope_theta));
-  const long double full = 18446744073709551616.0L;  // 2^64
-  for (int i = 0; i < head_dim / 2; ++i) {
-    const long double f = expl(-ln_theta * (2.0L * i / head_dim)) / 6.283185307179586476925286766559L * full;
-    a.turns[i] = static_cast<uint64_t>(fmodl(roundl(f), full));
-  }
+  turn_table(a.turns, head_dim, rope_theta);
   const dim3 grid(tokens, (units + 7) / 8);
   cudaStream_t s = as_stream(stream);
   const bool e4m3 = code == NQT_E4M3;

@@ -19,12 +19,19 @@
 // every CTA moves the same bytes whatever the lengths are.  The tile prefix is
 // computed by every CTA from the row lengths (one read and a scan, which costs
 // no more than reading a prefix that a plan kernel left), so the call is one
-// launch.  A sequence that several CTAs cover is finished by the warp that
-// completes its ticket, from fp32 partials in the workspace, in CTA order: the
-// result does not depend on which one that is.  No CTA waits for another.
+// launch.  A row that several CTAs cover leaves fp32 partials in the workspace.
+// They are joined in two steps, 16 CTAs at a time: the warp that completes the
+// ticket of 16 neighbours joins their parts into one, the warp that completes
+// the row's ticket joins those.  One warp never reads more than 16 + n / 16
+// parts, whatever the length, and the order is that of the CTAs: the result
+// does not depend on which warp comes last.  No CTA waits for another.
 //
 // Data path.  A producer warp keeps STAGES tiles in flight with TMA boxes
-// {D bytes, 1 head, 16 tokens, K and V}; each consumer warp owns one KV head.
+// {D bytes, 1 head, 16 tokens, K and V}.  Four consumer warps: one for each of
+// four KV heads, or two or four for each of fewer, which then take turns and
+// join their states in shared memory at the end of a row.  A warp takes two
+// tiles at a time: their products are independent, and the maximum's shuffles
+// and the reference's check are paid once for both.
 // Rows of 128 (64) bytes use the 128-byte (64-byte) swizzle, so ldmatrix reads
 // eight rows without bank conflicts.  ldmatrix moves 16-bit units: as an A
 // operand K's bytes 4t..4t+3 of a row become two fp16 pairs, and since a dot
@@ -41,17 +48,22 @@ using namespace c8;
 
 constexpr int kMaxCtas = 1184;     // split CTAs per head group (8 per SM on 148 SMs)
 constexpr int kMaxRows8 = 8192;    // rows whose prefix a CTA holds in shared memory
+constexpr int kFewRows8 = 255;     // up to here the shared memory is sized alike, so its occupancy is asked for once
+constexpr int kGroup8 = 16;        // CTAs whose parts are joined at once
+constexpr int kMinTiles8 = 4;      // tiles of a CTA at least: shorter parts cost more to join than they save
 constexpr int kPageWindow = 1024;  // page ids of one CTA's tile range staged in shared memory
 
 constexpr size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 struct Ws8 {
-  size_t lse, o, total;  // tickets i32 [batch_cap * hq] come first, zero between launches
+  // tickets come first, zero between launches: i32 [batch_cap * hq] of the rows, then [2 * kMaxCtas * hq] of groups
+  size_t groups, lse, o, total;
 };
 
 constexpr Ws8 ws8_layout(int batch_cap, int hq, int d) {
   Ws8 w{};
-  w.lse = up256(4 * static_cast<size_t>(batch_cap) * hq);
+  w.groups = up256(4 * static_cast<size_t>(batch_cap) * hq);
+  w.lse = up256(w.groups + 4 * static_cast<size_t>(2 * kMaxCtas) * hq);
   w.o = up256(w.lse + 4 * static_cast<size_t>(2 * kMaxCtas) * hq);
   w.total = up256(w.o + 4 * static_cast<size_t>(2 * kMaxCtas) * hq * d);
   return w;
@@ -64,7 +76,7 @@ struct Decode8Args {
   int64_t o_st, o_sh;
   const float* scales;
   const int32_t *indptr, *indices, *last_len;
-  int32_t* tickets;
+  int32_t *tickets, *group_tickets;
   float *part_lse, *part_o;
   int32_t* status;
   int batch, hq, hkv, group, page_size, total_pages, n_ctas;
@@ -147,82 +159,119 @@ __device__ __forceinline__ int row_of_tile(const int32_t* prefix, int batch, int
   return lo;
 }
 
-// out = sum_i 2^(lse_i - M) O_i / sum_i 2^(lse_i - M) over the CTAs c0..c1 that cover `row`, for the query heads
-// of one KV head, by one warp; lane l owns the float4 columns l, l + 32, ...  A CTA's part is in slot 2c when the
-// row starts inside its range, else in 2c + 1.
-template <int D>
-__device__ __forceinline__ void combine_row(const Decode8Args& p, int row, int kvh, int64_t total, int n, int c0,
-                                            int c1, int64_t row_t0, int lane) {
-  constexpr int QD = D / 4;
-  constexpr int kBatch = 4;
+// A CTA has at most two split rows: the one of its first tile leaves its part in slot 2c, one that starts later (and
+// goes on behind the range) in slot 2c + 1.  `late`: the row starts inside its first CTA's range.
+__device__ __forceinline__ int part_slot(int c, int ca, bool late) { return c == ca && late ? 2 * c + 1 : 2 * c; }
+
+// Counts the warp in on a ticket (release of its stores, acquire of the others'); true for the one that completes
+// it with `others` before, which leaves it at zero for the next launch.
+__device__ __forceinline__ bool count_in(int32_t* ticket, int others, int lane) {
+  int arrived = 0;
+  if (lane == 0) {
+    arrived = atomic_inc_acq_rel(ticket);
+    if (arrived == others) *ticket = 0;
+  }
+  return __shfl_sync(kFull, arrived, 0) == others;
+}
+
+// Joins `count` parts of one row and KV head: sum_i 2^(lse_i - M) O_i / sum_i 2^(lse_i - M) for every query head of
+// the group, by one warp.  slot(i): the slot of part i.  Goes to `out` (last) or to slot `dst` as a part.
+template <int D, typename Slot>
+__device__ __forceinline__ void join_parts(const Decode8Args& p, int row, int kvh, int count, Slot slot, bool last,
+                                           int dst, int lane) {
+  constexpr int QD = D / 4;          // float4 of a head
+  constexpr int HP = 32 / QD;        // heads that the warp handles at once
+  constexpr int kBatch = 16;
   const float NEG_INF = -__int_as_float(0x7f800000);
-  for (int f = lane; f < p.group * QD; f += 32) {
-    const int head = kvh * p.group + f / QD;
+  const int col = lane % QD;
+  for (int g0 = 0; g0 < p.group; g0 += HP) {
+    const int g = g0 + lane / QD;
+    const bool live = g < p.group;
+    const int head = kvh * p.group + (live ? g : 0);
     float m = NEG_INF, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int cb = c0; cb <= c1; cb += kBatch) {
+    for (int i0 = 0; i0 < count; i0 += kBatch) {
       float lse[kBatch];
       float4 v[kBatch];
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
-        const int cc = cb + k;
         lse[k] = NEG_INF;
         v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (cc <= c1) {
-          const int slot = first_tile(total, cc, n) >= row_t0 ? 2 * cc : 2 * cc + 1;
-          const int64_t r = static_cast<int64_t>(slot) * p.hq + head;
+        if (i0 + k < count) {
+          const int64_t r = static_cast<int64_t>(slot(i0 + k)) * p.hq + head;
           lse[k] = __ldcg(p.part_lse + r);
-          v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D) + f % QD);
+          v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D) + col);
         }
       }
+      float nm = m;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) nm = fmaxf(nm, lse[k]);
+      const float ref = nm == NEG_INF ? 0.f : nm;
+      const float a = ex2(m - ref);
+      sum *= a;
+      acc.x *= a;
+      acc.y *= a;
+      acc.z *= a;
+      acc.w *= a;
+      m = nm;
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
-        if (cb + k > c1) continue;
-        const float nm = fmaxf(m, lse[k]);
-        const float ref = nm == NEG_INF ? 0.f : nm;
-        const float a = exp2f(m - ref), w = exp2f(lse[k] - ref);
-        sum = sum * a + w;
-        acc.x = acc.x * a + w * v[k].x;
-        acc.y = acc.y * a + w * v[k].y;
-        acc.z = acc.z * a + w * v[k].z;
-        acc.w = acc.w * a + w * v[k].w;
-        m = nm;
+        if (i0 + k >= count) continue;
+        const float w = ex2(lse[k] - ref);
+        sum += w;
+        acc.x = fmaf(w, v[k].x, acc.x);
+        acc.y = fmaf(w, v[k].y, acc.y);
+        acc.z = fmaf(w, v[k].z, acc.z);
+        acc.w = fmaf(w, v[k].w, acc.w);
       }
     }
+    if (!live) continue;
     const float inv = 1.f / sum;
-    __nv_bfloat16* dst = p.out + row * p.o_st + static_cast<int64_t>(head) * p.o_sh + (f % QD) * 4;
-    *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-    *reinterpret_cast<__nv_bfloat162*>(dst + 2) = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+    if (last) {
+      __nv_bfloat16* o = p.out + row * p.o_st + static_cast<int64_t>(head) * p.o_sh + col * 4;
+      *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+      *reinterpret_cast<__nv_bfloat162*>(o + 2) = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+    } else {
+      const int64_t r = static_cast<int64_t>(dst) * p.hq + head;
+      __stcg(reinterpret_cast<float4*>(p.part_o + r * D) + col,
+             make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+      if (col == 0) __stcg(p.part_lse + r, m + log2f(sum));
+    }
   }
 }
 
 template <int D, int HPC, int STAGES>
 struct Cfg8 {
-  static constexpr int kBox = 2 * kBlock * D;  // K then V of 16 tokens of one head
+  static constexpr int kWarps = 4;               // consumer warps
+  static constexpr int kPerHead = kWarps / HPC;  // of one KV head
+  static constexpr int kBox = 2 * kBlock * D;    // K then V of 16 tokens of one head
   static constexpr int kStage = HPC * kBox;
-  static constexpr int kThreads = (HPC + 1) * 32;
-  static constexpr int kBars = 2 * STAGES * 8;
-  static __host__ __device__ constexpr int smem(int batch) {
-    return STAGES * kStage + 1024 + kBars + 4 * kPageWindow + 4 * (2 * (batch + 1)) + (batch + 3) / 4 * 4;
+  static constexpr int kThreads = (kWarps + 1) * 32;
+  static constexpr int kState = 32 * (D / 4 + 4) * 4;  // a warp's O, m and l
+  static constexpr int kJoin = HPC * (kPerHead - 1) * kState;
+  static __host__ __device__ constexpr int smem(int rows) {
+    return STAGES * kStage + 1024 + 2 * STAGES * 8 + kJoin + 4 * kPageWindow + 4 * (2 * (rows + 1)) + (rows + 3) / 4 * 4;
   }
 };
 
 template <int D, int HPC, int STAGES, bool E4M3>
-__global__ void __launch_bounds__((HPC + 1) * 32) decode8_kernel(const __grid_constant__ CUtensorMap tmap,
-                                                                 const __grid_constant__ Decode8Args p) {
+__global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__ CUtensorMap tmap,
+                                                      const __grid_constant__ Decode8Args p) {
   using Cfg = Cfg8<D, HPC, STAGES>;
   constexpr int CH = D / 16;  // 16-byte chunks of a row
+  constexpr int kWarps = Cfg::kWarps, kPerHead = Cfg::kPerHead;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::kStage);
   uint64_t* empty = full + STAGES;
-  int32_t* s_pages = reinterpret_cast<int32_t*>(empty + STAGES);
+  float* s_join = reinterpret_cast<float*>(empty + STAGES);  // [head][warp - 1][O, m, l][lane]
+  int32_t* s_pages = reinterpret_cast<int32_t*>(s_join + Cfg::kJoin / 4);
   int32_t* s_prefix = s_pages + kPageWindow;      // [batch + 1] first tile of every row
   int32_t* s_base = s_prefix + p.batch + 1;       // [batch + 1] kv_indptr
   uint8_t* s_valid = reinterpret_cast<uint8_t*>(s_base + p.batch + 1);  // [batch] tokens of the row's last tile
-  __shared__ int s_warp_sum[HPC + 1];
+  __shared__ int s_warp_sum[kWarps + 1];
   __shared__ int s_issued;
-  __shared__ int s_progress[HPC];
+  __shared__ int s_progress[kWarps];
 
   // see nqt_decode_attention_ex: by default everything waits for the previous grid; with `early` only q, each
   // row's last tile and its scales, the workspace and all writes do
@@ -260,7 +309,7 @@ __global__ void __launch_bounds__((HPC + 1) * 32) decode8_kernel(const __grid_co
     __syncthreads();
     int before = carry, sum = 0;
 #pragma unroll
-    for (int w = 0; w < HPC + 1; ++w) {
+    for (int w = 0; w < kWarps + 1; ++w) {
       if (w < warp) before += s_warp_sum[w];
       sum += s_warp_sum[w];
     }
@@ -288,14 +337,15 @@ __global__ void __launch_bounds__((HPC + 1) * 32) decode8_kernel(const __grid_co
     for (int i = threadIdx.x; i < HPC * p.group * D; i += Cfg::kThreads)
       p.out[b * p.o_st + static_cast<int64_t>(kv0 * p.group + i / D) * p.o_sh + i % D] = __float2bfloat16_rn(0.f);
   }
-  // fewer tiles than CTAs: one tile each and the rest idle, so every range is non-empty
-  const int n = total < p.n_ctas ? static_cast<int>(total) : p.n_ctas;
+  // few tiles: fewer CTAs, so that each has some; every range is non-empty (n <= total)
+  const int64_t want = (total + kMinTiles8 - 1) / kMinTiles8;
+  const int n = want < p.n_ctas ? static_cast<int>(want) : p.n_ctas;
   if (c >= n) return;  // uniform over the block
   const int64_t t_begin = first_tile(total, c, n);
   const int64_t t_end = first_tile(total, c + 1, n);
   const int n_tiles = static_cast<int>(t_end - t_begin);
 
-  if (warp == HPC) {
+  if (warp == kWarps) {
     // ---------------------------------------------------------- producer
     const int row_a = row_of_tile(s_prefix, p.batch, t_begin);
     const int row_b = row_of_tile(s_prefix, p.batch, t_end - 1);
@@ -340,16 +390,12 @@ __global__ void __launch_bounds__((HPC + 1) * 32) decode8_kernel(const __grid_co
     if (lane == 0) s_issued = issued;
   } else {
     // ------------------------------------------------------------ consumers
-    const int kvh = kv0 + warp;
+    const int hw = warp / kPerHead, sub = warp % kPerHead;  // head in the CTA, place among the head's warps
+    const int kvh = kv0 + hw;
     const int g = lane >> 2, t4 = lane & 3;
     const int lm_j = lane >> 3, lm_r = lane & 7;
     const int group = p.group;
     const float NEG_INF = -__int_as_float(0x7f800000);
-
-    uint32_t qf[CH][2];
-    float o[CH][4];
-    float m0 = NEG_INF, m1 = NEG_INF, l0 = 0.f, l1 = 0.f;  // references and sums of heads 2 t4, 2 t4 + 1
-    float f0 = 0.f, f1 = 0.f;                              // their score factors: 2^e of q, sm_scale, log2 e
 
     // scales of up to 32 tiles ahead, one per lane; the page ids are a chunk further ahead
     auto tile_page = [&](int i) -> int {  // page of this lane's tile i, -1 past the range
@@ -366,49 +412,62 @@ __global__ void __launch_bounds__((HPC + 1) * 32) decode8_kernel(const __grid_co
       ks = __ldcg(sp);  // from L2: the previous grid may have written neighbouring scales
       vs = __ldcg(sp + static_cast<int64_t>(tpp) * p.hkv);
     };
+    int chunk = 0;  // the 32 tiles whose scales are in ks_c, vs_c
+    float ks_c, vs_c, ks_n, vs_n;
     int page_nx = tile_page(lane);
-    float ks_c = 0.f, vs_c = 0.f, ks_n, vs_n;
-    if (p.early) grid_dependency_wait();  // q, the last tiles' scales, the partials and tickets of the last launch
-    tile_scales(lane, page_nx, ks_n, vs_n);
+    if (p.early) grid_dependency_wait();  // q, the last tiles' scales, the parts and tickets of the last launch
+    tile_scales(lane, page_nx, ks_c, vs_c);
     page_nx = tile_page(32 + lane);
-
-    int row = row_of_tile(s_prefix, p.batch, t_begin);
-    int row_t0 = s_prefix[row], row_t1 = s_prefix[row + 1];
-    bool open = false;
-    int fix_a = -1, fix_b = -1;  // split rows whose ticket this warp completed
-    int stop = n_tiles;          // first tile that was not consumed
-
-    for (int i = 0; i < n_tiles; ++i) {
-      if ((i & 31) == 0) {  // the next 32 tiles' scales have arrived; start on those after them
+    tile_scales(32 + lane, page_nx, ks_n, vs_n);
+    page_nx = tile_page(64 + lane);
+    auto scales_of = [&](int i, float& ks, float& vs) {  // i does not fall
+      while (chunk < (i >> 5)) {
+        ++chunk;
         ks_c = ks_n;
         vs_c = vs_n;
-        tile_scales(i + 32 + lane, page_nx, ks_n, vs_n);
-        page_nx = tile_page(i + 64 + lane);
+        tile_scales((chunk + 1) * 32 + lane, page_nx, ks_n, vs_n);
+        page_nx = tile_page((chunk + 2) * 32 + lane);
       }
-      const int64_t t = t_begin + i;
-      while (t >= row_t1) {
-        ++row;
-        row_t0 = row_t1;
-        row_t1 = s_prefix[row + 1];
-      }
-      if (!open) {
-        // a new row: its query heads of the group, as B fragments in K's byte order, scaled to a maximum in [1, 2)
+      ks = __shfl_sync(kFull, ks_c, i & 31);
+      vs = __shfl_sync(kFull, vs_c, i & 31);
+    };
+
+    const int tok = ((lm_j & 1) << 3) + lm_r;  // ldmatrix row of this lane
+    const int sw = D == 128 ? (tok & 7) : ((tok >> 1) & 3);
+    const uint32_t box0 = smem_addr(smem) + hw * Cfg::kBox + tok * D;
+    int row = row_of_tile(s_prefix, p.batch, t_begin);
+    int fix_a = -1, fix_b = -1;  // split rows whose group's ticket this warp completed
+    int stop = n_tiles;          // first tile of this warp that was not consumed
+    bool dead = false;           // a wait gave up: the rows are still gone through, so that every ticket completes
+
+    for (int i0 = 0; i0 < n_tiles; ++row) {
+      const int row_t0 = s_prefix[row], row_t1 = s_prefix[row + 1];
+      const int i1 = static_cast<int>(row_t1 - t_begin < n_tiles ? row_t1 - t_begin : n_tiles);
+      if (i1 <= i0) continue;  // a row without pages
+      const bool ends = row_t1 - t_begin == i1;
+      const int valid_last = ends ? s_valid[row] : kBlock;
+
+      // the row's query heads of the group, as B fragments in K's byte order, scaled to a maximum in [1, 2)
+      uint32_t qf[CH][2];
+      float f0, f1;  // score factors of heads 2 t4, 2 t4 + 1: q's power of two, sm_scale, log2 e
+      {
         const __nv_bfloat16* qrow = p.q + row * p.q_st + static_cast<int64_t>(kvh * group + g) * p.q_sh;
-        uint32_t raw[CH][2];
         float amax = 0.f;
 #pragma unroll
         for (int ch = 0; ch < CH; ++ch) {
-          raw[ch][0] = raw[ch][1] = 0u;
+          qf[ch][0] = qf[ch][1] = 0u;
           if (g < group) {
-            raw[ch][0] = *reinterpret_cast<const uint32_t*>(qrow + ch * 16 + 4 * t4);
-            raw[ch][1] = *reinterpret_cast<const uint32_t*>(qrow + ch * 16 + 4 * t4 + 2);
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ch][h]));
-            amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+            qf[ch][0] = *reinterpret_cast<const uint32_t*>(qrow + ch * 16 + 4 * t4);
+            qf[ch][1] = *reinterpret_cast<const uint32_t*>(qrow + ch * 16 + 4 * t4 + 2);
           }
         }
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qf[ch][h]));
+            amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
         amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 2));
         int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
@@ -418,174 +477,238 @@ __global__ void __launch_bounds__((HPC + 1) * 32) decode8_kernel(const __grid_co
         for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ch][h]));
+            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qf[ch][h]));
             qf[ch][h] = pack_f16x2(v.x * down, v.y * down);
           }
         f0 = fp8::exp2_int(__shfl_sync(kFull, e, 8 * t4)) * p.scale_log2;
         f1 = fp8::exp2_int(__shfl_sync(kFull, e, 8 * t4 + 4)) * p.scale_log2;
-#pragma unroll
-        for (int ch = 0; ch < CH; ++ch) o[ch][0] = o[ch][1] = o[ch][2] = o[ch][3] = 0.f;
-        m0 = m1 = NEG_INF;
-        l0 = l1 = 0.f;
-        open = true;
       }
-      const bool last_tile = t == row_t1 - 1;
-      const int valid = last_tile ? s_valid[row] : kBlock;
-      const float ks = __shfl_sync(kFull, ks_c, i & 31), vs = __shfl_sync(kFull, vs_c, i & 31);
+      float o[CH][4];
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) o[ch][0] = o[ch][1] = o[ch][2] = o[ch][3] = 0.f;
+      float m0 = NEG_INF, m1 = NEG_INF, l0 = 0.f, l1 = 0.f;  // references and sums of heads 2 t4, 2 t4 + 1
 
-      const int s = i % STAGES;
-      if (!__all_sync(kFull, pipe_wait(&full[s], (i / STAGES) & 1, p))) {
-        stop = i;
-        break;
-      }
-      const uint32_t box = smem_addr(smem + s * Cfg::kStage + warp * Cfg::kBox);
-      const int tok = ((lm_j & 1) << 3) + lm_r;  // ldmatrix row of this lane
-      const uint32_t krow = box + tok * D, vrow = krow + kBlock * D;
-      const int sw = D == 128 ? (tok & 7) : ((tok >> 1) & 3);
+      for (int i = i0 + 2 * sub; i < i1 && !dead; i += 2 * kPerHead) {
+        const bool two = i + 1 < i1;
+        const int sA = i % STAGES, sB = (i + 1) % STAGES;
+        float ksA, vsA, ksB = 0.f, vsB = 0.f;
+        scales_of(i, ksA, vsA);
+        if (two) scales_of(i + 1, ksB, vsB);
+        bool ok = pipe_wait(&full[sA], (i / STAGES) & 1, p);
+        if (two) ok = pipe_wait(&full[sB], ((i + 1) / STAGES) & 1, p) && ok;
+        if (!__all_sync(kFull, ok)) {
+          dead = true;
+          stop = i;
+          break;
+        }
+        const uint32_t rowA = box0 + sA * Cfg::kStage, rowB = box0 + sB * Cfg::kStage;
 
-      // S^T[tok][head] = sum_d K[tok][d] Q[head][d], in two chains
-      float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
+        // S^T[tok][head] = sum_d K[tok][d] Q[head][d]
+        auto scores = [&](uint32_t krow, float (&s)[4]) {
+          float x[4] = {0.f, 0.f, 0.f, 0.f};
+          s[0] = s[1] = s[2] = s[3] = 0.f;
 #pragma unroll
-      for (int cc = 0; cc < CH; cc += 2) {
-        uint32_t r0, r1, r2, r3;
-        ldmatrix_x4(r0, r1, r2, r3, krow + (((cc + (lm_j >> 1)) ^ sw) << 4));
-        uint32_t a0, a1, a2, a3;
-        codes_to_f16_rows<E4M3>(r0, a0, a2);
-        codes_to_f16_rows<E4M3>(r1, a1, a3);
-        mma_f16_16816(sa, a0, a1, a2, a3, qf[cc][0], qf[cc][1]);
-        codes_to_f16_rows<E4M3>(r2, a0, a2);
-        codes_to_f16_rows<E4M3>(r3, a1, a3);
-        mma_f16_16816(sb, a0, a1, a2, a3, qf[cc + 1][0], qf[cc + 1][1]);
-      }
-      // online softmax (log2): the lane holds heads 2 t4 (0, 2) and 2 t4 + 1 (1, 3) of tokens g and g + 8
-      const bool lo = g < valid, hi = g + 8 < valid;
-      const float c0 = ks * f0, c1 = ks * f1;
-      const float s0 = lo ? (sa[0] + sb[0]) * c0 : NEG_INF;
-      const float s1 = lo ? (sa[1] + sb[1]) * c1 : NEG_INF;
-      const float s2 = hi ? (sa[2] + sb[2]) * c0 : NEG_INF;
-      const float s3 = hi ? (sa[3] + sb[3]) * c1 : NEG_INF;
-      float x0 = fmaxf(s0, s2), x1 = fmaxf(s1, s3);
+          for (int cc = 0; cc < CH; cc += 2) {
+            uint32_t r0, r1, r2, r3, a0, a1, a2, a3;
+            ldmatrix_x4(r0, r1, r2, r3, krow + (((cc + (lm_j >> 1)) ^ sw) << 4));
+            codes_to_f16_rows<E4M3>(r0, a0, a2);
+            codes_to_f16_rows<E4M3>(r1, a1, a3);
+            mma_f16_16816(s, a0, a1, a2, a3, qf[cc][0], qf[cc][1]);
+            codes_to_f16_rows<E4M3>(r2, a0, a2);
+            codes_to_f16_rows<E4M3>(r3, a1, a3);
+            mma_f16_16816(x, a0, a1, a2, a3, qf[cc + 1][0], qf[cc + 1][1]);
+          }
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        x0 = fmaxf(x0, __shfl_xor_sync(kFull, x0, off));
-        x1 = fmaxf(x1, __shfl_xor_sync(kFull, x1, off));
-      }
-      if (__any_sync(kFull, x0 > m0 + 7.f || x1 > m1 + 7.f)) {  // always on a row's first tile (m = -inf)
-        const float n0 = x0 > m0 + 7.f ? x0 : m0, n1 = x1 > m1 + 7.f ? x1 : m1;
-        const float a0 = n0 == m0 ? 1.f : ex2(m0 - n0), a1 = n1 == m1 ? 1.f : ex2(m1 - n1);
-        l0 *= a0;
-        l1 *= a1;
-        m0 = n0;
-        m1 = n1;
+          for (int e = 0; e < 4; ++e) s[e] += x[e];
+        };
+        float sa[4], sb[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+        scores(rowA, sa);
+        if (two) scores(rowB, sb);
+
+        // online softmax (log2): the lane holds heads 2 t4 (0, 2) and 2 t4 + 1 (1, 3) of tokens g and g + 8
+        const int validA = !two && i + 1 == i1 ? valid_last : kBlock;
+        const int validB = two ? (i + 2 == i1 ? valid_last : kBlock) : 0;
+        {
+          const float c0 = ksA * f0, c1 = ksA * f1;
+          sa[0] = g < validA ? sa[0] * c0 : NEG_INF;
+          sa[1] = g < validA ? sa[1] * c1 : NEG_INF;
+          sa[2] = g + 8 < validA ? sa[2] * c0 : NEG_INF;
+          sa[3] = g + 8 < validA ? sa[3] * c1 : NEG_INF;
+        }
+        if (two) {
+          const float c0 = ksB * f0, c1 = ksB * f1;
+          sb[0] = g < validB ? sb[0] * c0 : NEG_INF;
+          sb[1] = g < validB ? sb[1] * c1 : NEG_INF;
+          sb[2] = g + 8 < validB ? sb[2] * c0 : NEG_INF;
+          sb[3] = g + 8 < validB ? sb[3] * c1 : NEG_INF;
+        }
+        float x0 = fmaxf(fmaxf(sa[0], sa[2]), fmaxf(sb[0], sb[2]));
+        float x1 = fmaxf(fmaxf(sa[1], sa[3]), fmaxf(sb[1], sb[3]));
 #pragma unroll
-        for (int ch = 0; ch < CH; ++ch) {
-          o[ch][0] *= a0;
-          o[ch][1] *= a1;
-          o[ch][2] *= a0;
-          o[ch][3] *= a1;
+        for (int off = 4; off < 32; off <<= 1) {
+          x0 = fmaxf(x0, __shfl_xor_sync(kFull, x0, off));
+          x1 = fmaxf(x1, __shfl_xor_sync(kFull, x1, off));
+        }
+        if (__any_sync(kFull, x0 > m0 + 7.f || x1 > m1 + 7.f)) {  // always on a row's first tiles (m = -inf)
+          const float n0 = x0 > m0 + 7.f ? x0 : m0, n1 = x1 > m1 + 7.f ? x1 : m1;
+          const float a0 = n0 == m0 ? 1.f : ex2(m0 - n0), a1 = n1 == m1 ? 1.f : ex2(m1 - n1);
+          l0 *= a0;
+          l1 *= a1;
+          m0 = n0;
+          m1 = n1;
+#pragma unroll
+          for (int ch = 0; ch < CH; ++ch) {
+            o[ch][0] *= a0;
+            o[ch][1] *= a1;
+            o[ch][2] *= a0;
+            o[ch][3] *= a1;
+          }
+        }
+        // p is held 2^8 above its value: fp16 then reaches down to 2^-32 of the reference
+        const float r0 = m0 - 8.f, r1 = m1 - 8.f;
+
+        // O^T[d][head] += c * sum_tok V[tok][d] P[head][tok]; rows g and g + 8 of a chunk are its dims 2g and 2g + 1
+        auto add_values = [&](uint32_t vrow, const float (&s)[4], float vs, int valid) {
+          const float p0 = ex2(s[0] - r0), p1 = ex2(s[1] - r1), p2 = ex2(s[2] - r0), p3 = ex2(s[3] - r1);
+          l0 += p0 + p2;
+          l1 += p1 + p3;
+          const uint32_t b0 = movmatrix_trans(pack_f16x2(p0, p1)), b1 = movmatrix_trans(pack_f16x2(p2, p3));
+          // e4m3 codes behind the row's end may be NaN codes: they count as zeros
+          uint32_t k0 = 0xffffffffu, k1 = 0xffffffffu;
+          if (E4M3) {
+            k0 = (2 * t4 < valid ? 0xffffu : 0u) | (2 * t4 + 1 < valid ? 0xffff0000u : 0u);
+            k1 = (2 * t4 + 8 < valid ? 0xffffu : 0u) | (2 * t4 + 9 < valid ? 0xffff0000u : 0u);
+          }
+#pragma unroll
+          for (int cc = 0; cc < CH; cc += 2) {
+            uint32_t v0, v1, v2, v3, a0, a1, a2, a3;
+            ldmatrix_x4_trans(v0, v1, v2, v3, vrow + (((cc + (lm_j >> 1)) ^ sw) << 4));
+            float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
+            codes_to_f16_cols<E4M3>(v0, a0, a1);
+            codes_to_f16_cols<E4M3>(v1, a2, a3);
+            mma_f16_16816(d, a0 & k0, a1 & k0, a2 & k1, a3 & k1, b0, b1);
+            codes_to_f16_cols<E4M3>(v2, a0, a1);
+            codes_to_f16_cols<E4M3>(v3, a2, a3);
+            mma_f16_16816(e, a0 & k0, a1 & k0, a2 & k1, a3 & k1, b0, b1);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              o[cc][x] = fmaf(vs, d[x], o[cc][x]);
+              o[cc + 1][x] = fmaf(vs, e[x], o[cc + 1][x]);
+            }
+          }
+        };
+        add_values(rowA + kBlock * D, sa, vsA, validA);
+        if (two) add_values(rowB + kBlock * D, sb, vsB, validB);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&empty[sA]);
+          if (two) mbar_arrive(&empty[sB]);
         }
       }
-      // p is held 2^8 above its value: fp16 then reaches down to 2^-32 of the reference
-      const float r0 = m0 - 8.f, r1 = m1 - 8.f;
-      const float p0 = ex2(s0 - r0), p1 = ex2(s1 - r1), p2 = ex2(s2 - r0), p3 = ex2(s3 - r1);
-      l0 += p0 + p2;
-      l1 += p1 + p3;
-      const uint32_t b0 = movmatrix_trans(pack_f16x2(p0, p1)), b1 = movmatrix_trans(pack_f16x2(p2, p3));
-      // e4m3 codes behind the row's end may be NaN codes: they count as zeros
-      uint32_t k0 = 0xffffffffu, k1 = 0xffffffffu;
-      if (E4M3) {
-        k0 = (2 * t4 < valid ? 0xffffu : 0u) | (2 * t4 + 1 < valid ? 0xffff0000u : 0u);
-        k1 = (2 * t4 + 8 < valid ? 0xffffu : 0u) | (2 * t4 + 9 < valid ? 0xffff0000u : 0u);
-      }
-      // O^T[d][head] += c * sum_tok V[tok][d] P[head][tok]; rows g and g + 8 of a chunk are its dims 2g and 2g + 1
-#pragma unroll
-      for (int cc = 0; cc < CH; cc += 2) {
-        uint32_t v0, v1, v2, v3;
-        ldmatrix_x4_trans(v0, v1, v2, v3, vrow + (((cc + (lm_j >> 1)) ^ sw) << 4));
-        uint32_t a0, a1, a2, a3;
-        float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
-        codes_to_f16_cols<E4M3>(v0, a0, a1);
-        codes_to_f16_cols<E4M3>(v1, a2, a3);
-        mma_f16_16816(d, a0 & k0, a1 & k0, a2 & k1, a3 & k1, b0, b1);
-        codes_to_f16_cols<E4M3>(v2, a0, a1);
-        codes_to_f16_cols<E4M3>(v3, a2, a3);
-        mma_f16_16816(e, a0 & k0, a1 & k0, a2 & k1, a3 & k1, b0, b1);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          o[cc][x] = fmaf(vs, d[x], o[cc][x]);
-          o[cc + 1][x] = fmaf(vs, e[x], o[cc + 1][x]);
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
 
-      if (last_tile || i == n_tiles - 1) {
+      if (kPerHead > 1) {
+        // the head's other warps hand their states over; lane by lane they are the same elements
+        float* mine = s_join + (hw * (kPerHead - 1) + (sub > 0 ? sub - 1 : 0)) * (Cfg::kState / 4) + lane;
+        if (sub > 0) {
+#pragma unroll
+          for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) mine[(ch * 4 + x) * 32] = o[ch][x];
+          mine[(CH * 4) * 32] = m0;
+          mine[(CH * 4 + 1) * 32] = m1;
+          mine[(CH * 4 + 2) * 32] = l0;
+          mine[(CH * 4 + 3) * 32] = l1;
+        }
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + hw), "n"(kPerHead * 32) : "memory");
+        if (sub == 0) {
+#pragma unroll 1
+          for (int w = 0; w < kPerHead - 1; ++w) {
+            const float* s = mine + w * (Cfg::kState / 4);
+            const float om0 = s[(CH * 4) * 32], om1 = s[(CH * 4 + 1) * 32];
+            const float n0 = fmaxf(m0, om0), n1 = fmaxf(m1, om1);
+            const float z0 = n0 == NEG_INF ? 0.f : n0, z1 = n1 == NEG_INF ? 0.f : n1;
+            const float a0 = ex2(m0 - z0), a1 = ex2(m1 - z1), b0 = ex2(om0 - z0), b1 = ex2(om1 - z1);
+            l0 = l0 * a0 + s[(CH * 4 + 2) * 32] * b0;
+            l1 = l1 * a1 + s[(CH * 4 + 3) * 32] * b1;
+            m0 = n0;
+            m1 = n1;
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch) {
+              o[ch][0] = o[ch][0] * a0 + s[(ch * 4) * 32] * b0;
+              o[ch][1] = o[ch][1] * a1 + s[(ch * 4 + 1) * 32] * b1;
+              o[ch][2] = o[ch][2] * a0 + s[(ch * 4 + 2) * 32] * b0;
+              o[ch][3] = o[ch][3] * a1 + s[(ch * 4 + 3) * 32] * b1;
+            }
+          }
+        }
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + hw), "n"(kPerHead * 32) : "memory");
+      }
+
+      if (sub == 0) {
         float t0 = l0, t1 = l1;
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
           t0 += __shfl_xor_sync(kFull, t0, off);
           t1 += __shfl_xor_sync(kFull, t1, off);
         }
-        const float i0 = 1.f / t0, i1 = 1.f / t1;
+        const float v0 = 1.f / t0, v1 = 1.f / t1;
         const int ha = kvh * group + 2 * t4;
         const bool has0 = 2 * t4 < group, has1 = 2 * t4 + 1 < group;
-        if (t_begin <= row_t0 && t_end >= row_t1) {
+        if (t_begin <= row_t0 && ends) {
           __nv_bfloat16* ob = p.out + row * p.o_st + static_cast<int64_t>(ha) * p.o_sh + 2 * g;
 #pragma unroll
           for (int ch = 0; ch < CH; ++ch) {
             if (has0)
-              *reinterpret_cast<__nv_bfloat162*>(ob + ch * 16) = __floats2bfloat162_rn(o[ch][0] * i0, o[ch][2] * i0);
+              *reinterpret_cast<__nv_bfloat162*>(ob + ch * 16) = __floats2bfloat162_rn(o[ch][0] * v0, o[ch][2] * v0);
             if (has1)
               *reinterpret_cast<__nv_bfloat162*>(ob + p.o_sh + ch * 16) =
-                  __floats2bfloat162_rn(o[ch][1] * i1, o[ch][3] * i1);
+                  __floats2bfloat162_rn(o[ch][1] * v1, o[ch][3] * v1);
           }
         } else {
-          const int slot = t_begin >= row_t0 ? 2 * c : 2 * c + 1;
+          const int ca = tile_owner(total, n, row_t0), cb = tile_owner(total, n, row_t1 - 1);
+          const bool late = first_tile(total, ca, n) < row_t0;
+          const int slot = part_slot(c, ca, late);
           float* po = p.part_o + (static_cast<int64_t>(slot) * p.hq + ha) * D + 2 * g;
           float* pl = p.part_lse + static_cast<int64_t>(slot) * p.hq + ha;
 #pragma unroll
           for (int ch = 0; ch < CH; ++ch) {
-            if (has0) *reinterpret_cast<float2*>(po + ch * 16) = make_float2(o[ch][0] * i0, o[ch][2] * i0);
-            if (has1) *reinterpret_cast<float2*>(po + D + ch * 16) = make_float2(o[ch][1] * i1, o[ch][3] * i1);
+            if (has0) __stcg(reinterpret_cast<float2*>(po + ch * 16), make_float2(o[ch][0] * v0, o[ch][2] * v0));
+            if (has1) __stcg(reinterpret_cast<float2*>(po + D + ch * 16), make_float2(o[ch][1] * v1, o[ch][3] * v1));
           }
           if (g == 0) {
-            if (has0) pl[0] = m0 + log2f(t0);
-            if (has1) pl[1] = m1 + log2f(t1);
+            if (has0) __stcg(pl, m0 + log2f(t0));
+            if (has1) __stcg(pl + 1, m1 + log2f(t1));
           }
           __syncwarp();
-          const int ca = tile_owner(total, n, row_t0), cb = tile_owner(total, n, row_t1 - 1);
-          int32_t* ticket = p.tickets + static_cast<int64_t>(row) * p.hq + kvh;
-          int arrived = 0;
-          if (lane == 0) arrived = atomic_inc_acq_rel(ticket);
-          arrived = __shfl_sync(kFull, arrived, 0);
-          if (arrived == cb - ca) {
-            if (lane == 0) *ticket = 0;  // ready for the next launch
+          const int lo = max(ca, c / kGroup8 * kGroup8), hi = min(cb, c / kGroup8 * kGroup8 + kGroup8 - 1);
+          if (count_in(p.group_tickets + static_cast<int64_t>(part_slot(lo, ca, late)) * p.hq + kvh, hi - lo,
+                       lane)) {
             if (fix_a < 0) fix_a = row;  // only a range's first and last rows can be split
             else fix_b = row;
           }
         }
-        open = false;
       }
+      i0 = i1;
     }
 
-    if (stop < n_tiles) {
-      // A wait gave up (NQT_DEV_TIMEOUT is set, the output is undefined).  The split rows that this warp did not
-      // finish still count in on their tickets, so that each returns to zero for the next launch.
-      const int last = row_of_tile(s_prefix, p.batch, t_end - 1);
-      for (int r = row; r <= last; r = r == row && last != row ? last : last + 1) {
-        const int r0 = s_prefix[r], r1 = s_prefix[r + 1];
-        if (t_begin <= r0 && t_end >= r1) continue;
-        const int ca = tile_owner(total, n, r0), cb = tile_owner(total, n, r1 - 1);
-        int32_t* ticket = p.tickets + static_cast<int64_t>(r) * p.hq + kvh;
-        if (lane == 0 && atomic_inc_acq_rel(ticket) == cb - ca) *ticket = 0;
-      }
-    }
+    // joins, behind the tile loop: its accumulators are dead here
     __syncwarp();
     for (int f = 0; f < 2; ++f) {
       const int r = f == 0 ? fix_a : fix_b;
       if (r < 0) continue;
-      const int r0 = s_prefix[r], r1 = s_prefix[r + 1];
-      combine_row<D>(p, r, kvh, total, n, tile_owner(total, n, r0), tile_owner(total, n, r1 - 1), r0, lane);
+      const int64_t r0 = s_prefix[r], r1 = s_prefix[r + 1];
+      const int ca = tile_owner(total, n, r0), cb = tile_owner(total, n, r1 - 1);
+      const int lo = max(ca, c / kGroup8 * kGroup8), hi = min(cb, c / kGroup8 * kGroup8 + kGroup8 - 1);
+      const bool late = first_tile(total, ca, n) < r0;
+      const int groups = cb / kGroup8 - ca / kGroup8;  // less one
+      join_parts<D>(p, r, kvh, hi - lo + 1, [&](int i) { return part_slot(lo + i, ca, late); }, groups == 0,
+                    part_slot(lo, ca, late), lane);
+      if (groups == 0) continue;
+      __syncwarp();
+      if (count_in(p.tickets + static_cast<int64_t>(r) * p.hq + kvh, groups, lane))
+        join_parts<D>(
+            p, r, kvh, groups + 1,
+            [&](int i) { return part_slot(i == 0 ? ca : (ca / kGroup8 + i) * kGroup8, ca, late); }, true, 0, lane);
     }
     if (lane == 0) s_progress[warp] = stop;
   }
@@ -593,7 +716,7 @@ __global__ void __launch_bounds__((HPC + 1) * 32) decode8_kernel(const __grid_co
   __syncthreads();
   if (threadIdx.x == 0) {
     int lo = n_tiles;
-    for (int w = 0; w < HPC; ++w) lo = s_progress[w] < lo ? s_progress[w] : lo;
+    for (int w = 0; w < kWarps; ++w) lo = s_progress[w] < lo ? s_progress[w] : lo;
     for (int j = lo; j < s_issued; ++j) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, p.status);
   }
 }
@@ -617,17 +740,23 @@ int encode_tiles(CUtensorMap* map, const void* layer, int total_pages, int page_
 template <int D, int HPC, int STAGES, bool E4M3>
 int launch8(const CUtensorMap& map, Decode8Args a, cudaStream_t s) {
   using Cfg = Cfg8<D, HPC, STAGES>;
-  constexpr int kMaxSmem = Cfg::smem(kMaxRows8);
+  static int few_occ = 1;
   static std::once_flag once;
-  std::call_once(once, [] {
-    cudaFuncSetAttribute(decode8_kernel<D, HPC, STAGES, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+  auto occupancy = [](int smem) {
+    int occ = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, decode8_kernel<D, HPC, STAGES, E4M3>, Cfg::kThreads, smem) !=
+            cudaSuccess ||
+        occ < 1)
+      occ = 1;
+    return occ;
+  };
+  std::call_once(once, [&] {
+    cudaFuncSetAttribute(decode8_kernel<D, HPC, STAGES, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         Cfg::smem(kMaxRows8));
+    few_occ = occupancy(Cfg::smem(kFewRows8));
   });
-  const int smem = Cfg::smem(a.batch);
-  int occ = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, decode8_kernel<D, HPC, STAGES, E4M3>, Cfg::kThreads, smem) !=
-          cudaSuccess ||
-      occ < 1)
-    occ = 1;
+  const int smem = Cfg::smem(a.batch <= kFewRows8 ? kFewRows8 : a.batch);
+  const int occ = a.batch <= kFewRows8 ? few_occ : occupancy(smem);
   const int groups = a.hkv / HPC;
   int n = num_sms() * occ / groups;
   n = n < 1 ? 1 : (n > kMaxCtas ? kMaxCtas : n);
@@ -643,9 +772,10 @@ int launch8(const CUtensorMap& map, Decode8Args a, cudaStream_t s) {
 
 template <int D, bool E4M3>
 int dispatch8(const CUtensorMap& map, const Decode8Args& a, cudaStream_t s) {
-  if (a.hkv % 4 == 0) return launch8<D, 4, 5, E4M3>(map, a, s);
-  if (a.hkv % 2 == 0) return launch8<D, 2, 6, E4M3>(map, a, s);
-  return launch8<D, 1, 8, E4M3>(map, a, s);
+  constexpr int kDeep = 128 / D;  // stages of D = 64 hold half the bytes
+  if (a.hkv % 4 == 0) return launch8<D, 4, 4 * kDeep, E4M3>(map, a, s);
+  if (a.hkv % 2 == 0) return launch8<D, 2, 8 * kDeep, E4M3>(map, a, s);
+  return launch8<D, 1, 16 * kDeep, E4M3>(map, a, s);
 }
 
 }  // namespace
@@ -697,6 +827,7 @@ extern "C" int nqt_decode_attention8(const void* q, int64_t q_stride_tok, int64_
   a.indices = kv_indices;
   a.last_len = last_page_len;
   a.tickets = reinterpret_cast<int32_t*>(base);
+  a.group_tickets = reinterpret_cast<int32_t*>(base + w.groups);
   a.part_lse = reinterpret_cast<float*>(base + w.lse);
   a.part_o = reinterpret_cast<float*>(base + w.o);
   a.status = status;

@@ -34,6 +34,18 @@ def device_status(device: torch.device) -> torch.Tensor:
     return word
 
 
+_STATUS_PTR: dict[int, int] = {}
+
+
+def status_ptr(index: int) -> int:
+    """Address of ``device_status`` of CUDA device ``index``."""
+
+    p = _STATUS_PTR.get(index)
+    if p is None:
+        p = _STATUS_PTR[index] = device_status(torch.device("cuda", index)).data_ptr()
+    return p
+
+
 def read_status(device: torch.device) -> int:
     """Host read of the status word (synchronises); 0 means no device error."""
 
@@ -361,10 +373,10 @@ def paired_qk_norm_rope_paged_cache8(
             raise TypeError("paged QKV metadata must be contiguous int64")
     if out is not None and (out.shape != query.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1):
         raise ValueError("the rotated query must be bf16 of the query's shape, contiguous per head")
-    device = _lib.require_cuda(query, key, value, query_weight, key_weight, position_ids, layer_cache, layer_scales,
-                               write_pages, write_offsets, out)
+    index = _lib.cuda_index(query, key, value, query_weight, key_weight, position_ids, layer_cache, layer_scales,
+                            write_pages, write_offsets, out)
     if out is None:
-        out = torch.empty((tokens, query_heads, head_dim), dtype=torch.bfloat16, device=device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if tokens == 0:
         return out
     if query_weight.dtype != torch.bfloat16 or not query_weight.is_contiguous():
@@ -372,7 +384,7 @@ def paired_qk_norm_rope_paged_cache8(
     if key_weight.dtype != torch.bfloat16 or not key_weight.is_contiguous():
         key_weight = key_weight.to(torch.bfloat16).contiguous()
     _lib.call_on(
-        device, "nqt_qk_norm_rope_paged_cache8",
+        index, "nqt_qk_norm_rope_paged_cache8",
         query.data_ptr(), query.stride(0), query.stride(1),
         key.data_ptr(), key.stride(0), key.stride(1),
         value.data_ptr(), value.stride(0), value.stride(1),
@@ -381,7 +393,7 @@ def paired_qk_norm_rope_paged_cache8(
         out.data_ptr(), out.stride(0), out.stride(1),
         layer_cache.data_ptr(), layer_scales.data_ptr(), layer_cache.shape[0], layer_cache.shape[2],
         tokens, query_heads, key_heads, head_dim,
-        float(epsilon), float(rope_theta), code, device_status(device).data_ptr(), _lib.stream_handle(device),
+        float(epsilon), float(rope_theta), code, status_ptr(index), _lib.raw_stream(index),
     )
     return out
 
@@ -399,14 +411,13 @@ def read_paged_cache8(layer_cache: torch.Tensor, layer_scales: torch.Tensor, pag
     shape = (pages.shape[0], *layer_cache.shape[1:])
     if out is not None and (out.shape != shape or out.dtype != torch.bfloat16 or not out.is_contiguous()):
         raise ValueError("read_paged_cache8 output must be contiguous bf16 [n, 2, page_size, kv_heads, head_dim]")
-    device = _lib.require_cuda(layer_cache, layer_scales, pages, out)
+    index = _lib.cuda_index(layer_cache, layer_scales, pages, out)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        out = layer_cache.new_empty(shape, dtype=torch.bfloat16)
     if pages.shape[0]:
-        _lib.call_on(device, "nqt_read_paged_cache8", layer_cache.data_ptr(), layer_scales.data_ptr(),
+        _lib.call_on(index, "nqt_read_paged_cache8", layer_cache.data_ptr(), layer_scales.data_ptr(),
                      layer_cache.shape[0], layer_cache.shape[2], layer_cache.shape[3], layer_cache.shape[4], code,
-                     pages.data_ptr(), pages.shape[0], out.data_ptr(), device_status(device).data_ptr(),
-                     _lib.stream_handle(device))
+                     pages.data_ptr(), pages.shape[0], out.data_ptr(), status_ptr(index), _lib.raw_stream(index))
     return out
 
 
@@ -716,13 +727,13 @@ def int8_quantize_rows(x: torch.Tensor, *, out: torch.Tensor | None = None,
         raise ValueError("int8_quantize_rows output must be int8 [m, k] with unit column stride")
     if scale is not None and (scale.shape != (m,) or scale.dtype != torch.float32 or not scale.is_contiguous()):
         raise ValueError("int8_quantize_rows scale must be contiguous float32 [m]")
-    device = _lib.require_cuda(x, out, scale)
+    index = _lib.cuda_index(x, out, scale)
     if out is None:
-        out = torch.empty((m, (k + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :k]
+        out = x.new_empty((m, (k + 15) // 16 * 16), dtype=torch.int8)[:, :k]
     if scale is None:
-        scale = torch.empty(m, dtype=torch.float32, device=device)
-    _lib.call_on(device, "nqt_int8_quantize_rows", x.data_ptr(), _row_pitch(x), m, k, out.data_ptr(), _row_pitch(out),
-                 scale.data_ptr(), _lib.stream_handle(device))
+        scale = x.new_empty(m, dtype=torch.float32)
+    _lib.call_on(index, "nqt_int8_quantize_rows", x.data_ptr(), _row_pitch(x), m, k, out.data_ptr(), _row_pitch(out),
+                 scale.data_ptr(), _lib.raw_stream(index))
     return out, scale
 
 
@@ -809,21 +820,20 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
                             or (out.stride(1) != 1 and weight.cols > 1)):
         raise ValueError("linear_int8 output must be bf16 [m, n] with unit column stride")
     epilogue = GEMM_SILU_MUL if weight.gate_up else (GEMM_PLAIN if bias is None else GEMM_BIAS)
-    device = _lib.require_cuda(x, weight.data, bias, xscale, out)
+    index = _lib.cuda_index(x, weight.data, bias, xscale, out)
     if out is None:
-        out = torch.empty((m, weight.cols), dtype=torch.bfloat16, device=device)
+        out = x.new_empty((m, weight.cols), dtype=torch.bfloat16)
     if m == 0:
         return out
     tail = (weight.data.data_ptr(), weight.pitch, weight.data_scale.data_ptr(), ptr(bias), out.data_ptr(),
-            _row_pitch(out), m, weight.rows, weight.cols, k, epilogue, device_status(device).data_ptr(),
-            _lib.stream_handle(device))
+            _row_pitch(out), m, weight.rows, weight.cols, k, epilogue, status_ptr(index), _lib.raw_stream(index))
     if x.dtype == torch.bfloat16:
         if xscale is not None:
             raise ValueError("xscale belongs to int8 codes")
         pitch = (k + 15) // 16 * 16
-        scratch = torch.empty(m * (pitch + 4), dtype=torch.uint8, device=device)
+        scratch = x.new_empty(m * (pitch + 4), dtype=torch.uint8)
         codes = scratch.data_ptr()
-        _lib.call_on(device, "nqt_linear_int8", x.data_ptr(), _row_pitch(x), codes, pitch, codes + m * pitch, *tail)
+        _lib.call_on(index, "nqt_linear_int8", x.data_ptr(), _row_pitch(x), codes, pitch, codes + m * pitch, *tail)
         return out
     if x.dtype != torch.int8 or xscale is None:
         raise TypeError("linear_int8 takes bf16 rows, or int8 codes with their xscale")
@@ -831,5 +841,5 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
         raise ValueError("linear_int8 xscale must be contiguous float32 [m]")
     if _row_pitch(x) % 16 or x.data_ptr() % 16:
         raise ValueError("linear_int8 codes need 16-byte aligned rows")
-    _lib.call_on(device, "nqt_gemm_int8", x.data_ptr(), _row_pitch(x), xscale.data_ptr(), *tail)
+    _lib.call_on(index, "nqt_gemm_int8", x.data_ptr(), _row_pitch(x), xscale.data_ptr(), *tail)
     return out

@@ -38,7 +38,7 @@ import torch
 
 from . import _lib
 from ._lib import call, ptr
-from .kernels import check_cache8, device_status, paired_qk_norm_rope_paged_cache_
+from .kernels import check_cache8, device_status, paired_qk_norm_rope_paged_cache_, status_ptr
 
 # nqt_decode_attention_ex flags (include/nqt.h NQT_DECODE_OVERLAP_KV_WRITE, NQT_DECODE_SHORT_WAIT)
 DECODE_OVERLAP_KV_WRITE = 0x1
@@ -241,14 +241,14 @@ def batch_decode_paged8(
 
     rows = query.shape[0]
     code = _check_paged8(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, rows, out)
-    device = _lib.require_cuda(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, workspace, out)
+    index = _lib.cuda_index(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, workspace, out)
     if out is None:
-        out = torch.empty(query.shape, dtype=torch.bfloat16, device=device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if rows == 0:
         return out
     _, hq, d = query.shape
     _lib.call_on(
-        device, "nqt_decode_attention8",
+        index, "nqt_decode_attention8",
         query.data_ptr(), query.stride(0), query.stride(1),
         layer_cache.data_ptr(), layer_scales.data_ptr(), layer_cache.shape[0], layer_cache.shape[2],
         kv_indptr.data_ptr(), _table_ptr(kv_indices, kv_indptr), last_page_len.data_ptr(),
@@ -257,7 +257,7 @@ def batch_decode_paged8(
         out.data_ptr(), out.stride(0), out.stride(1),
         workspace.data_ptr(), workspace.nbytes,
         (DECODE_OVERLAP_KV_WRITE if overlap_kv_write else 0) | (DECODE_SHORT_WAIT if short_wait else 0),
-        device_status(device).data_ptr(), _lib.stream_handle(device),
+        status_ptr(index), _lib.raw_stream(index),
     )
     return out
 
@@ -287,23 +287,23 @@ def batch_prefill_paged8(
         raise ValueError("paged KV metadata must cover every row")
     if sm_scale is not None and not sm_scale >= 0:
         raise ValueError("prefill attention needs sm_scale >= 0")
-    device = _lib.require_cuda(query, layer_cache, layer_scales, qo_indptr, kv_indptr, kv_indices, last_page_len, out)
+    index = _lib.cuda_index(query, layer_cache, layer_scales, qo_indptr, kv_indptr, kv_indices, last_page_len, out)
     if out is None:
-        out = torch.empty(query.shape, dtype=torch.bfloat16, device=device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     tokens, hq, d = query.shape
     if tokens == 0 or rows == 0:
         return out
     if query.data_ptr() % 16 or query.stride(0) % 8 or query.stride(1) % 8:
         query = query.clone(memory_format=torch.contiguous_format)
     _lib.call_on(
-        device, "nqt_prefill_attention8",
+        index, "nqt_prefill_attention8",
         query.data_ptr(), query.stride(0), query.stride(1),
         layer_cache.data_ptr(), layer_scales.data_ptr(), layer_cache.shape[0], layer_cache.shape[2],
         qo_indptr.data_ptr(), kv_indptr.data_ptr(), _table_ptr(kv_indices, kv_indptr), last_page_len.data_ptr(),
         rows, tokens, hq, layer_cache.shape[3], d,
         d**-0.5 if sm_scale is None else float(sm_scale), code,
         out.data_ptr(), out.stride(0), out.stride(1),
-        device_status(device).data_ptr(), _lib.stream_handle(device),
+        status_ptr(index), _lib.raw_stream(index),
     )
     return out
 
