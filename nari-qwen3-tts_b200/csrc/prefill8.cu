@@ -13,9 +13,10 @@
 //
 // A CTA owns two 128-row query tiles of one row and KV head (a tile row is a token x query head of the group) and
 // walks over blocks of 64 keys:
-//   warps 0..3    Q loader and TMEM owner (0), MMA issuers of tile A (1) and B (2)
-//   warps 4..7    converters: codes from global memory one block ahead, in registers; 16 bits into shared memory in
-//                 the operands' 128-byte-swizzled layout, and the block's scale factors beside them
+//   warp 0        Q loader and TMEM owner; warps 1 and 2: MMA issuers of tile A and B
+//   warp 3        brings the codes of a block by TMA (one box of 16 tokens, K and V, per lane) into a raw ring, and
+//                 the scale factors of four blocks at a time
+//   warps 4..7    converters: raw codes to 16 bits in the operands' 128-byte-swizzled layout
 //   warps 8..15   softmax, one query row per thread (8..11 tile A, 12..15 tile B)
 // TMEM: S double-buffered per tile, p' over its own S buffer, O per tile.  The two tiles share every converted
 // block, which halves the conversions per product.  setmaxnreg gives the softmax warps the registers that the
@@ -37,7 +38,9 @@ namespace p8 {
 constexpr int kM = 128;       // rows per tile
 constexpr int kTiles = 2;     // tiles per CTA
 constexpr int kN = 64;        // keys per block
-constexpr int kStages = 4;
+constexpr int kStages = 3;     // converted blocks
+constexpr int kRaw = 3;        // raw blocks
+constexpr int kScaleRing = 4;  // groups of four blocks whose scale factors are kept
 constexpr int kThreads = 512;
 constexpr int kPages = 1024;  // page ids of the row staged in shared memory
 constexpr int kRows = 512;    // rows of the batch whose tiles are put in order, longest first
@@ -50,15 +53,15 @@ struct P8Cfg {
   static constexpr int kQBytes = p8::kM * D * 2;               // [half][128 rows][128 B]
   static constexpr int kHalf = p8::kN * 128;                   // [64 tokens][128 B]
   static constexpr int kKV = 2 * kHalves * kHalf;              // K halves, V halves
+  static constexpr int kRawBytes = 2 * p8::kN * D;             // [tile][K, V][16 tokens][D]
   static constexpr int kBars = 512;
-  static constexpr int kScales = p8::kStages * 4 * 3 * 4;      // [stage][tile][score factor, log2 c, 1 / c]
+  static constexpr int kScales = p8::kScaleRing * 4 * 4 * 3 * 4;  // [block][tile][score factor, log2 c, 1 / c]
   static constexpr int kRowState = p8::kTiles * p8::kM * 4;    // log2-sum-exp of every row, for the join
   static constexpr int kSmem =
-      1024 + p8::kTiles * kQBytes + p8::kStages * kKV + kBars + kScales + kRowState + 4 * p8::kPages;
+      1024 + p8::kTiles * kQBytes + p8::kStages * kKV + p8::kRaw * kRawBytes + kBars + kScales + kRowState + 4 * p8::kPages;
 };
 
 struct Prefill8Args {
-  const uint8_t* cache;
   const float* scales;
   __nv_bfloat16* out;
   int64_t o_st, o_sh;
@@ -215,8 +218,8 @@ __device__ void find_tile(const Prefill8Args& p, int tpc, int want, int2* stage,
 
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(p8::kThreads, 1)
-    prefill8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap omap,
-                    const __grid_constant__ Prefill8Args p) {
+    prefill8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kvmap,
+                    const __grid_constant__ CUtensorMap omap, const __grid_constant__ Prefill8Args p) {
   using namespace p8;
   using Cfg = P8Cfg<D>;
   constexpr int kHalves = Cfg::kHalves;
@@ -224,16 +227,20 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sKV = sQ + kTiles * Cfg::kQBytes;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(sKV + kStages * Cfg::kKV);
-  uint64_t* kv_full = q_full + 1;
+  uint8_t* sRaw = sKV + kStages * Cfg::kKV;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sRaw + kRaw * Cfg::kRawBytes);
+  uint64_t* raw_full = q_full + 1;
+  uint64_t* raw_empty = raw_full + kRaw;
+  uint64_t* sc_full = raw_empty + kRaw;            // [group of the scale ring]
+  uint64_t* kv_full = sc_full + kScaleRing;
   uint64_t* kv_empty = kv_full + kStages;          // [tile][stage]
   uint64_t* s_full = kv_empty + kTiles * kStages;  // [tile][S buffer]
   uint64_t* p_full = s_full + 2 * kTiles;
   uint64_t* o_done = p_full + 2 * kTiles;          // [tile][parity of the block]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2 * kTiles);
   int* found = reinterpret_cast<int*>(tmem_slot + 1);
-  float* s_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(q_full) + Cfg::kBars);  // [stage][4][3]
-  float* s_lse = s_scale + kStages * 4 * 3;
+  float* s_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(q_full) + Cfg::kBars);  // [block][4][3]
+  float* s_lse = s_scale + kScaleRing * 4 * 4 * 3;
   int32_t* s_pages = reinterpret_cast<int32_t*>(s_lse + kTiles * kM);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -244,6 +251,11 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
   const int tpt = kM / G;  // tokens per tile
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
+    for (int s = 0; s < kRaw; ++s) {
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], 4);
+    }
+    for (int s = 0; s < kScaleRing; ++s) mbar_init(&sc_full[s], 1);
     for (int s = 0; s < kStages; ++s) mbar_init(&kv_full[s], 4);
     for (int s = 0; s < kTiles * kStages; ++s) mbar_init(&kv_empty[s], 1);
     for (int b = 0; b < 2 * kTiles; ++b) {
@@ -253,6 +265,7 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
     }
     fence_barrier_init();
     prefetch_tensormap(&qmap);
+    prefetch_tensormap(&kvmap);
   }
   if (warp == 0) {
     tc::tmem_alloc(tmem_slot, 512);
@@ -356,6 +369,76 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
           if (ok && j + 2 < nbx) issue_s(j + 2);
         }
       }
+    } else if (nb > 0) {
+      // ------------------------------------------------------------ codes and scales
+      const int tpp = p.page_size / kBlock;
+      const uint32_t inv_tpp = static_cast<uint32_t>(0xffffffffu / static_cast<uint32_t>(tpp)) + 1u;  // tpp = 1: 0
+      auto page_index = [&](int tile) -> int {
+        return tpp == 1 ? tile : static_cast<int>(__umulhi(static_cast<uint32_t>(tile), inv_tpp));
+      };
+      const int first_page = page_index(j0 * 4);
+      const int used = min(n_pages, page_index((j0 + nb) * 4 - 1) + 1) - first_page;
+      const bool staged = used <= kPages;
+      if (staged)
+        for (int i = lane; i < used; i += 32) s_pages[i] = pages_g[first_page + i];
+      __syncwarp();
+      // page and block in it of 16-token tile `tile` of the row; total_pages where there is none
+      auto locate = [&](int tile, int& blk) -> int {
+        blk = 0;
+        if (tile * kBlock >= kv_len) return p.total_pages;
+        const int pi = page_index(tile);
+        blk = tile - pi * tpp;
+        const int page = staged ? s_pages[pi - first_page] : pages_g[pi];
+        if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.total_pages)) {
+          report(p.status, NQT_DEV_BAD_PAGE);
+          return p.total_pages;
+        }
+        return page;
+      };
+      // lane: block lane / 8 of a group of four, tile (lane / 2) % 4, K (even) or V (odd)
+      auto load_scale = [&](int group) -> float {
+        const int in = group * 16 + (lane >> 1);  // tile of this CTA's part
+        if (in >= nb * 4) return 0.f;
+        int blk;
+        const int page = locate(j0 * 4 + in, blk);
+        if (page >= p.total_pages) return 0.f;
+        return __ldg(p.scales + ((static_cast<int64_t>(page) * 2 + (lane & 1)) * tpp + blk) * p.hkv + kvh);
+      };
+      float sc = load_scale(0);
+      bool ok = true;
+      int issued = 0;
+      for (int j = 0; j < nb; ++j) {
+        const int s = j % kRaw;
+        if (j >= kRaw) ok = mbar_wait(&raw_empty[s], ((j / kRaw) - 1) & 1, p.status);
+        ok = __all_sync(kFull, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&raw_full[s], Cfg::kRawBytes);
+        __syncwarp();
+        if (lane < 4) {
+          int blk;
+          const int page = locate((j0 + j) * 4 + lane, blk);
+          tma_load_4d(sRaw + s * Cfg::kRawBytes + lane * (2 * kBlock * D), &kvmap, &raw_full[s], 0, kvh, blk * kBlock,
+                      page * 2);
+        }
+        issued = j + 1;
+        if ((j & 3) == 0) {
+          // the ring holds 16 blocks; this warp is at most kRaw + kStages + 1 ahead of the softmax
+          const int group = j >> 2;
+          float* f = s_scale + (((group % kScaleRing) * 16 + (lane >> 1)) * 3);
+          if (lane & 1) {
+            const float c = fmaxf(sc, 8.271806e-25f);  // 2^-80
+            f[1] = log2f(c);
+            f[2] = __fdiv_rn(1.f, c);
+          } else {
+            f[0] = fmaxf(sc * p.scale_log2, 1.17549435e-38f);  // a masked -inf times it stays -inf
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_full[group % kScaleRing]);
+          if (j + 4 < nb) sc = load_scale(group + 1);
+        }
+      }
+      // the last copies have landed before the CTA leaves, also when a wait gave up
+      for (int j = max(0, issued - kRaw); j < issued; ++j) mbar_wait(&raw_full[j % kRaw], (j / kRaw) & 1, p.status);
     }
     if (S > 1) {  // the join's two barriers belong to every thread of the cluster
       gemm_detail::cluster_arrive();
@@ -373,113 +456,72 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
   } else if (warp < 8) {
     // ------------------------------------------------------------ converters
     reg_dec<112>();
-    if (nb > 0) {
+    {
       const int ct = threadIdx.x - 128;
-      constexpr int kChunks = D / 16;          // 16-code chunks of a row
-      constexpr int kStep = 128 / kChunks;     // tokens that the 128 threads cover at once
+      constexpr int kChunks = D / 16;       // 16-code chunks of a row
+      constexpr int kStep = 128 / kChunks;  // tokens that the 128 threads cover at once
       constexpr int kIter = kN / kStep;
       const int chunk = ct % kChunks, tok0 = ct / kChunks;
-      const int first_page = j0 * kN / p.page_size;
-      const int used = min(n_pages, ((j0 + nb) * kN + p.page_size - 1) / p.page_size) - first_page;
-      const bool staged = used <= kPages;
-      if (staged)
-        for (int i = ct; i < used; i += 128) s_pages[i] = pages_g[first_page + i];
-      bar_sync(1, 128);
-      const int64_t row_bytes = static_cast<int64_t>(p.hkv) * D;
-      const int64_t kind_bytes = p.page_size * row_bytes;
-      const int tpp = p.page_size / kBlock;
-
-      struct Block {
-        uint4 k[kIter], v[kIter];
-        float sc;  // threads 0..7: scale of tile ct / 2, K (even) or V (odd)
-      };
-      // page of the key at `pos`, or total_pages where there is none
-      auto page_of = [&](int pos) -> int {
-        if (pos >= kv_len) return p.total_pages;
-        const int pi = pos / p.page_size;
-        const int page = staged ? s_pages[pi - first_page] : pages_g[pi];
-        if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.total_pages)) {
-          report(p.status, NQT_DEV_BAD_PAGE);
-          return p.total_pages;
-        }
-        return page;
-      };
-      auto load = [&](int j, Block& b) {
-        const int base = (j0 + j) * kN;
-#pragma unroll
-        for (int i = 0; i < kIter; ++i) {
-          const int pos = base + tok0 + i * kStep;
-          const int page = page_of(pos);
-          b.k[i] = b.v[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (page < p.total_pages) {
-            const uint8_t* src = p.cache + static_cast<int64_t>(page) * 2 * kind_bytes + (pos % p.page_size) * row_bytes +
-                                 kvh * D + chunk * 16;
-            b.k[i] = *reinterpret_cast<const uint4*>(src);
-            b.v[i] = *reinterpret_cast<const uint4*>(src + kind_bytes);
-          }
-        }
-        b.sc = 0.f;
-        if (ct < 8) {
-          const int pos = base + (ct >> 1) * kBlock;
-          const int page = page_of(pos);
-          if (page < p.total_pages)
-            b.sc = p.scales[((static_cast<int64_t>(page) * 2 + (ct & 1)) * tpp + pos % p.page_size / kBlock) * p.hkv + kvh];
-        }
-      };
-      auto put = [&](uint8_t* dst, int tok, uint4 w, bool is_v) {
-        // dims 16 chunk .. + 15: two 16-byte pieces of the token's 128-byte line, swizzled by the token; the two
-        // halves of a row write their pieces in opposite order, so that a quarter-warp's stores meet no bank twice
-        uint32_t o[8];
-        if (is_v) {
-          codes_to_f16_rows<E4M3>(w.x, o[0], o[1]);
-          codes_to_f16_rows<E4M3>(w.y, o[2], o[3]);
-          codes_to_f16_rows<E4M3>(w.z, o[4], o[5]);
-          codes_to_f16_rows<E4M3>(w.w, o[6], o[7]);
-        } else {
-          codes_to_bf16<E4M3>(w.x, o[0], o[1]);
-          codes_to_bf16<E4M3>(w.y, o[2], o[3]);
-          codes_to_bf16<E4M3>(w.z, o[4], o[5]);
-          codes_to_bf16<E4M3>(w.w, o[6], o[7]);
-        }
-        uint8_t* line = dst + (chunk >> 2) * Cfg::kHalf + tok * 128;
-        const int c = (chunk & 3) * 2, flip = (chunk >> 2) & 1;
-        const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-        *reinterpret_cast<uint4*>(line + (((c + flip) ^ (tok & 7)) << 4)) = flip ? hi : lo;
-        *reinterpret_cast<uint4*>(line + (((c + 1 - flip) ^ (tok & 7)) << 4)) = flip ? lo : hi;
-      };
-      Block cur, nxt;
-      load(0, cur);
-      for (int j = 0; j < nb; ++j) {
-        if (j + 1 < nb) load(j + 1, nxt);
-        const int s = j % kStages;
-        bool ready = true;
+      // Where the thread's chunk lies in a raw tile pair, and its two 16-byte pieces in the token's 128-byte line,
+      // swizzled by the token (kStep is a multiple of 8, so the same for all of its tokens).  The two halves of a row
+      // write their pieces in opposite order, so that a quarter-warp's stores meet no bank twice.
+      const uint32_t raw0 = (tok0 / kBlock) * (2 * kBlock * D) + (tok0 % kBlock) * D + chunk * 16;
+      const int c = (chunk & 3) * 2, flip = (chunk >> 2) & 1;
+      const uint32_t line = (chunk >> 2) * Cfg::kHalf + tok0 * 128;
+      const uint32_t at0 = line + (((c + flip) ^ (tok0 & 7)) << 4), at1 = line + (((c + 1 - flip) ^ (tok0 & 7)) << 4);
+      bool ok = true;
+      for (int j = 0; j < nb && ok; ++j) {
+        const int rs = j % kRaw, s = j % kStages;
+        ok = mbar_wait(&raw_full[rs], (j / kRaw) & 1, p.status);
         if (j >= kStages) {
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)
             if (j - kStages < nbt[t] && !mbar_wait(&kv_empty[t * kStages + s], ((j / kStages) - 1) & 1, p.status))
-              ready = false;
+              ok = false;
         }
-        if (!__all_sync(kFull, ready)) break;
+        ok = __all_sync(kFull, ok);
+        if (!ok) break;
+        const uint8_t* raw = sRaw + rs * Cfg::kRawBytes + raw0;
+        uint4 k[kIter], v[kIter];
+#pragma unroll
+        for (int i = 0; i < kIter; ++i) {
+          k[i] = *reinterpret_cast<const uint4*>(raw + i * (kStep * 2 * D));
+          v[i] = *reinterpret_cast<const uint4*>(raw + i * (kStep * 2 * D) + kBlock * D);
+        }
+        const int left = kv_len - (j0 + j) * kN;  // tokens of the block that exist
+        if (E4M3 && left < kN) {  // what lies behind them may be NaN codes, which no probability of 0 silences
+#pragma unroll
+          for (int i = 0; i < kIter; ++i)
+            if (tok0 + i * kStep >= left) v[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
         uint8_t* st = sKV + s * Cfg::kKV;
 #pragma unroll
         for (int i = 0; i < kIter; ++i) {
-          put(st, tok0 + i * kStep, cur.k[i], false);
-          put(st + kHalves * Cfg::kHalf, tok0 + i * kStep, cur.v[i], true);
+          uint32_t o[8];
+          codes_to_bf16<E4M3>(k[i].x, o[0], o[1]);
+          codes_to_bf16<E4M3>(k[i].y, o[2], o[3]);
+          codes_to_bf16<E4M3>(k[i].z, o[4], o[5]);
+          codes_to_bf16<E4M3>(k[i].w, o[6], o[7]);
+          *reinterpret_cast<uint4*>(st + at0 + i * (kStep * 128)) = flip ? make_uint4(o[4], o[5], o[6], o[7]) : make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(st + at1 + i * (kStep * 128)) = flip ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(o[4], o[5], o[6], o[7]);
         }
-        if (ct < 8) {
-          float* f = s_scale + (s * 4 + (ct >> 1)) * 3;
-          if (ct & 1) {
-            const float c = fmaxf(cur.sc, 8.271806e-25f);  // 2^-80
-            f[1] = log2f(c);
-            f[2] = __fdiv_rn(1.f, c);
-          } else {
-            f[0] = fmaxf(cur.sc * p.scale_log2, 1.17549435e-38f);  // a masked -inf times it stays -inf
-          }
+#pragma unroll
+        for (int i = 0; i < kIter; ++i) {
+          uint32_t o[8];
+          codes_to_f16_rows<E4M3>(v[i].x, o[0], o[1]);
+          codes_to_f16_rows<E4M3>(v[i].y, o[2], o[3]);
+          codes_to_f16_rows<E4M3>(v[i].z, o[4], o[5]);
+          codes_to_f16_rows<E4M3>(v[i].w, o[6], o[7]);
+          uint8_t* sv = st + kHalves * Cfg::kHalf + i * (kStep * 128);
+          *reinterpret_cast<uint4*>(sv + at0) = flip ? make_uint4(o[4], o[5], o[6], o[7]) : make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(sv + at1) = flip ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(o[4], o[5], o[6], o[7]);
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[s]);
-        cur = nxt;
+        if (lane == 0) {
+          mbar_arrive(&raw_empty[rs]);
+          mbar_arrive(&kv_full[s]);
+        }
       }
     }
     if (S > 1) {  // the join's two barriers belong to every thread of the cluster
@@ -506,8 +548,9 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
     float m_used = NEG_INF, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nbx; ++j) {
-      const int sb = j & 1, s = j % kStages;
-      ok = mbar_wait(&kv_full[s], (j / kStages) & 1, p.status) && mbar_wait(&sfull[sb], (j >> 1) & 1, p.status);
+      const int sb = j & 1, s = j % (4 * kScaleRing);
+      if ((j & 3) == 0) ok = mbar_wait(&sc_full[(j >> 2) % kScaleRing], ((j >> 2) / kScaleRing) & 1, p.status);
+      ok = mbar_wait(&sfull[sb], (j >> 1) & 1, p.status) && ok;
       ok = __all_sync(kFull, ok);
       if (!ok) break;
       tc::fence_after_sync();
@@ -745,9 +788,25 @@ int encode_rows(CUtensorMap* map, const void* q, int64_t st, int64_t sh, int tok
   return r == CUDA_SUCCESS ? NQT_OK : NQT_ERR_CUDA;
 }
 
+// The layer's codes as {D, Hkv, P, pages x 2} in boxes of one head x 16 tokens x K and V, rows as they are.
+int encode_codes(CUtensorMap* map, const void* layer, int total_pages, int page_size, int hkv, int d) {
+  auto encode = c8::get_encode();
+  if (encode == nullptr) return NQT_ERR_CUDA;
+  const cuuint64_t D = static_cast<cuuint64_t>(d);
+  cuuint64_t dims[4] = {D, static_cast<cuuint64_t>(hkv), static_cast<cuuint64_t>(page_size),
+                        static_cast<cuuint64_t>(total_pages) * 2};
+  cuuint64_t strides[3] = {D, static_cast<cuuint64_t>(hkv) * D, static_cast<cuuint64_t>(page_size) * hkv * D};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(d), 1, kBlock, 2};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(layer), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? NQT_OK : NQT_ERR_CUDA;
+}
+
 template <int D, bool E4M3>
-int launch_prefill8(const CUtensorMap& qmap, const CUtensorMap& omap, const Prefill8Args& a, int total_q,
-                    cudaStream_t s) {
+int launch_prefill8(const CUtensorMap& qmap, const CUtensorMap& kvmap, const CUtensorMap& omap,
+                    const Prefill8Args& a, int total_q, cudaStream_t s) {
   using Cfg = P8Cfg<D>;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -773,7 +832,7 @@ int launch_prefill8(const CUtensorMap& qmap, const CUtensorMap& omap, const Pref
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = split > 1 ? 1 : 0;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, prefill8_kernel<D, E4M3>, qmap, omap, a);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, prefill8_kernel<D, E4M3>, qmap, kvmap, omap, a);
   if (err != cudaSuccess) {
     set_last_error("prefill_attention8", err);
     return NQT_ERR_CUDA;
@@ -802,14 +861,14 @@ extern "C" int nqt_prefill_attention8(const void* q, int64_t q_stride_tok, int64
   if (group > 8) return NQT_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || q_stride_tok % 8 || q_stride_head % 8) return NQT_ERR_ARG;
   if (total_q_tokens == 0) return NQT_OK;
-  CUtensorMap qmap, omap{};
+  CUtensorMap qmap, kvmap, omap{};
   rc = encode_rows(&qmap, q, q_stride_tok, q_stride_head, total_q_tokens, num_qo_heads, group, head_dim);
+  if (rc == NQT_OK) rc = encode_codes(&kvmap, layer_cache, total_pages, page_size, num_kv_heads, head_dim);
   if (rc != NQT_OK) {
     set_last_message("prefill_attention8: cuTensorMapEncodeTiled failed");
     return rc;
   }
   Prefill8Args a{};
-  a.cache = static_cast<const uint8_t*>(layer_cache);
   a.scales = layer_scales;
   a.out = static_cast<__nv_bfloat16*>(out);
   a.o_st = out_stride_tok;
@@ -831,8 +890,8 @@ extern "C" int nqt_prefill_attention8(const void* q, int64_t q_stride_tok, int64
                                      head_dim) == NQT_OK;
   cudaStream_t s = as_stream(stream);
   if (head_dim == 128)
-    return code == NQT_E4M3 ? launch_prefill8<128, true>(qmap, omap, a, total_q_tokens, s)
-                            : launch_prefill8<128, false>(qmap, omap, a, total_q_tokens, s);
-  return code == NQT_E4M3 ? launch_prefill8<64, true>(qmap, omap, a, total_q_tokens, s)
-                          : launch_prefill8<64, false>(qmap, omap, a, total_q_tokens, s);
+    return code == NQT_E4M3 ? launch_prefill8<128, true>(qmap, kvmap, omap, a, total_q_tokens, s)
+                            : launch_prefill8<128, false>(qmap, kvmap, omap, a, total_q_tokens, s);
+  return code == NQT_E4M3 ? launch_prefill8<64, true>(qmap, kvmap, omap, a, total_q_tokens, s)
+                          : launch_prefill8<64, false>(qmap, kvmap, omap, a, total_q_tokens, s);
 }
