@@ -4,15 +4,16 @@
 //
 // over the (n_pages - 1) * P + last_page_len tokens of row b, one query per row.
 //
-// Mathematics.  With codes k_t, v_t and block scales a, c (16 tokens each):
-//   s_t = a * (q . k_t) * sm_scale,   O = sum_t 2^(s_t - m) c v_t / sum_t 2^(s_t - m)
-// in one pass with a running reference m and fp32 sums.  q . k and p . v are
-// fp16 tensor-core tiles with fp32 accumulation: codes are exact in fp16; q is
-// brought to [1, 2) by the power of two of its row maximum, which is exact for
-// every element above 2^-14 of it; p is rounded to fp16's 11 bits and kept
-// between 2^-32 and 2^7 of the reference, so m only moves when a score exceeds
-// it by more than 7 (in log2) and the accumulators are rarely rescaled.  The
-// scale c multiplies the tile's fp32 product, so no rounding depends on it.
+// Mathematics.  With codes k_t, v_t and block scales a, c (16 tokens each), in log2 units and with a running
+// reference M:
+//   x_t = a sm_scale log2(e) (q . k_t),  y_t = x_t + log2 c,  p'_t = 2^(y_t - M + 8),
+//   O = sum_t p'_t v_t,  l = sum_t p'_t / c,  out = O / l
+// so a value's scale is a summand of an exponent.  q . k and p' v are fp16 tensor-core tiles with fp32
+// accumulation: codes are exact in fp16; q is brought to [1, 2) by the power of two of its row maximum, which is
+// exact for every element above 2^-14 of it; p' is rounded to fp16's 11 bits.  M follows the maximum of y, the
+// weight with which a token's codes enter the output, and moves only when that grows by more than 7: p' lies below
+// 2^15, fp16 reaches down to 2^-32 of the largest weight, and the accumulators are rarely rescaled.  Scales below
+// 2^-80 count as 2^-80.
 //
 // Work split.  The KV of one KV-head group is a flat list of 16-token tiles;
 // CTA c of n streams tiles [T c / n, T (c + 1) / n) across sequence borders, so
@@ -27,7 +28,7 @@
 // does not depend on which warp comes last.  No CTA waits for another.
 //
 // Data path.  A producer warp keeps STAGES tiles in flight with TMA boxes
-// {D bytes, 1 head, 16 tokens, K and V}.  Four consumer warps: one for each of
+// {one head, or two of 64 dims, 16 tokens, K and V}.  Four consumer warps: one for each of
 // four KV heads, or two or four for each of fewer, which then take turns and
 // join their states in shared memory at the end of a row.  A warp takes two
 // tiles at a time: their products are independent, and the maximum's shuffles
@@ -51,7 +52,6 @@ constexpr int kMaxRows8 = 8192;    // rows whose prefix a CTA holds in shared me
 constexpr int kFewRows8 = 255;     // up to here the shared memory is sized alike, so its occupancy is asked for once
 constexpr int kGroup8 = 16;        // CTAs whose parts are joined at once
 constexpr int kMinTiles8 = 4;      // tiles of a CTA at least: shorter parts cost more to join than they save
-constexpr int kPageWindow = 1024;  // page ids of one CTA's tile range staged in shared memory
 
 constexpr size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -175,67 +175,84 @@ __device__ __forceinline__ bool count_in(int32_t* ticket, int others, int lane) 
 }
 
 // Joins `count` parts of one row and KV head: sum_i 2^(lse_i - M) O_i / sum_i 2^(lse_i - M) for every query head of
-// the group, by one warp.  slot(i): the slot of part i.  Goes to `out` (last) or to slot `dst` as a part.
+// the group, by one warp.  slot(i): the slot of part i.  Goes to `out` (last) or to slot `dst` as a part.  The loads
+// of two sets of heads and eight parts are in flight at once: a join is a chain of trips to L2.
 template <int D, typename Slot>
 __device__ __forceinline__ void join_parts(const Decode8Args& p, int row, int kvh, int count, Slot slot, bool last,
                                            int dst, int lane) {
-  constexpr int QD = D / 4;          // float4 of a head
-  constexpr int HP = 32 / QD;        // heads that the warp handles at once
-  constexpr int kBatch = 16;
+  constexpr int QD = D / 4;    // float4 of a head
+  constexpr int HP = 32 / QD;  // heads of a set: the warp's lanes
+  constexpr int kBatch = 8;
   const float NEG_INF = -__int_as_float(0x7f800000);
   const int col = lane % QD;
-  for (int g0 = 0; g0 < p.group; g0 += HP) {
-    const int g = g0 + lane / QD;
-    const bool live = g < p.group;
-    const int head = kvh * p.group + (live ? g : 0);
-    float m = NEG_INF, sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < count; i0 += kBatch) {
-      float lse[kBatch];
-      float4 v[kBatch];
+  for (int g0 = 0; g0 < p.group; g0 += 2 * HP) {
+    int head[2];
+    bool live[2];
+    float m[2], sum[2];
+    float4 acc[2];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        lse[k] = NEG_INF;
-        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i0 + k < count) {
-          const int64_t r = static_cast<int64_t>(slot(i0 + k)) * p.hq + head;
-          lse[k] = __ldcg(p.part_lse + r);
-          v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D) + col);
+    for (int u = 0; u < 2; ++u) {
+      const int g = g0 + u * HP + lane / QD;
+      live[u] = g < p.group;
+      head[u] = kvh * p.group + (live[u] ? g : 0);
+      m[u] = NEG_INF;
+      sum[u] = 0.f;
+      acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int i0 = 0; i0 < count; i0 += kBatch) {
+      float lse[2][kBatch];
+      float4 v[2][kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          lse[u][k] = NEG_INF;
+          v[u][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i0 + k < count && live[u]) {
+            const int64_t r = static_cast<int64_t>(slot(i0 + k)) * p.hq + head[u];
+            lse[u][k] = __ldcg(p.part_lse + r);
+            v[u][k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D) + col);
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float nm = m[u];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) nm = fmaxf(nm, lse[u][k]);
+        const float ref = nm == NEG_INF ? 0.f : nm;
+        const float a = ex2(m[u] - ref);
+        m[u] = nm;
+        sum[u] *= a;
+        acc[u].x *= a;
+        acc[u].y *= a;
+        acc[u].z *= a;
+        acc[u].w *= a;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          if (i0 + k >= count) continue;
+          const float w = ex2(lse[u][k] - ref);
+          sum[u] += w;
+          acc[u].x = fmaf(w, v[u][k].x, acc[u].x);
+          acc[u].y = fmaf(w, v[u][k].y, acc[u].y);
+          acc[u].z = fmaf(w, v[u][k].z, acc[u].z);
+          acc[u].w = fmaf(w, v[u][k].w, acc[u].w);
         }
       }
-      float nm = m;
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) nm = fmaxf(nm, lse[k]);
-      const float ref = nm == NEG_INF ? 0.f : nm;
-      const float a = ex2(m - ref);
-      sum *= a;
-      acc.x *= a;
-      acc.y *= a;
-      acc.z *= a;
-      acc.w *= a;
-      m = nm;
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        if (i0 + k >= count) continue;
-        const float w = ex2(lse[k] - ref);
-        sum += w;
-        acc.x = fmaf(w, v[k].x, acc.x);
-        acc.y = fmaf(w, v[k].y, acc.y);
-        acc.z = fmaf(w, v[k].z, acc.z);
-        acc.w = fmaf(w, v[k].w, acc.w);
-      }
     }
-    if (!live) continue;
-    const float inv = 1.f / sum;
-    if (last) {
-      __nv_bfloat16* o = p.out + row * p.o_st + static_cast<int64_t>(head) * p.o_sh + col * 4;
-      *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-      *reinterpret_cast<__nv_bfloat162*>(o + 2) = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-    } else {
-      const int64_t r = static_cast<int64_t>(dst) * p.hq + head;
-      __stcg(reinterpret_cast<float4*>(p.part_o + r * D) + col,
-             make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-      if (col == 0) __stcg(p.part_lse + r, m + log2f(sum));
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (!live[u]) continue;
+      const float inv = 1.f / sum[u];
+      if (last) {
+        __nv_bfloat16* o = p.out + row * p.o_st + static_cast<int64_t>(head[u]) * p.o_sh + col * 4;
+        *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(acc[u].x * inv, acc[u].y * inv);
+        *reinterpret_cast<__nv_bfloat162*>(o + 2) = __floats2bfloat162_rn(acc[u].z * inv, acc[u].w * inv);
+      } else {
+        const int64_t r = static_cast<int64_t>(dst) * p.hq + head[u];
+        __stcg(reinterpret_cast<float4*>(p.part_o + r * D) + col,
+               make_float4(acc[u].x * inv, acc[u].y * inv, acc[u].z * inv, acc[u].w * inv));
+        if (col == 0) __stcg(p.part_lse + r, m[u] + log2f(sum[u]));
+      }
     }
   }
 }
@@ -244,13 +261,16 @@ template <int D, int HPC, int STAGES>
 struct Cfg8 {
   static constexpr int kWarps = 4;               // consumer warps
   static constexpr int kPerHead = kWarps / HPC;  // of one KV head
-  static constexpr int kBox = 2 * kBlock * D;    // K then V of 16 tokens of one head
-  static constexpr int kStage = HPC * kBox;
+  static constexpr int kBoxHeads = D == 64 && HPC > 1 ? 2 : 1;  // heads of a TMA box: rows of 128 bytes if it can be
+  static constexpr int kBoxRow = kBoxHeads * D;
+  static constexpr int kBox = 2 * kBlock * kBoxRow;  // K then V of 16 tokens
+  static constexpr int kBoxes = HPC / kBoxHeads;
+  static constexpr int kStage = kBoxes * kBox;
   static constexpr int kThreads = (kWarps + 1) * 32;
   static constexpr int kState = 32 * (D / 4 + 4) * 4;  // a warp's O, m and l
   static constexpr int kJoin = HPC * (kPerHead - 1) * kState;
   static __host__ __device__ constexpr int smem(int rows) {
-    return STAGES * kStage + 1024 + 2 * STAGES * 8 + kJoin + 4 * kPageWindow + 4 * (2 * (rows + 1)) + (rows + 3) / 4 * 4;
+    return STAGES * kStage + 1024 + 2 * STAGES * 8 + kJoin + 4 * (2 * (rows + 1)) + (rows + 3) / 4 * 4;
   }
 };
 
@@ -265,8 +285,7 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::kStage);
   uint64_t* empty = full + STAGES;
   float* s_join = reinterpret_cast<float*>(empty + STAGES);  // [head][warp - 1][O, m, l][lane]
-  int32_t* s_pages = reinterpret_cast<int32_t*>(s_join + Cfg::kJoin / 4);
-  int32_t* s_prefix = s_pages + kPageWindow;      // [batch + 1] first tile of every row
+  int32_t* s_prefix = reinterpret_cast<int32_t*>(s_join + Cfg::kJoin / 4);  // [batch + 1] first tile of every row
   int32_t* s_base = s_prefix + p.batch + 1;       // [batch + 1] kv_indptr
   uint8_t* s_valid = reinterpret_cast<uint8_t*>(s_base + p.batch + 1);  // [batch] tokens of the row's last tile
   __shared__ int s_warp_sum[kWarps + 1];
@@ -347,45 +366,53 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
 
   if (warp == kWarps) {
     // ---------------------------------------------------------- producer
-    const int row_a = row_of_tile(s_prefix, p.batch, t_begin);
-    const int row_b = row_of_tile(s_prefix, p.batch, t_end - 1);
-    // the range's tiles read one contiguous window of kv_indices: bring it in with all lanes
-    const int win0 = s_base[row_a] + static_cast<int>(t_begin - s_prefix[row_a]) / tpp;
-    const int win1 = s_base[row_b] + static_cast<int>(t_end - 1 - s_prefix[row_b]) / tpp + 1;
-    const bool windowed = win1 - win0 <= kPageWindow;
-    if (windowed)
-      for (int i = lane; i < win1 - win0; i += 32) s_pages[i] = p.indices[win0 + i];
-    __syncwarp();
+    // lane l looks up the page of tile 32 k + l of the range: one search and one load for 32 tiles, a chunk ahead
+    auto look_up = [&](int i, int& page, int& tok) -> bool {  // whether the tile is its row's last
+      page = p.total_pages;  // a box outside the map: TMA fills zeros
+      tok = 0;
+      if (i >= n_tiles) return false;
+      const int64_t t = t_begin + i;
+      const int r = row_of_tile(s_prefix, p.batch, t);
+      const int in_row = static_cast<int>(t - s_prefix[r]);
+      const int pl = in_row / tpp;
+      tok = (in_row - pl * tpp) * kBlock;
+      page = p.indices[s_base[r] + pl];
+      return t == s_prefix[r + 1] - 1;
+    };
+    int page_n, tok_n;
+    bool last_n = look_up(lane, page_n, tok_n);
     if (lane == 0) prefetch_tensormap(&tmap);
     uint64_t evict_first;
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(evict_first));
-    int row = row_a;
     bool met = !p.early;
     int issued = 0;
-    for (int i = 0; i < n_tiles; ++i) {
-      const int64_t t = t_begin + i;
-      while (t >= s_prefix[row + 1]) ++row;
-      if (!met && t == s_prefix[row + 1] - 1) {  // a row's last tile may come from the previous grid
-        grid_dependency_wait();
-        met = true;
+    bool ready = true;
+    for (int i0 = 0; i0 < n_tiles && ready; i0 += 32) {
+      int page_c = page_n;
+      const int tok_c = tok_n;
+      const unsigned lasts = __ballot_sync(kFull, last_n);
+      if (i0 + lane < n_tiles && static_cast<unsigned>(page_c) >= static_cast<unsigned>(p.total_pages)) {
+        report(p.status, NQT_DEV_BAD_PAGE);
+        page_c = p.total_pages;
       }
-      const int s = i % STAGES;
-      const bool ready = i < STAGES || pipe_wait(&empty[s], ((i / STAGES) - 1) & 1, p);
-      if (!__all_sync(kFull, ready)) break;
-      const int in_row = static_cast<int>(t - s_prefix[row]);
-      const int pl = in_row / tpp;
-      const int pos = s_base[row] + pl;
-      int page = windowed ? s_pages[pos - win0] : p.indices[pos];
-      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.total_pages)) {
-        if (lane == 0) report(p.status, NQT_DEV_BAD_PAGE);
-        page = p.total_pages;  // a box outside the map: TMA fills zeros
+      last_n = look_up(i0 + 32 + lane, page_n, tok_n);
+      for (int u = 0; u < 32 && i0 + u < n_tiles; ++u) {
+        const int i = i0 + u, s = i % STAGES;
+        if (!met && (lasts >> u & 1u)) {  // a row's last tile may come from the previous grid
+          grid_dependency_wait();
+          met = true;
+        }
+        if (i >= STAGES) ready = pipe_wait(&empty[s], ((i / STAGES) - 1) & 1, p);
+        ready = __all_sync(kFull, ready);
+        if (!ready) break;
+        const int page = __shfl_sync(kFull, page_c, u), tok = __shfl_sync(kFull, tok_c, u);
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], Cfg::kStage);
+        __syncwarp();
+        if (lane < Cfg::kBoxes)
+          tma_tile(smem + s * Cfg::kStage + lane * Cfg::kBox, &tmap, &full[s], kv0 / Cfg::kBoxHeads + lane, tok,
+                   page * 2, evict_first);
+        issued = i + 1;
       }
-      if (lane == 0) mbar_arrive_expect_tx(&full[s], Cfg::kStage);
-      __syncwarp();
-      if (lane < HPC)
-        tma_tile(smem + s * Cfg::kStage + lane * Cfg::kBox, &tmap, &full[s], kv0 + lane, (in_row - pl * tpp) * kBlock,
-                 page * 2, evict_first);
-      issued = i + 1;
     }
     if (lane == 0) s_issued = issued;
   } else {
@@ -404,7 +431,8 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
       return p.indices[s_base[r] + static_cast<int>(t_begin + i - s_prefix[r]) / tpp];
     };
     auto tile_scales = [&](int i, int page, float& ks, float& vs) {
-      ks = vs = 0.f;
+      ks = 0.f;
+      vs = 1.f;  // a page outside the pool: keys and values of zeros
       if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.total_pages)) return;
       const int r = row_of_tile(s_prefix, p.batch, t_begin + i);
       const int blk = static_cast<int>(t_begin + i - s_prefix[r]) % tpp;
@@ -412,30 +440,59 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
       ks = __ldcg(sp);  // from L2: the previous grid may have written neighbouring scales
       vs = __ldcg(sp + static_cast<int64_t>(tpp) * p.hkv);
     };
-    int chunk = 0;  // the 32 tiles whose scales are in ks_c, vs_c
-    float ks_c, vs_c, ks_n, vs_n;
+    // what a tile needs of its scales, per lane of the chunk: score factor, log2 c, 1 / c
+    float ks_c, lc_c, rc_c;
+    auto take = [&](float ks, float vs) {
+      const float c = fmaxf(vs, 8.271806e-25f);  // 2^-80
+      ks_c = ks;
+      lc_c = log2f(c);
+      rc_c = __frcp_rn(c);
+    };
+    // query heads of the group: lane (g, t4) holds elements 16 ch + 4 t4 .. + 3 of head g
+    auto load_q = [&](int r, uint32_t (&qf)[CH][2]) {
+      const __nv_bfloat16* qrow = p.q + r * p.q_st + static_cast<int64_t>(kvh * group + g) * p.q_sh;
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) {
+        qf[ch][0] = qf[ch][1] = 0u;
+        if (g < group) {
+          qf[ch][0] = *reinterpret_cast<const uint32_t*>(qrow + ch * 16 + 4 * t4);
+          qf[ch][1] = *reinterpret_cast<const uint32_t*>(qrow + ch * 16 + 4 * t4 + 2);
+        }
+      }
+    };
+    int row = row_of_tile(s_prefix, p.batch, t_begin);
+    uint32_t qf[CH][2];
+
+    int chunk = 0;  // the 32 tiles whose factors are in ks_c, lc_c, rc_c; the next 32 scales are in ks_n, vs_n
+    float ks_n, vs_n;
     int page_nx = tile_page(lane);
     if (p.early) grid_dependency_wait();  // q, the last tiles' scales, the parts and tickets of the last launch
-    tile_scales(lane, page_nx, ks_c, vs_c);
+    load_q(row, qf);
+    bool q_ready = true;
+    tile_scales(lane, page_nx, ks_n, vs_n);
     page_nx = tile_page(32 + lane);
+    take(ks_n, vs_n);
     tile_scales(32 + lane, page_nx, ks_n, vs_n);
     page_nx = tile_page(64 + lane);
-    auto scales_of = [&](int i, float& ks, float& vs) {  // i does not fall
+    auto factors_of = [&](int i, float& ks, float& lc, float& rc) {  // i does not fall
       while (chunk < (i >> 5)) {
         ++chunk;
-        ks_c = ks_n;
-        vs_c = vs_n;
+        take(ks_n, vs_n);
         tile_scales((chunk + 1) * 32 + lane, page_nx, ks_n, vs_n);
         page_nx = tile_page((chunk + 2) * 32 + lane);
       }
       ks = __shfl_sync(kFull, ks_c, i & 31);
-      vs = __shfl_sync(kFull, vs_c, i & 31);
+      lc = __shfl_sync(kFull, lc_c, i & 31);
+      rc = __shfl_sync(kFull, rc_c, i & 31);
     };
 
     const int tok = ((lm_j & 1) << 3) + lm_r;  // ldmatrix row of this lane
-    const int sw = D == 128 ? (tok & 7) : ((tok >> 1) & 3);
-    const uint32_t box0 = smem_addr(smem) + hw * Cfg::kBox + tok * D;
-    int row = row_of_tile(s_prefix, p.batch, t_begin);
+    const int sw = Cfg::kBoxRow == 128 ? (tok & 7) : ((tok >> 1) & 3);
+    const uint32_t box0 = smem_addr(smem) + hw / Cfg::kBoxHeads * Cfg::kBox + tok * Cfg::kBoxRow;
+    uint32_t at[CH / 2];  // the lane's 16-byte chunk of each chunk pair, swizzled
+#pragma unroll
+    for (int i = 0; i < CH / 2; ++i)
+      at[i] = static_cast<uint32_t>((hw % Cfg::kBoxHeads * CH + 2 * i + (lm_j >> 1)) ^ sw) << 4;
     int fix_a = -1, fix_b = -1;  // split rows whose group's ticket this warp completed
     int stop = n_tiles;          // first tile of this warp that was not consumed
     bool dead = false;           // a wait gave up: the rows are still gone through, so that every ticket completes
@@ -448,19 +505,11 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
       const int valid_last = ends ? s_valid[row] : kBlock;
 
       // the row's query heads of the group, as B fragments in K's byte order, scaled to a maximum in [1, 2)
-      uint32_t qf[CH][2];
+      if (!q_ready) load_q(row, qf);
+      q_ready = false;
       float f0, f1;  // score factors of heads 2 t4, 2 t4 + 1: q's power of two, sm_scale, log2 e
       {
-        const __nv_bfloat16* qrow = p.q + row * p.q_st + static_cast<int64_t>(kvh * group + g) * p.q_sh;
         float amax = 0.f;
-#pragma unroll
-        for (int ch = 0; ch < CH; ++ch) {
-          qf[ch][0] = qf[ch][1] = 0u;
-          if (g < group) {
-            qf[ch][0] = *reinterpret_cast<const uint32_t*>(qrow + ch * 16 + 4 * t4);
-            qf[ch][1] = *reinterpret_cast<const uint32_t*>(qrow + ch * 16 + 4 * t4 + 2);
-          }
-        }
 #pragma unroll
         for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
@@ -491,9 +540,9 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
       for (int i = i0 + 2 * sub; i < i1 && !dead; i += 2 * kPerHead) {
         const bool two = i + 1 < i1;
         const int sA = i % STAGES, sB = (i + 1) % STAGES;
-        float ksA, vsA, ksB = 0.f, vsB = 0.f;
-        scales_of(i, ksA, vsA);
-        if (two) scales_of(i + 1, ksB, vsB);
+        float ksA, lcA, rcA, ksB = 0.f, lcB = 0.f, rcB = 0.f;
+        factors_of(i, ksA, lcA, rcA);
+        if (two) factors_of(i + 1, ksB, lcB, rcB);
         bool ok = pipe_wait(&full[sA], (i / STAGES) & 1, p);
         if (two) ok = pipe_wait(&full[sB], ((i + 1) / STAGES) & 1, p) && ok;
         if (!__all_sync(kFull, ok)) {
@@ -510,7 +559,7 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
 #pragma unroll
           for (int cc = 0; cc < CH; cc += 2) {
             uint32_t r0, r1, r2, r3, a0, a1, a2, a3;
-            ldmatrix_x4(r0, r1, r2, r3, krow + (((cc + (lm_j >> 1)) ^ sw) << 4));
+            ldmatrix_x4(r0, r1, r2, r3, krow + at[cc / 2]);
             codes_to_f16_rows<E4M3>(r0, a0, a2);
             codes_to_f16_rows<E4M3>(r1, a1, a3);
             mma_f16_16816(s, a0, a1, a2, a3, qf[cc][0], qf[cc][1]);
@@ -530,17 +579,17 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
         const int validB = two ? (i + 2 == i1 ? valid_last : kBlock) : 0;
         {
           const float c0 = ksA * f0, c1 = ksA * f1;
-          sa[0] = g < validA ? sa[0] * c0 : NEG_INF;
-          sa[1] = g < validA ? sa[1] * c1 : NEG_INF;
-          sa[2] = g + 8 < validA ? sa[2] * c0 : NEG_INF;
-          sa[3] = g + 8 < validA ? sa[3] * c1 : NEG_INF;
+          sa[0] = g < validA ? fmaf(sa[0], c0, lcA) : NEG_INF;
+          sa[1] = g < validA ? fmaf(sa[1], c1, lcA) : NEG_INF;
+          sa[2] = g + 8 < validA ? fmaf(sa[2], c0, lcA) : NEG_INF;
+          sa[3] = g + 8 < validA ? fmaf(sa[3], c1, lcA) : NEG_INF;
         }
         if (two) {
           const float c0 = ksB * f0, c1 = ksB * f1;
-          sb[0] = g < validB ? sb[0] * c0 : NEG_INF;
-          sb[1] = g < validB ? sb[1] * c1 : NEG_INF;
-          sb[2] = g + 8 < validB ? sb[2] * c0 : NEG_INF;
-          sb[3] = g + 8 < validB ? sb[3] * c1 : NEG_INF;
+          sb[0] = g < validB ? fmaf(sb[0], c0, lcB) : NEG_INF;
+          sb[1] = g < validB ? fmaf(sb[1], c1, lcB) : NEG_INF;
+          sb[2] = g + 8 < validB ? fmaf(sb[2], c0, lcB) : NEG_INF;
+          sb[3] = g + 8 < validB ? fmaf(sb[3], c1, lcB) : NEG_INF;
         }
         float x0 = fmaxf(fmaxf(sa[0], sa[2]), fmaxf(sb[0], sb[2]));
         float x1 = fmaxf(fmaxf(sa[1], sa[3]), fmaxf(sb[1], sb[3]));
@@ -564,14 +613,13 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
             o[ch][3] *= a1;
           }
         }
-        // p is held 2^8 above its value: fp16 then reaches down to 2^-32 of the reference
         const float r0 = m0 - 8.f, r1 = m1 - 8.f;
 
-        // O^T[d][head] += c * sum_tok V[tok][d] P[head][tok]; rows g and g + 8 of a chunk are its dims 2g and 2g + 1
-        auto add_values = [&](uint32_t vrow, const float (&s)[4], float vs, int valid) {
+        // O^T[d][head] += sum_tok V[tok][d] P'[head][tok]; rows g and g + 8 of a chunk are its dims 2g and 2g + 1
+        auto add_values = [&](uint32_t vrow, const float (&s)[4], float rc, int valid) {
           const float p0 = ex2(s[0] - r0), p1 = ex2(s[1] - r1), p2 = ex2(s[2] - r0), p3 = ex2(s[3] - r1);
-          l0 += p0 + p2;
-          l1 += p1 + p3;
+          l0 = fmaf(p0 + p2, rc, l0);
+          l1 = fmaf(p1 + p3, rc, l1);
           const uint32_t b0 = movmatrix_trans(pack_f16x2(p0, p1)), b1 = movmatrix_trans(pack_f16x2(p2, p3));
           // e4m3 codes behind the row's end may be NaN codes: they count as zeros
           uint32_t k0 = 0xffffffffu, k1 = 0xffffffffu;
@@ -582,23 +630,17 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
 #pragma unroll
           for (int cc = 0; cc < CH; cc += 2) {
             uint32_t v0, v1, v2, v3, a0, a1, a2, a3;
-            ldmatrix_x4_trans(v0, v1, v2, v3, vrow + (((cc + (lm_j >> 1)) ^ sw) << 4));
-            float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
+            ldmatrix_x4_trans(v0, v1, v2, v3, vrow + at[cc / 2]);
             codes_to_f16_cols<E4M3>(v0, a0, a1);
             codes_to_f16_cols<E4M3>(v1, a2, a3);
-            mma_f16_16816(d, a0 & k0, a1 & k0, a2 & k1, a3 & k1, b0, b1);
+            mma_f16_16816(o[cc], a0 & k0, a1 & k0, a2 & k1, a3 & k1, b0, b1);
             codes_to_f16_cols<E4M3>(v2, a0, a1);
             codes_to_f16_cols<E4M3>(v3, a2, a3);
-            mma_f16_16816(e, a0 & k0, a1 & k0, a2 & k1, a3 & k1, b0, b1);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              o[cc][x] = fmaf(vs, d[x], o[cc][x]);
-              o[cc + 1][x] = fmaf(vs, e[x], o[cc + 1][x]);
-            }
+            mma_f16_16816(o[cc + 1], a0 & k0, a1 & k0, a2 & k1, a3 & k1, b0, b1);
           }
         };
-        add_values(rowA + kBlock * D, sa, vsA, validA);
-        if (two) add_values(rowB + kBlock * D, sb, vsB, validB);
+        add_values(rowA + kBlock * Cfg::kBoxRow, sa, rcA, validA);
+        if (two) add_values(rowB + kBlock * Cfg::kBoxRow, sb, rcB, validB);
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&empty[sA]);
@@ -676,11 +718,11 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
             if (has1) __stcg(reinterpret_cast<float2*>(po + D + ch * 16), make_float2(o[ch][1] * v1, o[ch][3] * v1));
           }
           if (g == 0) {
-            if (has0) __stcg(pl, m0 + log2f(t0));
-            if (has1) __stcg(pl + 1, m1 + log2f(t1));
+            if (has0) __stcg(pl, m0 - 8.f + log2f(t0));
+            if (has1) __stcg(pl + 1, m1 - 8.f + log2f(t1));
           }
           __syncwarp();
-          const int lo = max(ca, c / kGroup8 * kGroup8), hi = min(cb, c / kGroup8 * kGroup8 + kGroup8 - 1);
+          const int lo = c - (c - ca) % kGroup8, hi = min(cb, lo + kGroup8 - 1);  // the CTAs joined with this one
           if (count_in(p.group_tickets + static_cast<int64_t>(part_slot(lo, ca, late)) * p.hq + kvh, hi - lo,
                        lane)) {
             if (fix_a < 0) fix_a = row;  // only a range's first and last rows can be split
@@ -698,9 +740,9 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
       if (r < 0) continue;
       const int64_t r0 = s_prefix[r], r1 = s_prefix[r + 1];
       const int ca = tile_owner(total, n, r0), cb = tile_owner(total, n, r1 - 1);
-      const int lo = max(ca, c / kGroup8 * kGroup8), hi = min(cb, c / kGroup8 * kGroup8 + kGroup8 - 1);
+      const int lo = c - (c - ca) % kGroup8, hi = min(cb, lo + kGroup8 - 1);
       const bool late = first_tile(total, ca, n) < r0;
-      const int groups = cb / kGroup8 - ca / kGroup8;  // less one
+      const int groups = (cb - ca) / kGroup8;  // less one
       join_parts<D>(p, r, kvh, hi - lo + 1, [&](int i) { return part_slot(lo + i, ca, late); }, groups == 0,
                     part_slot(lo, ca, late), lane);
       if (groups == 0) continue;
@@ -708,7 +750,7 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
       if (count_in(p.tickets + static_cast<int64_t>(r) * p.hq + kvh, groups, lane))
         join_parts<D>(
             p, r, kvh, groups + 1,
-            [&](int i) { return part_slot(i == 0 ? ca : (ca / kGroup8 + i) * kGroup8, ca, late); }, true, 0, lane);
+            [&](int i) { return part_slot(ca + i * kGroup8, ca, late); }, true, 0, lane);
     }
     if (lane == 0) s_progress[warp] = stop;
   }
@@ -721,25 +763,31 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
   }
 }
 
-int encode_tiles(CUtensorMap* map, const void* layer, int total_pages, int page_size, int hkv, int d) {
+// The layer as {bytes of `heads` heads, groups of heads, P, pages x 2} in boxes of one group x 16 tokens x K and V.
+int encode_tiles(CUtensorMap* map, const void* layer, int total_pages, int page_size, int hkv, int d, int heads) {
   auto encode = c8::get_encode();
   if (encode == nullptr) return NQT_ERR_CUDA;
-  const cuuint64_t D = static_cast<cuuint64_t>(d);
-  cuuint64_t dims[4] = {D, static_cast<cuuint64_t>(hkv), static_cast<cuuint64_t>(page_size),
+  const cuuint64_t row = static_cast<cuuint64_t>(heads) * d;
+  cuuint64_t dims[4] = {row, static_cast<cuuint64_t>(hkv / heads), static_cast<cuuint64_t>(page_size),
                         static_cast<cuuint64_t>(total_pages) * 2};
-  cuuint64_t strides[3] = {D, static_cast<cuuint64_t>(hkv) * D, static_cast<cuuint64_t>(page_size) * hkv * D};
-  cuuint32_t box[4] = {static_cast<cuuint32_t>(d), 1, kBlock, 2};
+  cuuint64_t strides[3] = {row, static_cast<cuuint64_t>(hkv) * d, static_cast<cuuint64_t>(page_size) * hkv * d};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(row), 1, kBlock, 2};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r =
       encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(layer), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? NQT_OK : NQT_ERR_CUDA;
 }
 
 template <int D, int HPC, int STAGES, bool E4M3>
-int launch8(const CUtensorMap& map, Decode8Args a, cudaStream_t s) {
+int launch8(const void* layer, Decode8Args a, cudaStream_t s) {
   using Cfg = Cfg8<D, HPC, STAGES>;
+  CUtensorMap map;
+  if (encode_tiles(&map, layer, a.total_pages, a.page_size, a.hkv, D, Cfg::kBoxHeads) != NQT_OK) {
+    set_last_message("decode_attention8: cuTensorMapEncodeTiled failed");
+    return NQT_ERR_CUDA;
+  }
   static int few_occ = 1;
   static std::once_flag once;
   auto occupancy = [](int smem) {
@@ -771,11 +819,11 @@ int launch8(const CUtensorMap& map, Decode8Args a, cudaStream_t s) {
 }
 
 template <int D, bool E4M3>
-int dispatch8(const CUtensorMap& map, const Decode8Args& a, cudaStream_t s) {
+int dispatch8(const void* layer, const Decode8Args& a, cudaStream_t s) {
   constexpr int kDeep = 128 / D;  // stages of D = 64 hold half the bytes
-  if (a.hkv % 4 == 0) return launch8<D, 4, 4 * kDeep, E4M3>(map, a, s);
-  if (a.hkv % 2 == 0) return launch8<D, 2, 8 * kDeep, E4M3>(map, a, s);
-  return launch8<D, 1, 16 * kDeep, E4M3>(map, a, s);
+  if (a.hkv % 4 == 0) return launch8<D, 4, 4 * kDeep, E4M3>(layer, a, s);
+  if (a.hkv % 2 == 0) return launch8<D, 2, 8 * kDeep, E4M3>(layer, a, s);
+  return launch8<D, 1, 16 * kDeep, E4M3>(layer, a, s);
 }
 
 }  // namespace
@@ -808,12 +856,6 @@ extern "C" int nqt_decode_attention8(const void* q, int64_t q_stride_tok, int64_
   if (workspace_bytes < w.total) return NQT_ERR_CAPACITY;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return NQT_ERR_ARG;
   if (batch == 0) return NQT_OK;
-  CUtensorMap map;
-  rc = encode_tiles(&map, layer_cache, total_pages, page_size, num_kv_heads, head_dim);
-  if (rc != NQT_OK) {
-    set_last_message("decode_attention8: cuTensorMapEncodeTiled failed");
-    return rc;
-  }
   uint8_t* base = static_cast<uint8_t*>(workspace);
   Decode8Args a{};
   a.q = static_cast<const __nv_bfloat16*>(q);
@@ -842,6 +884,6 @@ extern "C" int nqt_decode_attention8(const void* q, int64_t q_stride_tok, int64_
   a.wait_ns = (flags & NQT_DECODE_SHORT_WAIT) ? 0 : kWaitLimitNs;
   cudaStream_t s = as_stream(stream);
   if (head_dim == 128)
-    return code == NQT_E4M3 ? dispatch8<128, true>(map, a, s) : dispatch8<128, false>(map, a, s);
-  return code == NQT_E4M3 ? dispatch8<64, true>(map, a, s) : dispatch8<64, false>(map, a, s);
+    return code == NQT_E4M3 ? dispatch8<128, true>(layer_cache, a, s) : dispatch8<128, false>(layer_cache, a, s);
+  return code == NQT_E4M3 ? dispatch8<64, true>(layer_cache, a, s) : dispatch8<64, false>(layer_cache, a, s);
 }
