@@ -97,6 +97,13 @@ __device__ __forceinline__ uint32_t f32_to_code(float x) {
   return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(x, -127.f), 127.f))) & 0xffu;
 }
 
+// Two codes, the first in the low byte.
+template <bool E4M3>
+__device__ __forceinline__ uint16_t codes_of_pair(float a, float b) {
+  if (E4M3) return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  return static_cast<uint16_t>(f32_to_code<false>(a) | (f32_to_code<false>(b) << 8));
+}
+
 // ---- host --------------------------------------------------------------------------
 inline PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
