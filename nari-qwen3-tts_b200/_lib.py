@@ -7,6 +7,8 @@ call raises.  ``lib()`` loads the in-tree library once per process.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import threading
 from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
@@ -14,6 +16,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libnqt.so"
+BIND_PATH = Path(__file__).resolve().parent / "_nqt_bind.so"
 
 NQT_OK = 0
 NQT_ERR_ARG = -1
@@ -170,6 +173,47 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+# entry points that the C++ binding (csrc/bind.cpp) calls, in its order
+_BOUND = ("nqt_decode_attention8", "nqt_prefill_attention8", "nqt_qk_norm_rope_paged_cache8", "nqt_read_paged_cache8",
+          "nqt_gemm_int8", "nqt_linear_int8")
+_bind = None
+
+
+def bind():
+    """The C++ entry of the 8-bit operators (loaded once): the same C ABI, with the checks and the launch in C++."""
+
+    global _bind
+    if _bind is None:
+        if not BIND_PATH.exists():
+            raise ImportError(
+                f"{BIND_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`"
+            )
+        handle = lib()
+        loader = importlib.machinery.ExtensionFileLoader("_nqt_bind", str(BIND_PATH))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_nqt_bind", loader))
+        loader.exec_module(module)
+        module.init(*(ctypes.cast(getattr(handle, name), c_void_p).value for name in _BOUND))
+        with _lock:
+            if _bind is None:
+                _bind = module
+    return _bind
+
+
+def settle(fn, name: str, rc: int, args: tuple):
+    """What a binding call that answered with a code becomes: the call again once its device has a status word, or
+    NqtError."""
+
+    if rc <= -1000:
+        from .kernels import device_status
+
+        index = -1000 - rc
+        bind().set_status(index, device_status(torch.device("cuda", index)).data_ptr())
+        rc = fn(*args)
+        if not isinstance(rc, int):
+            return rc
+    raise NqtError(name, rc, (lib().nqt_last_error() or b"").decode(errors="replace") if rc == NQT_ERR_CUDA else "")
+
+
 def exported_symbols() -> list[str]:
     return list(SIGNATURES)
 
@@ -185,12 +229,14 @@ _launches = 0
 def reset_launch_count() -> None:
     global _launches
     _launches = 0
+    if _bind is not None:
+        _bind.launches(True)
 
 
 def launch_count() -> int:
     """libnqt kernel launches issued since the last reset (graph capture included)."""
 
-    return _launches
+    return _launches + (_bind.launches() if _bind is not None else 0)
 
 
 def call(name: str, *args) -> int:

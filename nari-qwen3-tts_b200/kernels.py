@@ -34,18 +34,6 @@ def device_status(device: torch.device) -> torch.Tensor:
     return word
 
 
-_STATUS_PTR: dict[int, int] = {}
-
-
-def status_ptr(index: int) -> int:
-    """Address of ``device_status`` of CUDA device ``index``."""
-
-    p = _STATUS_PTR.get(index)
-    if p is None:
-        p = _STATUS_PTR[index] = device_status(torch.device("cuda", index)).data_ptr()
-    return p
-
-
 def read_status(device: torch.device) -> int:
     """Host read of the status word (synchronises); 0 means no device error."""
 
@@ -353,49 +341,11 @@ def paired_qk_norm_rope_paged_cache8(
     again.  The tokens of one block have to follow one another in the call, at rising offsets, which is the
     planner's order."""
 
-    if query.ndim != 3 or key.ndim != 3 or value.ndim != 3:
-        raise ValueError("Qwen3-TTS QKV tensors must have rank three")
-    tokens, query_heads, head_dim = query.shape
-    if key.shape != value.shape or key.shape[0] != tokens or key.shape[2] != head_dim:
-        raise ValueError("Qwen3-TTS QKV shapes are incompatible")
-    key_heads = key.shape[1]
-    if not (query.dtype == key.dtype == value.dtype == torch.bfloat16):
-        raise TypeError("8-bit paged staging takes bf16 query, key and value")
-    code = check_cache8(layer_cache, layer_scales, key_heads, head_dim)
-    if query_weight.shape != (head_dim,) or key_weight.shape != (head_dim,):
-        raise ValueError("QK norm weights must match the head dimension")
-    if position_ids.shape != (tokens,) or write_pages.shape != (tokens,) or write_offsets.shape != (tokens,):
-        raise ValueError("paged QKV metadata must contain one entry per token")
-    if query.stride(2) != 1 or key.stride(2) != 1 or value.stride(2) != 1:
-        raise ValueError("QKV must be contiguous per head")
-    for t in (position_ids, write_pages, write_offsets):
-        if t.dtype != torch.long or not t.is_contiguous():
-            raise TypeError("paged QKV metadata must be contiguous int64")
-    if out is not None and (out.shape != query.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1):
-        raise ValueError("the rotated query must be bf16 of the query's shape, contiguous per head")
-    index = _lib.cuda_index(query, key, value, query_weight, key_weight, position_ids, layer_cache, layer_scales,
-                            write_pages, write_offsets, out)
-    if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    if tokens == 0:
-        return out
-    if query_weight.dtype != torch.bfloat16 or not query_weight.is_contiguous():
-        query_weight = query_weight.to(torch.bfloat16).contiguous()
-    if key_weight.dtype != torch.bfloat16 or not key_weight.is_contiguous():
-        key_weight = key_weight.to(torch.bfloat16).contiguous()
-    _lib.call_on(
-        index, "nqt_qk_norm_rope_paged_cache8",
-        query.data_ptr(), query.stride(0), query.stride(1),
-        key.data_ptr(), key.stride(0), key.stride(1),
-        value.data_ptr(), value.stride(0), value.stride(1),
-        query_weight.data_ptr(), key_weight.data_ptr(),
-        position_ids.data_ptr(), write_pages.data_ptr(), write_offsets.data_ptr(),
-        out.data_ptr(), out.stride(0), out.stride(1),
-        layer_cache.data_ptr(), layer_scales.data_ptr(), layer_cache.shape[0], layer_cache.shape[2],
-        tokens, query_heads, key_heads, head_dim,
-        float(epsilon), float(rope_theta), code, status_ptr(index), _lib.raw_stream(index),
-    )
-    return out
+    args = (query, key, value, query_weight, key_weight, position_ids, epsilon, rope_theta, layer_cache, layer_scales,
+            write_pages, write_offsets, out)
+    fn = (_lib._bind or _lib.bind()).write8
+    r = fn(*args)
+    return r if r.__class__ is not int else _lib.settle(fn, "nqt_qk_norm_rope_paged_cache8", r, args)
 
 
 def read_paged_cache8(layer_cache: torch.Tensor, layer_scales: torch.Tensor, pages: torch.Tensor, *,
@@ -403,22 +353,10 @@ def read_paged_cache8(layer_cache: torch.Tensor, layer_scales: torch.Tensor, pag
     """Pages of an 8-bit cache layer as bf16 [n, 2, P, Hkv, D] (a bf16 pool's layout): to move a request's KV to
     a bf16 pool or off the device.  ``pages``: int64 [n] page ids."""
 
-    if layer_cache.ndim != 5:
-        raise ValueError("8-bit paged cache must be [pages, 2, page_size, kv_heads, head_dim]")
-    code = check_cache8(layer_cache, layer_scales, layer_cache.shape[3], layer_cache.shape[4])
-    if pages.ndim != 1 or pages.dtype != torch.long or not pages.is_contiguous():
-        raise TypeError("page ids must be contiguous int64 [n]")
-    shape = (pages.shape[0], *layer_cache.shape[1:])
-    if out is not None and (out.shape != shape or out.dtype != torch.bfloat16 or not out.is_contiguous()):
-        raise ValueError("read_paged_cache8 output must be contiguous bf16 [n, 2, page_size, kv_heads, head_dim]")
-    index = _lib.cuda_index(layer_cache, layer_scales, pages, out)
-    if out is None:
-        out = layer_cache.new_empty(shape, dtype=torch.bfloat16)
-    if pages.shape[0]:
-        _lib.call_on(index, "nqt_read_paged_cache8", layer_cache.data_ptr(), layer_scales.data_ptr(),
-                     layer_cache.shape[0], layer_cache.shape[2], layer_cache.shape[3], layer_cache.shape[4], code,
-                     pages.data_ptr(), pages.shape[0], out.data_ptr(), status_ptr(index), _lib.raw_stream(index))
-    return out
+    args = (layer_cache, layer_scales, pages, out)
+    fn = (_lib._bind or _lib.bind()).read8
+    r = fn(*args)
+    return r if r.__class__ is not int else _lib.settle(fn, "nqt_read_paged_cache8", r, args)
 
 
 __all__ = [
@@ -791,7 +729,6 @@ class Int8Weight:
             self.data = torch.zeros((n, pitch), dtype=torch.int8, device=q.device)
             self.data[:, :k] = q
             self.data_scale = scale.contiguous()
-        self.rows, self.pitch = self.data.shape[0], _row_pitch(self.data)
 
     @property
     def shape(self) -> tuple[int, int]:
@@ -808,38 +745,7 @@ def linear_int8(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
 
     if not isinstance(weight, Int8Weight):
         raise TypeError("linear_int8 takes an Int8Weight")
-    if x.dim() != 2 or x.shape[1] != weight.k or (x.stride(1) != 1 and weight.k > 1):
-        raise ValueError("linear_int8 needs x [m, k] matching the weight, with unit stride along k")
-    m, k = x.shape
-    if bias is not None:
-        if weight.gate_up:
-            raise ValueError("the silu_mul epilogue takes no bias")
-        if bias.dtype != torch.bfloat16 or bias.shape != (weight.n,) or not bias.is_contiguous():
-            raise ValueError("linear_int8 bias must be contiguous bf16 [n]")
-    if out is not None and (out.shape != (m, weight.cols) or out.dtype != torch.bfloat16
-                            or (out.stride(1) != 1 and weight.cols > 1)):
-        raise ValueError("linear_int8 output must be bf16 [m, n] with unit column stride")
-    epilogue = GEMM_SILU_MUL if weight.gate_up else (GEMM_PLAIN if bias is None else GEMM_BIAS)
-    index = _lib.cuda_index(x, weight.data, bias, xscale, out)
-    if out is None:
-        out = x.new_empty((m, weight.cols), dtype=torch.bfloat16)
-    if m == 0:
-        return out
-    tail = (weight.data.data_ptr(), weight.pitch, weight.data_scale.data_ptr(), ptr(bias), out.data_ptr(),
-            _row_pitch(out), m, weight.rows, weight.cols, k, epilogue, status_ptr(index), _lib.raw_stream(index))
-    if x.dtype == torch.bfloat16:
-        if xscale is not None:
-            raise ValueError("xscale belongs to int8 codes")
-        pitch = (k + 15) // 16 * 16
-        scratch = x.new_empty(m * (pitch + 4), dtype=torch.uint8)
-        codes = scratch.data_ptr()
-        _lib.call_on(index, "nqt_linear_int8", x.data_ptr(), _row_pitch(x), codes, pitch, codes + m * pitch, *tail)
-        return out
-    if x.dtype != torch.int8 or xscale is None:
-        raise TypeError("linear_int8 takes bf16 rows, or int8 codes with their xscale")
-    if xscale.dtype != torch.float32 or xscale.shape != (m,) or not xscale.is_contiguous():
-        raise ValueError("linear_int8 xscale must be contiguous float32 [m]")
-    if _row_pitch(x) % 16 or x.data_ptr() % 16:
-        raise ValueError("linear_int8 codes need 16-byte aligned rows")
-    _lib.call_on(index, "nqt_gemm_int8", x.data_ptr(), _row_pitch(x), xscale.data_ptr(), *tail)
-    return out
+    args = (x, weight.data, weight.data_scale, weight.k, weight.cols, weight.gate_up, bias, xscale, out)
+    fn = (_lib._bind or _lib.bind()).linear8
+    r = fn(*args)
+    return r if r.__class__ is not int else _lib.settle(fn, "nqt_linear_int8", r, args)

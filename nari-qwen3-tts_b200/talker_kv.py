@@ -38,7 +38,7 @@ import torch
 
 from . import _lib
 from ._lib import call, ptr
-from .kernels import check_cache8, device_status, paired_qk_norm_rope_paged_cache_, status_ptr
+from .kernels import device_status, paired_qk_norm_rope_paged_cache_
 
 # nqt_decode_attention_ex flags (include/nqt.h NQT_DECODE_OVERLAP_KV_WRITE, NQT_DECODE_SHORT_WAIT)
 DECODE_OVERLAP_KV_WRITE = 0x1
@@ -178,33 +178,6 @@ def batch_prefill_paged(
     return out
 
 
-def _check_paged8(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, rows, out):
-    if query.ndim != 3 or layer_cache.ndim != 5:
-        raise ValueError("8-bit paged attention takes query [tokens, heads, head_dim] and a rank-five cache")
-    _, hq, d = query.shape
-    hkv = layer_cache.shape[3]
-    if hq % hkv or hq // hkv > 8:
-        raise ValueError("8-bit paged attention needs 1 to 8 query heads per KV head")
-    if query.dtype != torch.bfloat16:
-        raise TypeError("8-bit paged attention runs on a bf16 query")
-    code = check_cache8(layer_cache, layer_scales, hkv, d)
-    if query.stride(2) != 1:
-        raise ValueError("query must be contiguous per head")
-    for t in (kv_indptr, kv_indices, last_page_len):
-        if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous():
-            raise TypeError("paged KV metadata must be contiguous int32")
-    if kv_indptr.shape[0] < rows + 1 or last_page_len.shape[0] < rows:
-        raise ValueError("paged KV metadata must cover every row")
-    if out is not None and (out.shape != query.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1):
-        raise ValueError("attention output must be bf16 of the query's shape, contiguous per head")
-    return code
-
-
-def _table_ptr(kv_indices: torch.Tensor, kv_indptr: torch.Tensor) -> int:
-    # no row has a page: the empty table has no address, and nothing reads one
-    return kv_indices.data_ptr() if kv_indices.numel() else kv_indptr.data_ptr()
-
-
 def decode_paged8_workspace(batch_capacity: int, num_qo_heads: int, head_dim: int,
                             device: torch.device) -> torch.Tensor:
     """The zeroed workspace of ``batch_decode_paged8`` for up to ``batch_capacity`` rows: make it once, outside
@@ -239,27 +212,11 @@ def batch_decode_paged8(
     ``short_wait`` as in ``batch_decode_paged``; the scales of each row's last 16-token block count as its last
     tile."""
 
-    rows = query.shape[0]
-    code = _check_paged8(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, rows, out)
-    index = _lib.cuda_index(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, workspace, out)
-    if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    if rows == 0:
-        return out
-    _, hq, d = query.shape
-    _lib.call_on(
-        index, "nqt_decode_attention8",
-        query.data_ptr(), query.stride(0), query.stride(1),
-        layer_cache.data_ptr(), layer_scales.data_ptr(), layer_cache.shape[0], layer_cache.shape[2],
-        kv_indptr.data_ptr(), _table_ptr(kv_indices, kv_indptr), last_page_len.data_ptr(),
-        rows, batch_capacity or rows, hq, layer_cache.shape[3], d,
-        d**-0.5 if sm_scale is None else float(sm_scale), code,
-        out.data_ptr(), out.stride(0), out.stride(1),
-        workspace.data_ptr(), workspace.nbytes,
-        (DECODE_OVERLAP_KV_WRITE if overlap_kv_write else 0) | (DECODE_SHORT_WAIT if short_wait else 0),
-        status_ptr(index), _lib.raw_stream(index),
-    )
-    return out
+    args = (query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, workspace, batch_capacity, sm_scale,
+            out, (DECODE_OVERLAP_KV_WRITE if overlap_kv_write else 0) | (DECODE_SHORT_WAIT if short_wait else 0))
+    fn = (_lib._bind or _lib.bind()).decode8
+    r = fn(*args)
+    return r if r.__class__ is not int else _lib.settle(fn, "nqt_decode_attention8", r, args)
 
 
 def batch_prefill_paged8(
@@ -279,33 +236,10 @@ def batch_prefill_paged8(
     to kv_len - n + i.  Queries that see no key give zeros; tokens behind ``qo_indptr[batch]`` are not written.  A
     query whose rows are not 16-byte aligned is copied first."""
 
-    rows = batch if batch is not None else qo_indptr.shape[0] - 1
-    code = _check_paged8(query, layer_cache, layer_scales, kv_indptr, kv_indices, last_page_len, rows, out)
-    if qo_indptr.dtype != torch.int32 or qo_indptr.ndim != 1 or not qo_indptr.is_contiguous():
-        raise TypeError("paged KV metadata must be contiguous int32")
-    if qo_indptr.shape[0] < rows + 1:
-        raise ValueError("paged KV metadata must cover every row")
-    if sm_scale is not None and not sm_scale >= 0:
-        raise ValueError("prefill attention needs sm_scale >= 0")
-    index = _lib.cuda_index(query, layer_cache, layer_scales, qo_indptr, kv_indptr, kv_indices, last_page_len, out)
-    if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    tokens, hq, d = query.shape
-    if tokens == 0 or rows == 0:
-        return out
-    if query.data_ptr() % 16 or query.stride(0) % 8 or query.stride(1) % 8:
-        query = query.clone(memory_format=torch.contiguous_format)
-    _lib.call_on(
-        index, "nqt_prefill_attention8",
-        query.data_ptr(), query.stride(0), query.stride(1),
-        layer_cache.data_ptr(), layer_scales.data_ptr(), layer_cache.shape[0], layer_cache.shape[2],
-        qo_indptr.data_ptr(), kv_indptr.data_ptr(), _table_ptr(kv_indices, kv_indptr), last_page_len.data_ptr(),
-        rows, tokens, hq, layer_cache.shape[3], d,
-        d**-0.5 if sm_scale is None else float(sm_scale), code,
-        out.data_ptr(), out.stride(0), out.stride(1),
-        status_ptr(index), _lib.raw_stream(index),
-    )
-    return out
+    args = (query, layer_cache, layer_scales, qo_indptr, kv_indptr, kv_indices, last_page_len, batch, sm_scale, out)
+    fn = (_lib._bind or _lib.bind()).prefill8
+    r = fn(*args)
+    return r if r.__class__ is not int else _lib.settle(fn, "nqt_prefill_attention8", r, args)
 
 
 class B200TalkerBinding:
