@@ -19,7 +19,16 @@
 // epilogue runs under the next tile's products.  Tokens are the MMA's rows: an
 // epilogue thread owns one token, its scale is one register, the weights' scales
 // are broadcast from shared memory, and gate and up columns (interleaved in groups
-// of 16 rows when the weight is laid out) meet in the same thread.
+// of 16 rows when the weight is laid out) meet in the same thread.  TN is chosen
+// per call (pick_tn): every SM should have a tile, of as many columns as that
+// allows, because a tile's tokens are read again for each.  A decode batch loads
+// only its own token rows; the MMA's other rows read whatever lies behind them in
+// shared memory, into accumulators that nobody reads.
+//
+// Up to 8 tokens the product is a stream of the weights: no tensor core, no
+// second launch.  Every CTA quantises the tokens for itself (they are a few KB),
+// its first weights already on their way, and a warp takes two weight rows at a
+// time (gate and up of one column) with dp4a.
 #include <mutex>
 
 #include "common.cuh"
@@ -32,6 +41,45 @@ namespace {
 using namespace gemm_detail;
 
 // ------------------------------------------------------------------ quantiser
+// The rule of a row whose largest |bf16| bits are `mx`: scale, factor and the code of a value.
+struct RowRule {
+  float s, f;
+  bool tiny;  // 127 / amax overflows: divide by the (subnormal) scale instead
+  __device__ __forceinline__ explicit RowRule(uint32_t mx) {
+    const float amax = __uint_as_float(mx << 16);
+    s = __fdiv_rn(amax, 127.f);
+    f = amax == 0.f ? 0.f : __fdiv_rn(127.f, amax);
+    tiny = f > 3.0e38f;
+  }
+  __device__ __forceinline__ uint32_t code(uint32_t bf16_bits) const {
+    const float v = __uint_as_float(bf16_bits << 16);
+    const float t = tiny ? fminf(fmaxf(__fdiv_rn(v, s), -127.f), 127.f) : v * f;
+    return static_cast<uint32_t>(__float2int_rn(t)) & 0xffu;
+  }
+  // eight bf16 -> eight codes
+  __device__ __forceinline__ uint2 codes(uint4 w) const {
+    return make_uint2(code(w.x & 0xffffu) | (code(w.x >> 16) << 8) | (code(w.y & 0xffffu) << 16) | (code(w.y >> 16) << 24),
+                      code(w.z & 0xffffu) | (code(w.z >> 16) << 8) | (code(w.w & 0xffffu) << 16) | (code(w.w >> 16) << 24));
+  }
+};
+
+__device__ __forceinline__ uint32_t magnitude2(uint4 v, uint32_t m2) {
+  m2 = __vmaxu2(m2, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
+  return __vmaxu2(m2, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+}
+
+// Vector v (8 elements) of a row of k; elements behind the row are zeros.
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* src, int v, int k) {
+  if (VEC) return *reinterpret_cast<const uint4*>(src + v * 8);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  const uint16_t* e = reinterpret_cast<const uint16_t*>(src) + v * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (v * 8 + i < k) w[i / 2] |= static_cast<uint32_t>(e[i]) << (16 * (i & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // One row by TPR threads; up to 4 vectors of 8 elements per thread stay in registers between the two passes,
 // longer rows are read again (from L2).
 template <int TPR, bool VEC>
@@ -47,19 +95,7 @@ __global__ void __launch_bounds__(256) int8_quantize_rows_kernel(const __nv_bflo
   const __nv_bfloat16* src = x + (live ? row : 0) * ldx;
   const int vecs = live ? (k + 7) / 8 : 0;
 
-  auto load = [&](int v) -> uint4 {
-    if (VEC) return *reinterpret_cast<const uint4*>(src + v * 8);
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-    const uint16_t* e = reinterpret_cast<const uint16_t*>(src) + v * 8;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (v * 8 + i < k) w[i / 2] |= static_cast<uint32_t>(e[i]) << (16 * (i & 1));
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  };
-  auto magnitude = [](uint4 v, uint32_t m2) {
-    m2 = __vmaxu2(m2, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
-    return __vmaxu2(m2, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
-  };
+  auto load = [&](int v) -> uint4 { return load8<VEC>(src, v, k); };
   uint4 keep[kKeep];
   uint32_t m2 = 0;
 #pragma unroll
@@ -67,9 +103,9 @@ __global__ void __launch_bounds__(256) int8_quantize_rows_kernel(const __nv_bflo
     const int v = lt + i * TPR;
     keep[i] = make_uint4(0u, 0u, 0u, 0u);
     if (v < vecs) keep[i] = load(v);
-    m2 = magnitude(keep[i], m2);
+    m2 = magnitude2(keep[i], m2);
   }
-  for (int v = lt + kKeep * TPR; v < vecs; v += TPR) m2 = magnitude(load(v), m2);
+  for (int v = lt + kKeep * TPR; v < vecs; v += TPR) m2 = magnitude2(load(v), m2);
   uint32_t mx = max(m2 & 0xffffu, m2 >> 16);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(kFull, mx, o));
@@ -80,26 +116,17 @@ __global__ void __launch_bounds__(256) int8_quantize_rows_kernel(const __nv_bflo
     for (int w = 0; w < 8; ++w) mx = max(mx, s_max[w]);
   }
   if (!live) return;
-  const float amax = __uint_as_float(mx << 16);
-  const float s = __fdiv_rn(amax, 127.f);
-  const float f = amax == 0.f ? 0.f : __fdiv_rn(127.f, amax);
-  const bool tiny = f > 3.0e38f;  // 127 / amax overflows: divide by the (subnormal) scale instead
-  if (lt == 0) scale[row] = s;
-  auto code = [&](uint32_t bf16_bits) -> uint32_t {
-    const float v = __uint_as_float(bf16_bits << 16);
-    const float t = tiny ? fminf(fmaxf(__fdiv_rn(v, s), -127.f), 127.f) : v * f;
-    return static_cast<uint32_t>(__float2int_rn(t)) & 0xffu;
-  };
+  const RowRule rule(mx);
+  if (lt == 0) scale[row] = rule.s;
   auto store = [&](int v, uint4 w) {
-    uint32_t lo = code(w.x & 0xffffu) | (code(w.x >> 16) << 8) | (code(w.y & 0xffffu) << 16) | (code(w.y >> 16) << 24);
-    uint32_t hi = code(w.z & 0xffffu) | (code(w.z >> 16) << 8) | (code(w.w & 0xffffu) << 16) | (code(w.w >> 16) << 24);
+    const uint2 c = rule.codes(w);
     int8_t* dst = q + row * ldq + v * 8;
     if (VEC) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+      *reinterpret_cast<uint2*>(dst) = c;
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (v * 8 + i < k) dst[i] = static_cast<int8_t>(((i < 4 ? lo : hi) >> (8 * (i & 3))) & 0xffu);
+        if (v * 8 + i < k) dst[i] = static_cast<int8_t>(((i < 4 ? c.x : c.y) >> (8 * (i & 3))) & 0xffu);
     }
   };
 #pragma unroll
@@ -112,7 +139,6 @@ __global__ void __launch_bounds__(256) int8_quantize_rows_kernel(const __nv_bflo
 constexpr int kTileM = 128;   // tokens per tile (MMA M)
 constexpr int kBlockK = 128;  // bytes of K per stage
 constexpr int kThreads = 6 * 32;
-constexpr int kABytes = kTileM * kBlockK;
 
 enum Epilogue : int { kPlain = 0, kBias = 1, kSiluMul = 2 };  // the numbering of nqt_gemm_bf16
 
@@ -127,16 +153,14 @@ struct Int8Args {
   int epilogue;
   int early;  // the weights may be read before the previous kernel has finished
   int vec16;  // y rows allow 16-byte stores
+  int tn, stages;
+  int a_bytes;  // of a stage's tokens: a multiple of 8 rows, up to 128
+  uint32_t tmem_cols;
 };
 
-template <int TN>
-struct CfgI8 {
-  static constexpr int kBBytes = TN * kBlockK;
-  static constexpr int kStage = kABytes + kBBytes;
-  static constexpr int kStages = TN == 256 ? 4 : (TN == 128 ? 6 : 8);
-  static constexpr uint32_t kTmemCols = 2 * TN < 32 ? 32 : 2 * TN;
-  static constexpr int kSmem = 1024 + kStages * kStage + 2 * TN * 4 * 2 + (2 * kStages + 4) * 8 + 32;
-};
+constexpr int kMaxTN = 256, kMaxStages8 = 16;
+constexpr int kTail8 = 2 * kMaxTN * 4 * 2 + (2 * kMaxStages8 + 4) * 8 + 64;  // scales, biases, barriers, flags
+constexpr int kSmem8 = 227 * 1024;
 
 __device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                           uint32_t accumulate) {
@@ -163,9 +187,10 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
 }
 
 // 32 accumulators of one token -> outputs, stored at column `col` of row y (plain, bias) or col / 2 (gate and up
-// columns in groups of 16).  `sw`, `sb`: the columns' scales and biases in shared memory.
+// columns in groups of 16).  `sw`, `sb`: the columns' scales and biases in shared memory; `width`: columns left in
+// the tile.
 __device__ __forceinline__ void finish_32(const Int8Args& a, const uint32_t (&r)[32], float sx, const float* sw,
-                                          const float* sb, __nv_bfloat16* yrow, int col) {
+                                          const float* sb, __nv_bfloat16* yrow, int col, int width) {
   float v[32];
 #pragma unroll
   for (int e = 0; e < 32; e += 4) {
@@ -175,7 +200,7 @@ __device__ __forceinline__ void finish_32(const Int8Args& a, const uint32_t (&r)
     v[e + 2] = static_cast<float>(static_cast<int32_t>(r[e + 2])) * (sx * w.z);
     v[e + 3] = static_cast<float>(static_cast<int32_t>(r[e + 3])) * (sx * w.w);
   }
-  int count = 32, out0 = col;
+  int count = width < 32 ? width : 32, out0 = col;
   if (a.epilogue == kBias) {
 #pragma unroll
     for (int e = 0; e < 32; ++e) v[e] += sb[e];
@@ -186,7 +211,7 @@ __device__ __forceinline__ void finish_32(const Int8Args& a, const uint32_t (&r)
     out0 = col / 2;
   }
   const int left = a.cols - out0;
-  if (a.vec16 && left >= count) {
+  if (a.vec16 && left >= count && count % 8 == 0) {
 #pragma unroll
     for (int e = 0; e < 32; e += 8) {
       if (e >= count) break;
@@ -201,19 +226,20 @@ __device__ __forceinline__ void finish_32(const Int8Args& a, const uint32_t (&r)
   }
 }
 
-template <int TN>
 __global__ void __launch_bounds__(kThreads, 1)
-    gemm_int8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, Int8Args a) {
-  using Cfg = CfgI8<TN>;
-  constexpr int ST = Cfg::kStages;
+    gemm_int8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+                     const __grid_constant__ Int8Args a) {
+  const int ST = a.stages, TN = a.tn;
+  const int a_bytes = a.a_bytes, stage_bytes = a_bytes + TN * kBlockK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* s_sw = reinterpret_cast<float*>(smem + ST * Cfg::kStage);  // [2][TN] scales, then [2][TN] biases
-  float* s_sb = s_sw + 2 * TN;
-  uint64_t* full = reinterpret_cast<uint64_t*>(s_sb + 2 * TN);
-  uint64_t* empty = full + ST;
-  uint64_t* accf = empty + ST;  // [2] accumulator complete
-  uint64_t* acce = accf + 2;    // [2] accumulator read
+  // behind the ring, and at least 128 token rows behind its last stage's start
+  float* s_sw = reinterpret_cast<float*>(smem_raw + kSmem8 - kTail8);  // [2][TN] scales, then [2][TN] biases
+  float* s_sb = s_sw + 2 * kMaxTN;
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_sb + 2 * kMaxTN);
+  uint64_t* empty = full + kMaxStages8;
+  uint64_t* accf = empty + kMaxStages8;  // [2] accumulator complete
+  uint64_t* acce = accf + 2;             // [2] accumulator read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acce + 2);
   volatile int* s_issued = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* s_consumed = s_issued + 1;
@@ -235,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&wmap);
   }
   if (warp == 1) {
-    tc::tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tc::tmem_alloc(tmem_slot, a.tmem_cols);
     tc::tmem_relinquish();
   }
   tc::fence_before_sync();
@@ -254,8 +280,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n0 = static_cast<int>(blockIdx.x) / a.m_tiles * TN;
         ahead = a.kb < ST ? a.kb : ST;
         for (int i = 0; i < ahead; ++i) {
-          mbar_arrive_expect_tx(&full[i], Cfg::kStage);
-          tma_load_2d(smem + i * Cfg::kStage + kABytes, &wmap, &full[i], i * kBlockK, n0);
+          mbar_arrive_expect_tx(&full[i], stage_bytes);
+          tma_load_2d(smem + i * stage_bytes + a_bytes, &wmap, &full[i], i * kBlockK, n0);
         }
       }
       grid_dependency_wait();
@@ -267,10 +293,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          uint8_t* st = smem + s * Cfg::kStage;
+          uint8_t* st = smem + s * stage_bytes;
           if (it >= ahead) {
-            mbar_arrive_expect_tx(&full[s], Cfg::kStage);
-            tma_load_2d(st + kABytes, &wmap, &full[s], kb * kBlockK, n0);
+            mbar_arrive_expect_tx(&full[s], stage_bytes);
+            tma_load_2d(st + a_bytes, &wmap, &full[s], kb * kBlockK, n0);
           }
           tma_load_2d(st, &xmap, &full[s], kb * kBlockK, m0);
           *s_issued = it + 1;
@@ -279,9 +305,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t idesc = idesc_s8_s32(kTileM, TN);
+      const uint32_t idesc = idesc_s8_s32(kTileM, TN);
       const uint64_t a_desc = tc::smem_desc_sw128(smem_addr(smem), 16, 1024);
-      const uint64_t b_desc = tc::smem_desc_sw128(smem_addr(smem + kABytes), 16, 1024);
+      const uint64_t b_desc = tc::smem_desc_sw128(smem_addr(smem + a_bytes), 16, 1024);
       int it = 0, t = 0;
       bool ok = true;
       for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, ++t) {
@@ -296,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           *s_consumed = it + 1;
           tc::fence_after_sync();
-          const uint32_t off = static_cast<uint32_t>(s * Cfg::kStage) >> 4;
+          const uint32_t off = static_cast<uint32_t>(s * stage_bytes) >> 4;
 #pragma unroll
           for (int kk = 0; kk < kBlockK / 32; ++kk)
             mma_i8_ss(tmem + buf * TN, a_desc + off + kk * 2, b_desc + off + kk * 2, idesc, (kb | kk) ? 1u : 0u);
@@ -313,8 +339,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++t) {
       const int buf = t & 1;
       const int m0 = tile % a.m_tiles * kTileM, n0 = tile / a.m_tiles * TN;
-      float* sw = s_sw + buf * TN;
-      float* sb = s_sb + buf * TN;
+      float* sw = s_sw + buf * kMaxTN;
+      float* sb = s_sb + buf * kMaxTN;
       for (int i = et; i < TN; i += 128) {
         sw[i] = n0 + i < a.n ? __ldg(a.wscale + n0 + i) : 0.f;
         if (a.epilogue == kBias) sb[i] = n0 + i < a.n ? __bfloat162float(a.bias[n0 + i]) : 0.f;
@@ -339,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&acce[buf]);
         }
-        if (tok < a.m && n0 + c < a.n) finish_32(a, r, sx, sw + c, sb + c, yrow, n0 + c);
+        if (tok < a.m && n0 + c < a.n) finish_32(a, r, sx, sw + c, sb + c, yrow, n0 + c, TN - c);
       }
     }
   }
@@ -349,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = *s_consumed; i < *s_issued; ++i) mbar_wait(&full[i % ST], (i / ST) & 1, a.status);
   if (warp == 1) {
     tc::fence_after_sync();
-    tc::tmem_dealloc(tmem, Cfg::kTmemCols);
+    tc::tmem_dealloc(tmem, a.tmem_cols);
   }
 }
 
@@ -367,26 +393,266 @@ int encode_i8(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64
   return r == CUDA_SUCCESS ? NQT_OK : NQT_ERR_CUDA;
 }
 
-template <int TN>
-int launch_i8(const void* xq, int64_t ldxq, const void* w, int64_t ldw, int k, Int8Args a, cudaStream_t s) {
-  using Cfg = CfgI8<TN>;
+// ------------------------------------------------------------------ few tokens
+constexpr int kGemvMaxM = 8;
+constexpr int kGemvSmem = 96 * 1024;  // codes of the tokens
+
+struct GemvArgs {
+  const __nv_bfloat16* x;  // bf16 rows, or null: codes
+  const int8_t* xq;
+  int64_t ldx, ldxq;
+  const float* xscale;
+  const int8_t* w;
+  int64_t ldw;
+  const float* wscale;
+  const __nv_bfloat16* bias;
+  __nv_bfloat16* y;
+  int64_t ldy;
+  int m, n, cols, k, kpad;  // kpad: bytes of a token's codes in shared memory, a multiple of 16
+  int epilogue;
+  int xvec;  // x rows allow 16-byte loads (and k is a multiple of 8)
+};
+
+// 16 weights of a row from byte 16 c; bytes behind k are not read (the row may end there) and count as zeros.
+__device__ __forceinline__ uint4 load_w16(const int8_t* row, int c, int k) {
+  if (c * 16 + 16 <= k) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(row + c * 16));
+    return v;
+  }
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (c * 16 + i < k) w[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(row[c * 16 + i])) << (8 * (i & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// M: token slots, a power of two >= m.  A warp takes pairs of weight rows: neighbours, or a gate row and its up row.
+template <int M>
+__global__ void __launch_bounds__(256, 2) gemv_int8_kernel(const __grid_constant__ GemvArgs a) {
+  extern __shared__ __align__(16) uint8_t s_codes[];  // [M][kpad]
+  __shared__ uint32_t s_max[8];
+  __shared__ float s_scale[M];
+  constexpr int kAhead = 4;  // 16-byte chunks of each row in flight
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunks = (a.k + 15) / 16;
+  const int pairs = (a.n + 1) / 2;
+  const bool silu = a.epilogue == kSiluMul;
+  // rows of pair i: gate_up: groups of 16 gate and 16 up rows
+  auto row_of = [&](int i, int h) -> int { return silu ? i / 16 * 32 + h * 16 + i % 16 : 2 * i + h; };
+  auto weights = [&](int i, int c0, uint4 (&w)[2][kAhead]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = row_of(i, h);
+      const int8_t* p = a.w + static_cast<int64_t>(r < a.n ? r : 0) * a.ldw;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int c = c0 + u * 32 + lane;
+        w[h][u] = make_uint4(0u, 0u, 0u, 0u);
+        if (c < chunks && i < pairs) w[h][u] = load_w16(p, c, a.k);
+      }
+    }
+  };
+  int pair = blockIdx.x * 8 + warp;
+  uint4 w[2][kAhead];
+  grid_dependency_wait();
+  weights(pair, 0, w);
+  grid_dependents_launch();
+
+  // the tokens' codes: M rows by 256 / M threads each (codes of absent rows and behind k are zeros)
+  {
+    constexpr int TPR = 256 / M;
+    const int t = threadIdx.x / TPR, lt = threadIdx.x % TPR;
+    uint8_t* dst = s_codes + t * a.kpad;
+    if (a.x != nullptr) {
+      const __nv_bfloat16* src = a.x + static_cast<int64_t>(t < a.m ? t : 0) * a.ldx;
+      const int vecs = (a.k + 7) / 8;
+      auto load = [&](int v) -> uint4 { return a.xvec ? load8<true>(src, v, a.k) : load8<false>(src, v, a.k); };
+      constexpr int kKeep = 4;
+      uint4 keep[kKeep];
+      uint32_t m2 = 0;
+#pragma unroll
+      for (int i = 0; i < kKeep; ++i) {
+        keep[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (lt + i * TPR < vecs) keep[i] = load(lt + i * TPR);
+        m2 = magnitude2(keep[i], m2);
+      }
+      for (int v = lt + kKeep * TPR; v < vecs; v += TPR) m2 = magnitude2(load(v), m2);
+      uint32_t mx = max(m2 & 0xffffu, m2 >> 16);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(kFull, mx, o));
+      if (TPR > 32) {
+        if (lane == 0) s_max[warp] = mx;
+        __syncthreads();
+        const int w0 = t * (TPR / 32);
+#pragma unroll
+        for (int i = 0; i < TPR / 32; ++i) mx = max(mx, s_max[w0 + i]);
+      }
+      const RowRule rule(mx);
+      if (lt == 0) s_scale[t] = rule.s;
+#pragma unroll
+      for (int i = 0; i < kKeep; ++i)
+        if (lt + i * TPR < vecs) *reinterpret_cast<uint2*>(dst + (lt + i * TPR) * 8) = rule.codes(keep[i]);
+      for (int v = lt + kKeep * TPR; v < vecs; v += TPR) *reinterpret_cast<uint2*>(dst + v * 8) = rule.codes(load(v));
+      for (int v = vecs + lt; v < a.kpad / 8; v += TPR) *reinterpret_cast<uint2*>(dst + v * 8) = make_uint2(0u, 0u);
+    } else {
+      const int8_t* src = a.xq + static_cast<int64_t>(t < a.m ? t : 0) * a.ldxq;
+      for (int c = lt; c < a.kpad / 16; c += TPR) *reinterpret_cast<uint4*>(dst + c * 16) = load_w16(src, c, a.k);
+      if (lt == 0) s_scale[t] = t < a.m ? a.xscale[t] : 0.f;
+    }
+  }
+  __syncthreads();
+
+  for (; pair < pairs; pair += gridDim.x * 8) {
+    int acc[2][M];
+#pragma unroll
+    for (int t = 0; t < M; ++t) acc[0][t] = acc[1][t] = 0;
+    for (int c0 = 0; c0 < chunks; c0 += 32 * kAhead) {
+      uint4 cur[2][kAhead];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) cur[h][u] = w[h][u];
+      // the next weights: of this pair, or the first of the warp's next
+      if (c0 + 32 * kAhead < chunks) weights(pair, c0 + 32 * kAhead, w);
+      else weights(pair + gridDim.x * 8, 0, w);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int c = c0 + u * 32 + lane;
+        if (c < chunks) {
+#pragma unroll
+          for (int t = 0; t < M; ++t) {
+            const uint4 x = *reinterpret_cast<const uint4*>(s_codes + t * a.kpad + c * 16);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              int v = acc[h][t];
+              v = __dp4a(static_cast<int>(cur[h][u].x), static_cast<int>(x.x), v);
+              v = __dp4a(static_cast<int>(cur[h][u].y), static_cast<int>(x.y), v);
+              v = __dp4a(static_cast<int>(cur[h][u].z), static_cast<int>(x.z), v);
+              acc[h][t] = __dp4a(static_cast<int>(cur[h][u].w), static_cast<int>(x.w), v);
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int t = 0; t < M; ++t) acc[h][t] = __reduce_add_sync(kFull, acc[h][t]);
+    // lane t finishes token t
+    int v0 = acc[0][0], v1 = acc[1][0];
+#pragma unroll
+    for (int t = 1; t < M; ++t)
+      if (lane == t) {
+        v0 = acc[0][t];
+        v1 = acc[1][t];
+      }
+    if (lane < a.m) {
+      const int r0 = row_of(pair, 0), r1 = row_of(pair, 1);
+      const float sx = s_scale[lane];
+      float y0 = static_cast<float>(v0) * (sx * a.wscale[r0]);
+      float y1 = r1 < a.n ? static_cast<float>(v1) * (sx * a.wscale[r1]) : 0.f;
+      __nv_bfloat16* yrow = a.y + lane * a.ldy;
+      if (silu) {
+        const int col = pair / 16 * 16 + pair % 16;
+        if (col < a.cols) yrow[col] = __float2bfloat16_rn(silu_mul(y0, y1));
+      } else {
+        if (a.epilogue == kBias) {
+          y0 += __bfloat162float(a.bias[r0]);
+          if (r1 < a.n) y1 += __bfloat162float(a.bias[r1]);
+        }
+        yrow[r0] = __float2bfloat16_rn(y0);
+        if (r1 < a.n) yrow[r1] = __float2bfloat16_rn(y1);
+      }
+    }
+  }
+}
+
+template <int M>
+int launch_gemv(const GemvArgs& a, cudaStream_t s) {
   static std::once_flag once;
   std::call_once(once, [] {
-    cudaFuncSetAttribute(gemm_int8_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+    cudaFuncSetAttribute(gemv_int8_kernel<M>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemvSmem);
   });
+  const int pairs = (a.n + 1) / 2;
+  const int most = num_sms() * 2;  // resident at once: a warp goes on to its next pair
+  const int grid = (pairs + 7) / 8 < most ? (pairs + 7) / 8 : most;
+  const cudaError_t err = launch_pdl(gemv_int8_kernel<M>, dim3(grid), dim3(256), static_cast<size_t>(M) * a.kpad, s, a);
+  if (err != cudaSuccess) {
+    set_last_error("gemv_int8", err);
+    return NQT_ERR_CUDA;
+  }
+  return NQT_OK;
+}
+
+int gemv_slots(int m) { return m <= 1 ? 1 : (m <= 2 ? 2 : (m <= 4 ? 4 : 8)); }
+
+bool takes_gemv(int m, int k) {
+  return m <= kGemvMaxM && static_cast<int64_t>(gemv_slots(m)) * ((k + 15) / 16 * 16) <= kGemvSmem;
+}
+
+int run_gemv(const GemvArgs& a, cudaStream_t s) {
+  switch (gemv_slots(a.m)) {
+    case 1: return launch_gemv<1>(a, s);
+    case 2: return launch_gemv<2>(a, s);
+    case 4: return launch_gemv<4>(a, s);
+    default: return launch_gemv<8>(a, s);
+  }
+}
+
+// ------------------------------------------------------------------ host
+// Weight rows per tile.  A CTA's time for a K block goes with the bytes it brings into shared memory, so a wave of
+// tiles costs (token rows + TN) and the narrowest widths win only while they save a wave.  (One B200, device time:
+// 64 tokens x 12288 x 2048: TN 96, one wave, against TN 64, two; see the product's comment for the figures.)
+int pick_tn(int m, int n, int epilogue) {
+  const int widths[] = {256, 224, 192, 160, 128, 96, 64, 32, 16};
+  const int64_t sms = num_sms();
+  const int64_t m_tiles = (m + kTileM - 1) / kTileM;
+  const int rows = m >= kTileM ? kTileM : (m + 7) / 8 * 8;
+  int best = 256;
+  int64_t best_cost = -1;
+  for (int tn : widths) {
+    if (epilogue == kSiluMul && tn % 32) continue;  // a group of gate and up rows stays together
+    const int64_t tiles = m_tiles * ((n + tn - 1) / tn);
+    const int64_t cost = (tiles + sms - 1) / sms * (rows + tn);
+    if (best_cost < 0 || cost < best_cost) {
+      best = tn;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
+int launch_i8(const void* xq, int64_t ldxq, const void* w, int64_t ldw, int k, Int8Args a, cudaStream_t s) {
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaFuncSetAttribute(gemm_int8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem8);
+  });
+  a.tn = pick_tn(a.m, a.n, a.epilogue);
+  const int rows = a.m >= kTileM ? kTileM : (a.m + 7) / 8 * 8;
+  a.a_bytes = rows * kBlockK;
+  // the MMA reads 128 token rows from a stage's start: the last stage keeps that much before the tail
+  const int stage = a.a_bytes + a.tn * kBlockK;
+  const int ring = kSmem8 - kTail8 - 1024;
+  a.stages = ring / stage < kMaxStages8 ? ring / stage : kMaxStages8;
+  while (a.stages > 1 && (a.stages - 1) * stage + kTileM * kBlockK > ring) --a.stages;
+  a.tmem_cols = 32;
+  while (a.tmem_cols < 2u * static_cast<uint32_t>(a.tn)) a.tmem_cols <<= 1;
+  if (a.tn < 32) a.tmem_cols = 64;  // the epilogue reads 32 columns of either buffer
   CUtensorMap xmap, wmap;
-  if (encode_i8(&xmap, xq, a.m, k, ldxq, kTileM) != NQT_OK || encode_i8(&wmap, w, a.n, k, ldw, TN) != NQT_OK) {
+  if (encode_i8(&xmap, xq, a.m, k, ldxq, rows) != NQT_OK || encode_i8(&wmap, w, a.n, k, ldw, a.tn) != NQT_OK) {
     set_last_message("gemm_int8: cuTensorMapEncodeTiled failed");
     return NQT_ERR_CUDA;
   }
   a.m_tiles = (a.m + kTileM - 1) / kTileM;
-  const int64_t tiles = static_cast<int64_t>(a.m_tiles) * ((a.n + TN - 1) / TN);
+  const int64_t tiles = static_cast<int64_t>(a.m_tiles) * ((a.n + a.tn - 1) / a.tn);
   if (tiles > 0x3fffffff) return NQT_ERR_UNSUPPORTED;
   a.tiles = static_cast<int>(tiles);
   const int sms = num_sms();
-  // one CTA per SM: the shared memory of two would fit for small TN, but TMEM and the ring are sized for one
   const int grid = a.tiles < sms ? a.tiles : sms;
-  const cudaError_t err = launch_pdl(gemm_int8_kernel<TN>, dim3(grid), dim3(kThreads), Cfg::kSmem, s, xmap, wmap, a);
+  const cudaError_t err = launch_pdl(gemm_int8_kernel, dim3(grid), dim3(kThreads), kSmem8, s, xmap, wmap, a);
   if (err != cudaSuccess) {
     set_last_error("gemm_int8", err);
     return NQT_ERR_CUDA;
@@ -425,14 +691,32 @@ int run_gemm(const void* xq, int64_t ldxq, const float* xscale, const void* w, i
   a.epilogue = epilogue;
   a.early = early;
   a.vec16 = aligned(y, 16) && ldy % 8 == 0;
-  // the widest tile that still gives every SM one
-  const int64_t m_tiles = (m + kTileM - 1) / kTileM;
-  const int64_t sms = num_sms();
-  auto tiles = [&](int tn) { return m_tiles * ((n + tn - 1) / tn); };
-  if (tiles(256) >= sms) return launch_i8<256>(xq, ldxq, w, ldw, k, a, s);
-  if (tiles(128) >= sms) return launch_i8<128>(xq, ldxq, w, ldw, k, a, s);
-  if (tiles(64) >= sms) return launch_i8<64>(xq, ldxq, w, ldw, k, a, s);
-  return launch_i8<32>(xq, ldxq, w, ldw, k, a, s);
+  return launch_i8(xq, ldxq, w, ldw, k, a, s);
+}
+
+GemvArgs gemv_args(const void* x, int64_t ldx, const void* xq, int64_t ldxq, const float* xscale, const void* w,
+                   int64_t ldw, const float* wscale, const void* bias, void* y, int64_t ldy, int m, int n, int cols,
+                   int k, int epilogue) {
+  GemvArgs a{};
+  a.x = static_cast<const __nv_bfloat16*>(x);
+  a.ldx = ldx;
+  a.xq = static_cast<const int8_t*>(xq);
+  a.ldxq = ldxq;
+  a.xscale = xscale;
+  a.w = static_cast<const int8_t*>(w);
+  a.ldw = ldw;
+  a.wscale = wscale;
+  a.bias = static_cast<const __nv_bfloat16*>(bias);
+  a.y = static_cast<__nv_bfloat16*>(y);
+  a.ldy = ldy;
+  a.m = m;
+  a.n = n;
+  a.cols = cols;
+  a.k = k;
+  a.kpad = (k + 15) / 16 * 16;
+  a.epilogue = epilogue;
+  a.xvec = x != nullptr && aligned(x, 16) && ldx % 8 == 0 && k % 8 == 0;
+  return a;
 }
 
 int run_quantize(const void* x, int64_t ldx, int m, int k, void* q, int64_t ldq, float* scale, cudaStream_t s) {
@@ -470,6 +754,9 @@ extern "C" int nqt_gemm_int8(const void* xq, int64_t ldxq, const float* xscale, 
   const int rc = check_gemm(xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue);
   if (rc != NQT_OK) return rc;
   if (m == 0) return NQT_OK;
+  if (takes_gemv(m, k))
+    return run_gemv(gemv_args(nullptr, 0, xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue),
+                    as_stream(stream));
   return run_gemm(xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue, 0, status,
                   as_stream(stream));
 }
@@ -482,6 +769,8 @@ extern "C" int nqt_linear_int8(const void* x, int64_t ldx, void* xq, int64_t ldx
   if (!x || ldx < k || !aligned(x, 2)) return NQT_ERR_ARG;
   if (m == 0) return NQT_OK;
   cudaStream_t s = as_stream(stream);
+  if (takes_gemv(m, k))
+    return run_gemv(gemv_args(x, ldx, nullptr, 0, nullptr, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue), s);
   const int rq = run_quantize(x, ldx, m, k, xq, ldxq, xscale, s);
   if (rq != NQT_OK) return rq;
   // the quantiser is an ordinary launch: what came before it has finished, so the weights can be read at once
