@@ -272,7 +272,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0;
+      int it = 0, s = 0;  // K block, its stage and the stage's turn (divisions by ST would cost more than a block)
+      uint32_t phase = 0;
       bool ok = true;
       // the first stages' weights do not depend on the previous kernel when the caller says so
       int ahead = 0;
@@ -288,8 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
         const int m0 = tile % a.m_tiles * kTileM, n0 = tile / a.m_tiles * TN;
         for (int kb = 0; kb < a.kb; ++kb, ++it) {
-          const int s = it % ST;
-          if (it >= ST && !mbar_wait(&empty[s], ((it / ST) - 1) & 1, a.status)) {
+          if (it >= ST && !mbar_wait(&empty[s], phase ^ 1u, a.status)) {
             ok = false;
             break;
           }
@@ -299,37 +299,45 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_2d(st + a_bytes, &wmap, &full[s], kb * kBlockK, n0);
           }
           tma_load_2d(st, &xmap, &full[s], kb * kBlockK, m0);
-          *s_issued = it + 1;
+          if (++s == ST) {
+            s = 0;
+            phase ^= 1u;
+          }
         }
       }
+      *s_issued = it;
     }
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t idesc = idesc_s8_s32(kTileM, TN);
       const uint64_t a_desc = tc::smem_desc_sw128(smem_addr(smem), 16, 1024);
       const uint64_t b_desc = tc::smem_desc_sw128(smem_addr(smem + a_bytes), 16, 1024);
-      int it = 0, t = 0;
+      int it = 0, s = 0, t = 0;
+      uint32_t phase = 0;
       bool ok = true;
       for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, ++t) {
         const int buf = t & 1;
         if (t >= 2 && !mbar_wait(&acce[buf], ((t >> 1) - 1) & 1, a.status)) break;
         tc::fence_after_sync();
         for (int kb = 0; kb < a.kb; ++kb, ++it) {
-          const int s = it % ST;
-          if (!mbar_wait(&full[s], (it / ST) & 1, a.status)) {
+          if (!mbar_wait(&full[s], phase, a.status)) {
             ok = false;
             break;
           }
-          *s_consumed = it + 1;
           tc::fence_after_sync();
           const uint32_t off = static_cast<uint32_t>(s * stage_bytes) >> 4;
 #pragma unroll
           for (int kk = 0; kk < kBlockK / 32; ++kk)
             mma_i8_ss(tmem + buf * TN, a_desc + off + kk * 2, b_desc + off + kk * 2, idesc, (kb | kk) ? 1u : 0u);
           tc::commit(&empty[s]);
+          if (++s == ST) {
+            s = 0;
+            phase ^= 1u;
+          }
         }
         if (ok) tc::commit(&accf[buf]);
       }
+      *s_consumed = it;
     }
   } else {
     const int quarter = warp & 3;
