@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acce + 2);
   volatile int* s_issued = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* s_consumed = s_issued + 1;
+  volatile int* s_ready = s_consumed + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -355,8 +356,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int tok = m0 + quarter * 32 + lane;
       const float sx = tok < a.m ? a.xscale[tok] : 0.f;
-      epi_bar();  // also: everybody is done with this buffer's scales of two tiles ago
-      if (!mbar_wait(&accf[buf], (t >> 1) & 1, a.status)) break;
+      // One warp polls for the accumulator and the others wait in the barrier, which costs no issue slots: polling
+      // warps slow the thread that issues the products.  Also: all are done with this buffer's scales of two tiles ago.
+      if (warp == 2) {
+        const bool ok = mbar_wait(&accf[buf], (t >> 1) & 1, a.status);
+        if (lane == 0) *s_ready = ok ? 1 : 0;
+      }
+      epi_bar();
+      if (!*s_ready) break;
       tc::fence_after_sync();
       const uint32_t src = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * TN;
       __nv_bfloat16* yrow = a.y + static_cast<int64_t>(tok) * a.ldy;
@@ -731,8 +738,10 @@ int run_quantize(const void* x, int64_t ldx, int m, int k, void* q, int64_t ldq,
   const bool vec = aligned(x, 16) && ldx % 8 == 0 && k % 8 == 0 && aligned(q, 8) && ldq % 8 == 0;
   const __nv_bfloat16* xp = static_cast<const __nv_bfloat16*>(x);
   int8_t* qp = static_cast<int8_t*>(q);
-  // a warp per row keeps rows of up to 1024 elements in registers; longer rows get a whole CTA
-  if (k <= 1024) {
+  // A warp per row where its lanes hold the row (k <= 1024), and up to 2048 when there are rows enough for the GPU
+  // (4613 x 2048 on one B200: 7 us, against 11 us with a CTA per row); else a CTA per row, which keeps 8192 elements
+  // (4613 x 6144: 19 us, 4.4 TB/s).
+  if (k <= 1024 || (k <= 2048 && m >= 8 * num_sms())) {
     const unsigned grid = (static_cast<unsigned>(m) + 7) / 8;
     if (vec) int8_quantize_rows_kernel<32, true><<<grid, 256, 0, s>>>(xp, ldx, m, k, qp, ldq, scale);
     else int8_quantize_rows_kernel<32, false><<<grid, 256, 0, s>>>(xp, ldx, m, k, qp, ldq, scale);
