@@ -27,6 +27,11 @@ Differences by design:
     (executor/talker.py plans before every replay).  Without a workspace, or
     with one smaller than ``nqt_decode_workspace_bytes`` (about 10.6 MB at
     64 rows, 16 heads, D 128), the binding allocates its own.
+
+A binding over 8-bit storage (int8 or float8_e4m3fn codes, with ``scales``
+[layers, pages, 2, page_size / 16, kv_heads]) runs the 8-bit operators behind
+the same protocol.  Its decode needs no plan, and its workspace, which has to
+start at zero, is its own.
 """
 
 from __future__ import annotations
@@ -38,7 +43,12 @@ import torch
 
 from . import _lib
 from ._lib import call, ptr
-from .kernels import device_status, paired_qk_norm_rope_paged_cache_
+from .kernels import (
+    check_cache8,
+    device_status,
+    paired_qk_norm_rope_paged_cache8,
+    paired_qk_norm_rope_paged_cache_,
+)
 
 # nqt_decode_attention_ex flags (include/nqt.h NQT_DECODE_OVERLAP_KV_WRITE, NQT_DECODE_SHORT_WAIT)
 DECODE_OVERLAP_KV_WRITE = 0x1
@@ -263,9 +273,11 @@ class B200TalkerBinding:
         slot: int | None = None,
         metadata: TalkerAttentionMetadata | None = None,
         mode: str | None = None,
+        scales: torch.Tensor | None = None,
     ) -> None:
         """``mode`` ("decode" or "prefill") fixes the binding's kind up front;
-        by default the first ``plan`` fixes it."""
+        by default the first ``plan`` fixes it.  ``scales`` belongs to 8-bit
+        storage, with ``dtype`` the type of queries and outputs (bf16)."""
 
         del shared_plan_state, slot  # no shared host plan: see the module docstring
         if mode not in (None, "decode", "prefill"):
@@ -277,7 +289,17 @@ class B200TalkerBinding:
             raise ValueError("Talker workspace must be a uint8 tensor on the execution device")
         if storage.ndim != 6 or storage.shape[2] != 2:
             raise ValueError("paged KV storage must be [layers, pages, 2, page_size, kv_heads, head_dim]")
+        self.quantized = storage.dtype in (torch.int8, torch.float8_e4m3fn)
+        if self.quantized != (scales is not None):
+            raise ValueError("8-bit paged KV storage comes with scales, other storage without")
+        if self.quantized:
+            if dtype != torch.bfloat16:
+                raise TypeError("8-bit paged attention runs on bf16 queries")
+            if scales.ndim != 5 or scales.shape[0] != storage.shape[0] or scales.device != storage.device:
+                raise ValueError("paged KV scales must be [layers, pages, 2, page_size / 16, kv_heads]")
+            check_cache8(storage[0], scales[0], num_kv_heads, head_dim)
         self.storage = storage
+        self.scales = scales
         self.capture_batch_size = capture_batch_size
         self.token_capacity = token_capacity
         self.num_qo_heads = num_qo_heads
@@ -295,8 +317,11 @@ class B200TalkerBinding:
         self.paged_kv_indices = torch.zeros(total_pages + capture_batch_size, dtype=torch.int32, device=device)
         self.paged_kv_last_page_len = torch.ones(capture_batch_size, dtype=torch.int32, device=device)
         nbytes = _lib.lib().nqt_decode_workspace_bytes(capture_batch_size, num_qo_heads, head_dim)
-        if mode == "prefill":
+        self.workspace8 = None
+        if mode == "prefill" or self.quantized:
             self.decode_workspace = torch.empty(0, dtype=torch.uint8, device=device)
+            if self.quantized and mode != "prefill":
+                self.workspace8 = decode_paged8_workspace(capture_batch_size, num_qo_heads, head_dim, device)
         elif workspace is not None and workspace.is_contiguous() and workspace.numel() >= nbytes:
             self.decode_workspace = workspace[:nbytes]
         else:
@@ -344,7 +369,7 @@ class B200TalkerBinding:
     def device_plan(self) -> None:
         """Build the split-KV partition from the staged buffers (device only)."""
 
-        if self._prefill:
+        if self._prefill or self.quantized:
             return
         call(
             "nqt_decode_plan",
@@ -385,6 +410,20 @@ class B200TalkerBinding:
 
     def attend(self, attention: object, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor) -> torch.Tensor:
         layer = self.storage[self._layer_index]
+        if self.quantized:
+            scales = self.scales[self._layer_index]
+            query = paired_qk_norm_rope_paged_cache8(
+                query, key, value, attention.q_norm.weight, attention.k_norm.weight, self.position_ids,
+                attention.q_norm.variance_epsilon, float(attention.rope_theta), layer, scales, self.write_pages,
+                self.write_offsets)
+            if self._prefill:
+                return batch_prefill_paged8(query, layer, scales, self.qo_indptr, self.paged_kv_indptr,
+                                            self.paged_kv_indices, self.paged_kv_last_page_len,
+                                            batch=self.capture_batch_size)
+            # the write just before touches each row's last 16-token block and its scales only
+            return batch_decode_paged8(query, layer, scales, self.paged_kv_indptr, self.paged_kv_indices,
+                                       self.paged_kv_last_page_len, self.workspace8,
+                                       batch_capacity=self.capture_batch_size, overlap_kv_write=True)
         query, key = paired_qk_norm_rope_paged_cache_(
             query,
             key,

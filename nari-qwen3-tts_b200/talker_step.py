@@ -32,6 +32,11 @@ bf16.  The mixed step defaults to bf16: its gate/up multiplies thousands of
 prefill tokens, where the FP8 kernel (built to stream weights for decode-sized
 batches) is slower than cuBLAS.  The other projections are library calls
 (torch -> cuBLAS), as in the reference.
+
+The decode step also runs at 8 bits throughout: ``kv="int8"`` or ``"e4m3"``
+keeps the page pool in codes with a scale per 16-token block and KV head, and
+``projections="int8"`` (with ``gate_up="int8"``) runs the projections as W8A8
+integer products.  The codec head stays in bf16.
 """
 
 from __future__ import annotations
@@ -110,6 +115,27 @@ class TalkerWeights:
         return sum(t.numel() * t.element_size() for t in tensors)
 
 
+KV_DTYPES = {"bf16": torch.bfloat16, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+
+
+def _kv_pool8(shape: TalkerShape, total_pages: int, page_size: int, device, generator,
+              kv: str) -> tuple[torch.Tensor, torch.Tensor]:
+    """8-bit KV pool and its scales, filled with N(0, 1) data quantised block by block."""
+
+    dims = (total_pages, 2, page_size, shape.num_kv_heads, shape.head_dim)
+    storage = torch.empty((shape.num_layers, *dims), dtype=KV_DTYPES[kv], device=device)
+    scales = torch.empty((shape.num_layers, total_pages, 2, page_size // kernels.CACHE_BLOCK, shape.num_kv_heads),
+                         dtype=torch.float32, device=device)
+    top = 127.0 if kv == "int8" else 448.0
+    for layer in range(shape.num_layers):
+        x = torch.empty((total_pages, 2, page_size // kernels.CACHE_BLOCK, kernels.CACHE_BLOCK, shape.num_kv_heads,
+                         shape.head_dim), device=device).normal_(generator=generator)
+        scales[layer] = x.abs().amax(dim=(3, 5)) / top
+        x /= scales[layer][:, :, :, None, :, None]
+        storage[layer] = (x.round_() if kv == "int8" else x).view(dims).to(storage.dtype)
+    return storage, scales
+
+
 def _kv_pool(shape: TalkerShape, total_pages: int, page_size: int, device, generator) -> torch.Tensor:
     """Paged KV pool [layers, pages, 2, P, Hkv, D] filled with N(0, 1) data."""
 
@@ -136,19 +162,47 @@ class GateUpFp8:
         return sum(w.data.numel() + w.scale.numel() * 4 for w in self.weights)
 
 
+class Int8Projections:
+    """The layers' projections in int8 with one scale per output channel (tokens are quantised on the way): QKV, O
+    and down with ``projections``, gate/up (SwiGLU fused) with ``gate_up``."""
+
+    def __init__(self, weights: TalkerWeights, *, projections: bool, gate_up: bool) -> None:
+        def pack(ws, **kw):
+            return [kernels.Int8Weight(w, **kw) for w in ws]
+
+        self.qkv = pack(weights.w_qkv) if projections else None
+        self.o = pack(weights.w_o) if projections else None
+        self.down = pack(weights.w_down) if projections else None
+        self.gate_up = pack(weights.w_gate_up, gate_up=True) if gate_up else None
+
+    def replaces(self, weights: TalkerWeights) -> int:
+        """Weight bytes that a step streams less than with the bf16 copies."""
+
+        pairs = ((self.qkv, weights.w_qkv), (self.o, weights.w_o), (self.down, weights.w_down),
+                 (self.gate_up, weights.w_gate_up))
+        return sum(b.numel() * b.element_size() - a.data.numel() - a.data_scale.numel() * 4
+                   for ours, theirs in pairs if ours is not None for a, b in zip(ours, theirs, strict=True))
+
+
 def _mlp_block(weights: TalkerWeights, shape: TalkerShape, layer: int, o: torch.Tensor, residual: torch.Tensor,
-               act: torch.Tensor, fp8: GateUpFp8 | None = None) -> torch.Tensor:
+               act: torch.Tensor, fp8: GateUpFp8 | None = None, int8: Int8Projections | None = None) -> torch.Tensor:
     """residual += o; MLP(norm(residual)); residual += mlp; returns the next layer's normed input.  With ``fp8``
-    the gate/up projection takes the reference's FP8 path."""
+    the gate/up projection takes the reference's FP8 path; ``int8`` holds the projections that run as W8A8."""
 
     if fp8 is None:
         kernels.fused_add_rmsnorm_(o, residual, weights.ln_post[layer], shape.eps)
-        gate_up = F.linear(o, weights.w_gate_up[layer])
-        kernels.silu_and_mul(gate_up, out=act)
+        if int8 is not None and int8.gate_up is not None:
+            kernels.linear_int8(o, int8.gate_up[layer], out=act)
+        else:
+            gate_up = F.linear(o, weights.w_gate_up[layer])
+            kernels.silu_and_mul(gate_up, out=act)
     else:
         kernels.fused_add_rmsnorm_fp8_(o, residual, weights.ln_post[layer], shape.eps, fp8.q, fp8.scale)
         kernels.linear_fp8(fp8.q, fp8.scale, fp8.weights[layer], out=act, workspace=fp8.workspace)
-    m = F.linear(act, weights.w_down[layer])
+    if int8 is not None and int8.down is not None:
+        m = kernels.linear_int8(act, int8.down[layer])
+    else:
+        m = F.linear(act, weights.w_down[layer])
     nxt = weights.ln_final if layer + 1 == shape.num_layers else weights.ln_in[layer + 1]
     kernels.fused_add_rmsnorm_(m, residual, nxt, shape.eps)
     return m
@@ -167,11 +221,19 @@ class TalkerDecodeStep:
         seed: int = 0,
         publish: bool = True,
         gate_up: str = "fp8",
+        kv: str = "bf16",
+        projections: str = "bf16",
     ) -> None:
-        if gate_up not in ("fp8", "bf16"):
-            raise ValueError("gate_up is 'fp8' (the reference's production path) or 'bf16'")
+        if gate_up not in ("fp8", "bf16", "int8"):
+            raise ValueError("gate_up is 'fp8' (the reference's production path), 'bf16' or 'int8'")
+        if kv not in KV_DTYPES:
+            raise ValueError("kv is 'bf16', 'int8' or 'e4m3'")
+        if projections not in ("bf16", "int8"):
+            raise ValueError("projections is 'bf16' or 'int8'")
         self.shape = s = shape
         self.gate_up = gate_up
+        self.kv = kv
+        self.projections = projections
         # publish=False discards each step's reservation after the step, so every
         # step sees the same context lengths (a stationary benchmark workload)
         self.publish = publish
@@ -181,7 +243,11 @@ class TalkerDecodeStep:
         g = torch.Generator(device=dev).manual_seed(seed)
         bf16 = torch.bfloat16
         self.weights = TalkerWeights(s, dev, g)
-        self.storage = _kv_pool(s, total_pages, page_size, dev, g)
+        self.scales = None
+        if kv == "bf16":
+            self.storage = _kv_pool(s, total_pages, page_size, dev, g)
+        else:
+            self.storage, self.scales = _kv_pool8(s, total_pages, page_size, dev, g, kv)
         self.planner = DevicePagePlanner(total_pages=total_pages, page_size=page_size, slots=batch,
                                          max_pages_per_slot=max_pages_per_seq, scratch_page_count=batch,
                                          capture_rows=batch, token_capacity=batch, device=dev,
@@ -189,7 +255,7 @@ class TalkerDecodeStep:
         self.binding = B200TalkerBinding(storage=self.storage, capture_batch_size=batch, token_capacity=batch,
                                          num_qo_heads=s.num_heads, num_kv_heads=s.num_kv_heads, head_dim=s.head_dim,
                                          page_size=page_size, total_pages=total_pages, device=dev, dtype=bf16,
-                                         mode="decode")
+                                         mode="decode", scales=self.scales)
         # static step buffers (graph inputs and outputs)
         self.hidden_in = torch.zeros(batch, s.hidden, dtype=bf16, device=dev)
         # request state on the device: row i serves request slot i
@@ -201,6 +267,9 @@ class TalkerDecodeStep:
         self._residual = torch.empty(batch, s.hidden, dtype=bf16, device=dev)
         self._act = torch.empty(batch, s.ffn, dtype=bf16, device=dev)
         self.fp8 = GateUpFp8(self.weights, s, batch, dev) if gate_up == "fp8" else None
+        self.int8 = None
+        if projections == "int8" or gate_up == "int8":
+            self.int8 = Int8Projections(self.weights, projections=projections == "int8", gate_up=gate_up == "int8")
         self.graph: torch.cuda.CUDAGraph | None = None
         self.contexts: list[int] = []
         # parity hook: Exp(1) noise [batch, vocab] for the sampler's noise entry instead of the Philox draw
@@ -279,13 +348,15 @@ class TalkerDecodeStep:
             trace.append((x.clone(), residual.clone()))
         for layer in range(s.num_layers):
             b.select_layer(layer)
-            qkv = F.linear(x, w.w_qkv[layer])
+            i8 = self.int8 if self.projections == "int8" else None
+            qkv = F.linear(x, w.w_qkv[layer]) if i8 is None else kernels.linear_int8(x, i8.qkv[layer])
             q = qkv[:, : hq * d].view(rows, hq, d)
             k = qkv[:, hq * d: (hq + hkv) * d].view(rows, hkv, d)
             v = qkv[:, (hq + hkv) * d:].view(rows, hkv, d)
             attn = b.attend(w.attn[layer], q, k, v)
-            o = F.linear(attn.view(rows, hq * d), w.w_o[layer])
-            x = _mlp_block(w, s, layer, o, residual, self._act, self.fp8)
+            attn = attn.view(rows, hq * d)
+            o = F.linear(attn, w.w_o[layer]) if i8 is None else kernels.linear_int8(attn, i8.o[layer])
+            x = _mlp_block(w, s, layer, o, residual, self._act, self.fp8, self.int8)
             if trace is not None:
                 trace.append((x.clone(), residual.clone()) + self._mlp_rows())
         self.last_hidden = x  # the final normed hidden state (the code predictor's input)
@@ -339,16 +410,20 @@ class TalkerDecodeStep:
         lengths: K and V of every cached token plus the new one, q in, out."""
 
         s = self.shape
-        kv = sum(n + 1 for n in self.contexts) * 2 * s.num_kv_heads * s.head_dim * 2
+        kv = sum(n + 1 for n in self.contexts) * 2 * s.num_kv_heads * s.head_dim * self.storage.element_size()
+        if self.scales is not None:
+            kv += sum(-(-(n + 1) // kernels.CACHE_BLOCK) for n in self.contexts) * 2 * s.num_kv_heads * 4
         qo = 2 * self.batch * s.num_heads * s.head_dim * 2
         return kv + qo
 
     def weight_bytes(self) -> int:
-        """Weight bytes one step streams (the FP8 gate/up in place of its bf16 copy)."""
+        """Weight bytes one step streams (the FP8 or int8 projections in place of their bf16 copies)."""
 
         total = self.weights.bytes()
         if self.fp8 is not None:
             total += self.fp8.bytes() - sum(w.numel() * w.element_size() for w in self.weights.w_gate_up)
+        if self.int8 is not None:
+            total -= self.int8.replaces(self.weights)
         return total
 
 
