@@ -20,15 +20,19 @@
 // epilogue thread owns one token, its scale is one register, the weights' scales
 // are broadcast from shared memory, and gate and up columns (interleaved in groups
 // of 16 rows when the weight is laid out) meet in the same thread.  TN is chosen
-// per call (pick_tn): every SM should have a tile, of as many columns as that
-// allows, because a tile's tokens are read again for each.  A decode batch loads
-// only its own token rows; the MMA's other rows read whatever lies behind them in
-// shared memory, into accumulators that nobody reads.
+// per call (pick_tiling).  A decode batch loads only its own token rows; the MMA's
+// other rows read whatever lies behind them in shared memory, into accumulators
+// that nobody reads.  Where a call has few tiles and a long K, a cluster of up to 8
+// CTAs shares a tile's K: each stages its int32 accumulators in its own shared
+// memory, and each finishes its part of the tokens from all of them (integer sums:
+// the order does not matter).
 //
 // Up to 8 tokens the product is a stream of the weights: no tensor core, no
 // second launch.  Every CTA quantises the tokens for itself (they are a few KB),
 // its first weights already on their way, and a warp takes two weight rows at a
 // time (gate and up of one column) with dp4a.
+#include <algorithm>
+#include <cstdint>
 #include <mutex>
 
 #include "common.cuh"
@@ -88,6 +92,9 @@ __global__ void __launch_bounds__(256) int8_quantize_rows_kernel(const __nv_bflo
   constexpr int kRows = 256 / TPR;
   constexpr int kKeep = 4;
   __shared__ uint32_t s_max[8];
+  // Waiting first, then letting the product start: what came before this kernel has finished by then, so the product
+  // may read its weights at once.
+  grid_dependency_wait();
   grid_dependents_launch();
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
   const int lt = threadIdx.x % TPR;
@@ -137,7 +144,7 @@ __global__ void __launch_bounds__(256) int8_quantize_rows_kernel(const __nv_bflo
 
 // ------------------------------------------------------------------ product
 constexpr int kTileM = 128;   // tokens per tile (MMA M)
-constexpr int kBlockK = 128;  // bytes of K per stage
+constexpr int kBlockK = 128;  // bytes of K per box, of which a stage holds one or two of each operand
 constexpr int kThreads = 6 * 32;
 
 enum Epilogue : int { kPlain = 0, kBias = 1, kSiluMul = 2 };  // the numbering of nqt_gemm_bf16
@@ -148,19 +155,25 @@ struct Int8Args {
   __nv_bfloat16* y;
   int64_t ldy;
   int32_t* status;
-  int m, n, cols, kb;  // cols: output columns; kb: K blocks
+  int m, n, cols, kb;  // cols: output columns; kb: K blocks (of SUB boxes)
   int m_tiles, tiles;
   int epilogue;
   int early;  // the weights may be read before the previous kernel has finished
   int vec16;  // y rows allow 16-byte stores
   int tn, stages;
-  int a_bytes;  // of a stage's tokens: a multiple of 8 rows, up to 128
+  int a_bytes;  // of a box of tokens: a multiple of 8 rows, up to 128
+  int split;    // CTAs of a cluster that share a tile's K
   uint32_t tmem_cols;
 };
 
 constexpr int kMaxTN = 256, kMaxStages8 = 16;
 constexpr int kTail8 = 2 * kMaxTN * 4 * 2 + (2 * kMaxStages8 + 4) * 8 + 64;  // scales, biases, barriers, flags
 constexpr int kSmem8 = 227 * 1024;
+constexpr int kRing8 = kSmem8 - kTail8 - 1024;  // 1024: the ring starts on a multiple of that
+constexpr int kMaxSplit = 8;
+
+// Bytes from one token's staged accumulators to the next's: 16 more than they need, against bank conflicts.
+__host__ __device__ constexpr int split_pitch(int tn) { return tn * 4 + 16; }
 
 __device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                           uint32_t accumulate) {
@@ -184,6 +197,64 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_addr(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(c0), "r"(c1)
       : "memory");
+}
+
+__device__ __forceinline__ int4 ld_cluster_i4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// Four columns' sums over the cluster's partial accumulators at `addr` (the same place in every CTA), scaled.
+__device__ __forceinline__ float4 join_4(uint32_t addr, int split, float sx, const float* sw) {
+  int4 s = make_int4(0, 0, 0, 0);
+#pragma unroll 4
+  for (int c = 0; c < split; ++c) {
+    const int4 v = ld_cluster_i4(map_rank(addr, c));
+    s.x += v.x;
+    s.y += v.y;
+    s.z += v.z;
+    s.w += v.w;
+  }
+  return make_float4(static_cast<float>(s.x) * (sx * sw[0]), static_cast<float>(s.y) * (sx * sw[1]),
+                     static_cast<float>(s.z) * (sx * sw[2]), static_cast<float>(s.w) * (sx * sw[3]));
+}
+
+// The split tile's epilogue: this CTA's share of the token rows, from the staged accumulators of all the cluster's CTAs.
+__device__ __forceinline__ void join_split(const Int8Args& a, const uint8_t* stage, int pitch, int rank, int m0, int n0,
+                                           const float* sw, const float* sb) {
+  const int rows = a.m - m0 < kTileM ? a.m - m0 : kTileM;
+  const int r0 = rows * rank / a.split, r1 = rows * (rank + 1) / a.split;
+  const bool silu = a.epilogue == kSiluMul;
+  const int quads = silu ? a.tn / 8 : a.tn / 4;  // of output columns
+  const int count = (r1 - r0) * quads;
+  for (int i = threadIdx.x; i < count; i += kThreads) {
+    const int row = r0 + i / quads, q = i % quads;
+    const int c = silu ? q / 4 * 32 + q % 4 * 4 : 4 * q;  // accumulator column
+    const int col = silu ? n0 / 2 + 4 * q : n0 + c;
+    if (col >= a.cols) continue;
+    const float sx = a.xscale[m0 + row];
+    const uint32_t addr = smem_addr(stage + row * pitch + c * 4);
+    float4 v = join_4(addr, a.split, sx, sw + c);
+    if (silu) {
+      const float4 u = join_4(addr + 64, a.split, sx, sw + c + 16);
+      v = make_float4(silu_mul(v.x, u.x), silu_mul(v.y, u.y), silu_mul(v.z, u.z), silu_mul(v.w, u.w));
+    } else if (a.epilogue == kBias) {
+      v = make_float4(v.x + sb[c], v.y + sb[c + 1], v.z + sb[c + 2], v.w + sb[c + 3]);
+    }
+    __nv_bfloat16* y = a.y + static_cast<int64_t>(m0 + row) * a.ldy + col;
+    if (a.vec16 && col + 4 <= a.cols) {
+      *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    } else {
+      y[0] = __float2bfloat16_rn(v.x);
+      if (col + 1 < a.cols) y[1] = __float2bfloat16_rn(v.y);
+      if (col + 2 < a.cols) y[2] = __float2bfloat16_rn(v.z);
+      if (col + 3 < a.cols) y[3] = __float2bfloat16_rn(v.w);
+    }
+  }
 }
 
 // 32 accumulators of one token -> outputs, stored at column `col` of row y (plain, bias) or col / 2 (gate and up
@@ -226,11 +297,13 @@ __device__ __forceinline__ void finish_32(const Int8Args& a, const uint32_t (&r)
   }
 }
 
+// SPLIT: the grid has one cluster of a.split CTAs for each tile, each with its part of K; else it is persistent.
+template <bool SPLIT, int SUB>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_int8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
                      const __grid_constant__ Int8Args a) {
   const int ST = a.stages, TN = a.tn;
-  const int a_bytes = a.a_bytes, stage_bytes = a_bytes + TN * kBlockK;
+  const int a_bytes = a.a_bytes, b_bytes = TN * kBlockK, stage_bytes = (a_bytes + b_bytes) * SUB;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // behind the ring, and at least 128 token rows behind its last stage's start
@@ -246,6 +319,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* s_ready = s_consumed + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = SPLIT ? static_cast<int>(cluster_rank()) : 0;
+  const int first = SPLIT ? static_cast<int>(blockIdx.x) / a.split : static_cast<int>(blockIdx.x);
+  const int kb0 = SPLIT ? a.kb * rank / a.split : 0, kb1 = SPLIT ? a.kb * (rank + 1) / a.split : a.kb;
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(&full[s], 1);
@@ -278,18 +354,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       // the first stages' weights do not depend on the previous kernel when the caller says so
       int ahead = 0;
-      if (a.early && blockIdx.x < a.tiles) {
-        const int n0 = static_cast<int>(blockIdx.x) / a.m_tiles * TN;
-        ahead = a.kb < ST ? a.kb : ST;
+      if (a.early && first < a.tiles) {
+        const int n0 = first / a.m_tiles * TN;
+        ahead = kb1 - kb0 < ST ? kb1 - kb0 : ST;
         for (int i = 0; i < ahead; ++i) {
           mbar_arrive_expect_tx(&full[i], stage_bytes);
-          tma_load_2d(smem + i * stage_bytes + a_bytes, &wmap, &full[i], i * kBlockK, n0);
+#pragma unroll
+          for (int u = 0; u < SUB; ++u)
+            tma_load_2d(smem + i * stage_bytes + a_bytes * SUB + u * b_bytes, &wmap, &full[i],
+                        ((kb0 + i) * SUB + u) * kBlockK, n0);
         }
       }
       grid_dependency_wait();
-      for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
+      for (int tile = first; tile < a.tiles && ok; tile += gridDim.x) {
         const int m0 = tile % a.m_tiles * kTileM, n0 = tile / a.m_tiles * TN;
-        for (int kb = 0; kb < a.kb; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           if (it >= ST && !mbar_wait(&empty[s], phase ^ 1u, a.status)) {
             ok = false;
             break;
@@ -297,9 +376,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* st = smem + s * stage_bytes;
           if (it >= ahead) {
             mbar_arrive_expect_tx(&full[s], stage_bytes);
-            tma_load_2d(st + a_bytes, &wmap, &full[s], kb * kBlockK, n0);
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+              tma_load_2d(st + a_bytes * SUB + u * b_bytes, &wmap, &full[s], (kb * SUB + u) * kBlockK, n0);
           }
-          tma_load_2d(st, &xmap, &full[s], kb * kBlockK, m0);
+#pragma unroll
+          for (int u = 0; u < SUB; ++u)
+            tma_load_2d(st + u * a_bytes, &xmap, &full[s], (kb * SUB + u) * kBlockK, m0);
           if (++s == ST) {
             s = 0;
             phase ^= 1u;
@@ -312,15 +395,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       const uint32_t idesc = idesc_s8_s32(kTileM, TN);
       const uint64_t a_desc = tc::smem_desc_sw128(smem_addr(smem), 16, 1024);
-      const uint64_t b_desc = tc::smem_desc_sw128(smem_addr(smem + a_bytes), 16, 1024);
+      const uint64_t b_desc = tc::smem_desc_sw128(smem_addr(smem + a_bytes * SUB), 16, 1024);
       int it = 0, s = 0, t = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, ++t) {
+      for (int tile = first; tile < a.tiles && ok; tile += gridDim.x, ++t) {
         const int buf = t & 1;
         if (t >= 2 && !mbar_wait(&acce[buf], ((t >> 1) - 1) & 1, a.status)) break;
         tc::fence_after_sync();
-        for (int kb = 0; kb < a.kb; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           if (!mbar_wait(&full[s], phase, a.status)) {
             ok = false;
             break;
@@ -328,8 +411,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::fence_after_sync();
           const uint32_t off = static_cast<uint32_t>(s * stage_bytes) >> 4;
 #pragma unroll
-          for (int kk = 0; kk < kBlockK / 32; ++kk)
-            mma_i8_ss(tmem + buf * TN, a_desc + off + kk * 2, b_desc + off + kk * 2, idesc, (kb | kk) ? 1u : 0u);
+          for (int u = 0; u < SUB; ++u) {
+            const uint64_t ad = a_desc + off + u * (a_bytes >> 4), bd = b_desc + off + u * (b_bytes >> 4);
+#pragma unroll
+            for (int kk = 0; kk < kBlockK / 32; ++kk)
+              mma_i8_ss(tmem + buf * TN, ad + kk * 2, bd + kk * 2, idesc, kb > kb0 || u || kk ? 1u : 0u);
+          }
           tc::commit(&empty[s]);
           if (++s == ST) {
             s = 0;
@@ -345,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int et = threadIdx.x - 64;
     grid_dependency_wait();  // the tokens' scales, and y, which the previous kernel may still read
     int t = 0;
-    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++t) {
+    for (int tile = first; tile < a.tiles; tile += gridDim.x, ++t) {
       const int buf = t & 1;
       const int m0 = tile % a.m_tiles * kTileM, n0 = tile / a.m_tiles * TN;
       float* sw = s_sw + buf * kMaxTN;
@@ -366,6 +453,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!*s_ready) break;
       tc::fence_after_sync();
       const uint32_t src = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + buf * TN;
+      if (SPLIT) {  // the products have read the ring: it takes the accumulators now
+        if (m0 + quarter * 32 < a.m) {
+#pragma unroll 1
+          for (int c = 0; c < TN; c += 32) {
+            uint32_t r[32];
+            tc::ld_32x32b_x32(src + c, r);
+            tc::wait_ld();
+            uint8_t* dst = smem + (quarter * 32 + lane) * split_pitch(TN) + c * 4;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (c + e < TN && tok < a.m) *reinterpret_cast<uint4*>(dst + e * 4) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+          }
+        }
+        break;
+      }
       __nv_bfloat16* yrow = a.y + static_cast<int64_t>(tok) * a.ldy;
       const bool live_warp = m0 + quarter * 32 < a.m;
 #pragma unroll 1
@@ -385,6 +487,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   tc::fence_before_sync();
+  if (SPLIT) {
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    join_split(a, smem, split_pitch(TN), rank, first % a.m_tiles * kTileM, first / a.m_tiles * TN, s_sw, s_sb);
+    __syncwarp();
+    cluster_arrive();  // nobody's shared memory goes away while it is read
+    cluster_wait();
+  }
   __syncthreads();
   if (threadIdx.x == 0)  // after a wait that gave up: copies still in flight land before the CTA leaves
     for (int i = *s_consumed; i < *s_issued; ++i) mbar_wait(&full[i % ST], (i / ST) & 1, a.status);
@@ -618,41 +729,89 @@ int run_gemv(const GemvArgs& a, cudaStream_t s) {
 }
 
 // ------------------------------------------------------------------ host
-// Weight rows per tile.  A CTA's time for a K block goes with the bytes it brings into shared memory, so a wave of
-// tiles costs (token rows + TN) and the narrowest widths win only while they save a wave.  (One B200, device time:
-// 64 tokens x 12288 x 2048: TN 96, one wave, against TN 64, two; see the product's comment for the figures.)
-int pick_tn(int m, int n, int epilogue) {
+// CTAs that run at once in clusters of `split` (each CTA takes its SM whole; clusters leave some SMs over).
+int max_ctas(int split) {
+  static std::once_flag once;
+  static int most[kMaxSplit + 1];
+  std::call_once(once, [] {
+    for (auto kernel : {gemm_int8_kernel<false, 1>, gemm_int8_kernel<false, 2>, gemm_int8_kernel<true, 1>,
+                        gemm_int8_kernel<true, 2>})
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem8);
+    most[1] = num_sms();
+    for (int c = 2; c <= kMaxSplit; c *= 2) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(c);
+      cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = kSmem8;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = c;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      int clusters = 0;
+      if (cudaOccupancyMaxActiveClusters(&clusters, gemm_int8_kernel<true, 1>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        clusters = 0;
+      }
+      most[c] = clusters * c;
+    }
+  });
+  return most[split];
+}
+
+// Two boxes of K a stage where the ring then still has three stages.
+int boxes_per_stage(int rows, int tn) { return 3 * 2 * (rows + tn) * kBlockK <= kRing8 ? 2 : 1; }
+
+// Weight rows per tile, and the CTAs that share a tile's K.  The times of a wave's tiles in ns, fitted to a sweep over
+// 16 to 4613 tokens and four weights on one B200.  A box of K costs its barriers and the issue of its products, about
+// 200 with two boxes a stage and 270 with one, and wide tiles what they bring into shared memory.  So tiles are as
+// narrow as one wave allows (64 tokens x 12288 x 2048: width 96, 8.5 us, against 128, 8.8, and 192, 10.4), and K is
+// shared where that saves more boxes than the cluster's two barriers and the exchange of rows x tn sums cost
+// (64 tokens x 2048 x 6144: 7.5 us, against 12.6 undivided; 64 x 4096 x 2048: 7.0 against 6.3, so undivided).
+struct Tiling {
+  int tn, split;
+};
+
+Tiling pick_tiling(int m, int n, int boxes, int epilogue) {
   const int widths[] = {256, 224, 192, 160, 128, 96, 64, 32, 16};
-  const int64_t sms = num_sms();
+  const int64_t sms = max_ctas(1);
   const int64_t m_tiles = (m + kTileM - 1) / kTileM;
   const int rows = m >= kTileM ? kTileM : (m + 7) / 8 * 8;
-  int best = 256;
-  int64_t best_cost = -1;
+  Tiling best{256, 1};
+  int64_t best_cost = INT64_MAX;
   for (int tn : widths) {
     if (epilogue == kSiluMul && tn % 32) continue;  // a group of gate and up rows stays together
     const int64_t tiles = m_tiles * ((n + tn - 1) / tn);
-    const int64_t cost = (tiles + sms - 1) / sms * (rows + tn);
-    if (best_cost < 0 || cost < best_cost) {
-      best = tn;
-      best_cost = cost;
+    const int64_t box = boxes_per_stage(rows, tn) == 2 ? std::max(200, (rows + tn) * 17 / 20)
+                                                       : std::max(270, (rows + tn) * 9 / 10);
+    for (int split = 1; split <= kMaxSplit; split *= 2) {
+      if (split > 1 && (2 * split > boxes || tiles * split > max_ctas(split))) break;
+      const int64_t cost = split == 1 ? (tiles + sms - 1) / sms * boxes * box
+                                      : (boxes + split - 1) / split * box + 1500 + rows * tn / 6;
+      if (cost <= best_cost) {
+        best = {tn, split};
+        best_cost = cost;
+      }
     }
   }
   return best;
 }
 
 int launch_i8(const void* xq, int64_t ldxq, const void* w, int64_t ldw, int k, Int8Args a, cudaStream_t s) {
-  static std::once_flag once;
-  std::call_once(once, [] {
-    cudaFuncSetAttribute(gemm_int8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem8);
-  });
-  a.tn = pick_tn(a.m, a.n, a.epilogue);
+  const Tiling tiling = pick_tiling(a.m, a.n, a.kb, a.epilogue);
+  a.tn = tiling.tn;
+  a.split = tiling.split;
   const int rows = a.m >= kTileM ? kTileM : (a.m + 7) / 8 * 8;
   a.a_bytes = rows * kBlockK;
-  // the MMA reads 128 token rows from a stage's start: the last stage keeps that much before the tail
-  const int stage = a.a_bytes + a.tn * kBlockK;
-  const int ring = kSmem8 - kTail8 - 1024;
-  a.stages = ring / stage < kMaxStages8 ? ring / stage : kMaxStages8;
-  while (a.stages > 1 && (a.stages - 1) * stage + kTileM * kBlockK > ring) --a.stages;
+  const int box = a.a_bytes + a.tn * kBlockK;
+  const int sub = a.kb > 1 ? boxes_per_stage(rows, a.tn) : 1;
+  a.kb = (a.kb + sub - 1) / sub;
+  const int stage = box * sub;
+  // the MMA reads 128 token rows from each box's start: the last stage keeps that much before the tail
+  const int reach = (sub - 1) * a.a_bytes + kTileM * kBlockK;
+  a.stages = std::min(kRing8 / stage, kMaxStages8);
+  while (a.stages > 1 && (a.stages - 1) * stage + reach > kRing8) --a.stages;
   a.tmem_cols = 32;
   while (a.tmem_cols < 2u * static_cast<uint32_t>(a.tn)) a.tmem_cols <<= 1;
   if (a.tn < 32) a.tmem_cols = 64;  // the epilogue reads 32 columns of either buffer
@@ -666,8 +825,14 @@ int launch_i8(const void* xq, int64_t ldxq, const void* w, int64_t ldw, int k, I
   if (tiles > 0x3fffffff) return NQT_ERR_UNSUPPORTED;
   a.tiles = static_cast<int>(tiles);
   const int sms = num_sms();
-  const int grid = a.tiles < sms ? a.tiles : sms;
-  const cudaError_t err = launch_pdl(gemm_int8_kernel, dim3(grid), dim3(kThreads), kSmem8, s, xmap, wmap, a);
+  cudaError_t err;
+  if (a.split > 1) {
+    err = launch_pdl_cluster(sub == 2 ? gemm_int8_kernel<true, 2> : gemm_int8_kernel<true, 1>, dim3(a.tiles * a.split), dim3(kThreads), kSmem8, s, a.split, xmap,
+                             wmap, a);
+  } else {
+    const int grid = a.tiles < sms ? a.tiles : sms;
+    err = launch_pdl(sub == 2 ? gemm_int8_kernel<false, 2> : gemm_int8_kernel<false, 1>, dim3(grid), dim3(kThreads), kSmem8, s, xmap, wmap, a);
+  }
   if (err != cudaSuccess) {
     set_last_error("gemm_int8", err);
     return NQT_ERR_CUDA;
@@ -741,15 +906,16 @@ int run_quantize(const void* x, int64_t ldx, int m, int k, void* q, int64_t ldq,
   // A warp per row where its lanes hold the row (k <= 1024), and up to 2048 when there are rows enough for the GPU
   // (4613 x 2048 on one B200: 7 us, against 11 us with a CTA per row); else a CTA per row, which keeps 8192 elements
   // (4613 x 6144: 19 us, 4.4 TB/s).
-  if (k <= 1024 || (k <= 2048 && m >= 8 * num_sms())) {
-    const unsigned grid = (static_cast<unsigned>(m) + 7) / 8;
-    if (vec) int8_quantize_rows_kernel<32, true><<<grid, 256, 0, s>>>(xp, ldx, m, k, qp, ldq, scale);
-    else int8_quantize_rows_kernel<32, false><<<grid, 256, 0, s>>>(xp, ldx, m, k, qp, ldq, scale);
-  } else {
-    if (vec) int8_quantize_rows_kernel<256, true><<<m, 256, 0, s>>>(xp, ldx, m, k, qp, ldq, scale);
-    else int8_quantize_rows_kernel<256, false><<<m, 256, 0, s>>>(xp, ldx, m, k, qp, ldq, scale);
+  const bool warp_rows = k <= 1024 || (k <= 2048 && m >= 8 * num_sms());
+  auto kernel = warp_rows ? (vec ? int8_quantize_rows_kernel<32, true> : int8_quantize_rows_kernel<32, false>)
+                          : (vec ? int8_quantize_rows_kernel<256, true> : int8_quantize_rows_kernel<256, false>);
+  const unsigned grid = warp_rows ? (static_cast<unsigned>(m) + 7) / 8 : static_cast<unsigned>(m);
+  const cudaError_t err = launch_pdl(kernel, dim3(grid), dim3(256), 0, s, xp, ldx, m, k, qp, ldq, scale);
+  if (err != cudaSuccess) {
+    set_last_error("int8_quantize_rows", err);
+    return NQT_ERR_CUDA;
   }
-  return check_launch("int8_quantize_rows");
+  return NQT_OK;
 }
 
 }  // namespace
@@ -790,6 +956,6 @@ extern "C" int nqt_linear_int8(const void* x, int64_t ldx, void* xq, int64_t ldx
     return run_gemv(gemv_args(x, ldx, nullptr, 0, nullptr, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue), s);
   const int rq = run_quantize(x, ldx, m, k, xq, ldxq, xscale, s);
   if (rq != NQT_OK) return rq;
-  // the quantiser is an ordinary launch: what came before it has finished, so the weights can be read at once
+  // the product starts when the quantiser has seen all earlier kernels finish, so it may read the weights at once
   return run_gemm(xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue, 1, status, s);
 }

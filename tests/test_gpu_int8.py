@@ -183,3 +183,31 @@ def test_nan_rows_stay_their_own(nqt, cuda):
         y = nqt.kernels.linear_int8(x[:rows].to(cuda), weight).cpu()
         assert y[3].isnan().all()
         assert y[torch.arange(rows) != 3].isfinite().all()
+
+
+@pytest.mark.parametrize(("m", "n", "k"), [(9, 256, 4096), (16, 2048, 2048), (64, 2048, 6144), (64, 333, 5000),
+                                           (128, 2048, 6144), (77, 100, 8192), (240, 2048, 6144), (130, 514, 4097),
+                                           (512, 2048, 6144), (24, 33, 20000), (12, 1, 6000)])
+@pytest.mark.parametrize("kind", ["plain", "bias", "gate_up"])
+def test_long_sums_shared_by_clusters(nqt, cuda, m, n, k, kind):
+    """Few tiles and a long K: the product of bf16 rows, its K shared among CTAs, next to the exact one of its codes."""
+
+    x = _rand((m, k), 5 * m + n, spread=1.0).to(cuda)
+    rows = 2 * n if kind == "gate_up" else n
+    wq, ws = _weight(rows, k, m + n)
+    weight = nqt.kernels.Int8Weight.from_quantized(wq.to(cuda), ws.to(cuda), gate_up=kind == "gate_up")
+    bias = (torch.arange(n) % 7 - 3).to(torch.bfloat16) if kind == "bias" else None
+    codes, scale = nqt.kernels.int8_quantize_rows(x)
+    nqt.kernels.clear_status(cuda)
+    got = nqt.kernels.linear_int8(x, weight, None if bias is None else bias.to(cuda))
+    again = nqt.kernels.linear_int8(codes, weight, None if bias is None else bias.to(cuda), xscale=scale)
+    assert nqt.kernels.read_status(cuda) == 0 and torch.equal(got, again)
+    want = _product((codes.cpu().double(), scale.cpu().double()), wq, ws, bias, kind == "gate_up")
+    # bf16's half step, and fp32: the sum's conversion, the scales' product, theirs, the bias's addition (2^-24 each, of
+    # the terms); gate_up also the exponential and the quotient, some 2^-21
+    size = want.abs() if bias is None else want.abs() + bias.double().abs()
+    if kind == "gate_up":
+        # silu's slope is under 1.1, so an error of 3 * 2^-24 |g| moves silu(g) u by as much of |g u| at most
+        g, u = _product((codes.cpu().double(), scale.cpu().double()), wq, ws).split(n, dim=1)
+        size = want.abs() + (g * u).abs() * 2.0**-2
+    assert ((got.cpu().double() - want).abs() <= 2.0**-8 * want.abs() + 2.0**-20 * size + 1e-30).all()
