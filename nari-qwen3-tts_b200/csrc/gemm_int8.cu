@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* s_consumed = s_issued + 1;
   volatile int* s_ready = s_consumed + 1;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = tc::uniform_warp(), lane = threadIdx.x & 31;
   const int rank = SPLIT ? static_cast<int>(cluster_rank()) : 0;
   const int first = SPLIT ? static_cast<int>(blockIdx.x) / a.split : static_cast<int>(blockIdx.x);
   const int kb0 = SPLIT ? a.kb * rank / a.split : 0, kb1 = SPLIT ? a.kb * (rank + 1) / a.split : a.kb;
@@ -347,8 +347,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   grid_dependents_launch();
 
+  // The producer's and the issuer's loops are run by whole warps, and one elected lane issues: operands and descriptors
+  // then stay in uniform registers.  (One lane's own loop cost some 20 clocks more for each product.)
   if (warp == 0) {
-    if (lane == 0) {
+    {
+      const bool lead = tc::elect_one();
       int it = 0, s = 0;  // K block, its stage and the stage's turn (divisions by ST would cost more than a block)
       uint32_t phase = 0;
       bool ok = true;
@@ -358,6 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n0 = first / a.m_tiles * TN;
         ahead = kb1 - kb0 < ST ? kb1 - kb0 : ST;
         for (int i = 0; i < ahead; ++i) {
+          if (!lead) continue;
           mbar_arrive_expect_tx(&full[i], stage_bytes);
 #pragma unroll
           for (int u = 0; u < SUB; ++u)
@@ -369,30 +373,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int tile = first; tile < a.tiles && ok; tile += gridDim.x) {
         const int m0 = tile % a.m_tiles * kTileM, n0 = tile / a.m_tiles * TN;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          if (it >= ST && !mbar_wait(&empty[s], phase ^ 1u, a.status)) {
+          if (it >= ST && !__all_sync(kFull, mbar_wait(&empty[s], phase ^ 1u, a.status))) {
             ok = false;
             break;
           }
-          uint8_t* st = smem + s * stage_bytes;
-          if (it >= ahead) {
-            mbar_arrive_expect_tx(&full[s], stage_bytes);
+          if (lead) {
+            uint8_t* st = smem + s * stage_bytes;
+            if (it >= ahead) {
+              mbar_arrive_expect_tx(&full[s], stage_bytes);
+#pragma unroll
+              for (int u = 0; u < SUB; ++u)
+                tma_load_2d(st + a_bytes * SUB + u * b_bytes, &wmap, &full[s], (kb * SUB + u) * kBlockK, n0);
+            }
 #pragma unroll
             for (int u = 0; u < SUB; ++u)
-              tma_load_2d(st + a_bytes * SUB + u * b_bytes, &wmap, &full[s], (kb * SUB + u) * kBlockK, n0);
+              tma_load_2d(st + u * a_bytes, &xmap, &full[s], (kb * SUB + u) * kBlockK, m0);
           }
-#pragma unroll
-          for (int u = 0; u < SUB; ++u)
-            tma_load_2d(st + u * a_bytes, &xmap, &full[s], (kb * SUB + u) * kBlockK, m0);
           if (++s == ST) {
             s = 0;
             phase ^= 1u;
           }
         }
       }
-      *s_issued = it;
+      if (lane == 0) *s_issued = it;
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    {
+      const bool lead = tc::elect_one();
       const uint32_t idesc = idesc_s8_s32(kTileM, TN);
       const uint64_t a_desc = tc::smem_desc_sw128(smem_addr(smem), 16, 1024);
       const uint64_t b_desc = tc::smem_desc_sw128(smem_addr(smem + a_bytes * SUB), 16, 1024);
@@ -401,31 +408,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int tile = first; tile < a.tiles && ok; tile += gridDim.x, ++t) {
         const int buf = t & 1;
-        if (t >= 2 && !mbar_wait(&acce[buf], ((t >> 1) - 1) & 1, a.status)) break;
+        if (t >= 2 && !__all_sync(kFull, mbar_wait(&acce[buf], ((t >> 1) - 1) & 1, a.status))) break;
         tc::fence_after_sync();
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          if (!mbar_wait(&full[s], phase, a.status)) {
+          if (!__all_sync(kFull, mbar_wait(&full[s], phase, a.status))) {
             ok = false;
             break;
           }
           tc::fence_after_sync();
-          const uint32_t off = static_cast<uint32_t>(s * stage_bytes) >> 4;
+          if (lead) {
+            const uint32_t off = static_cast<uint32_t>(s * stage_bytes) >> 4;
 #pragma unroll
-          for (int u = 0; u < SUB; ++u) {
-            const uint64_t ad = a_desc + off + u * (a_bytes >> 4), bd = b_desc + off + u * (b_bytes >> 4);
+            for (int u = 0; u < SUB; ++u) {
+              const uint64_t ad = a_desc + off + u * (a_bytes >> 4), bd = b_desc + off + u * (b_bytes >> 4);
 #pragma unroll
-            for (int kk = 0; kk < kBlockK / 32; ++kk)
-              mma_i8_ss(tmem + buf * TN, ad + kk * 2, bd + kk * 2, idesc, kb > kb0 || u || kk ? 1u : 0u);
+              for (int kk = 0; kk < kBlockK / 32; ++kk)
+                mma_i8_ss(tmem + buf * TN, ad + kk * 2, bd + kk * 2, idesc, kb > kb0 || u || kk ? 1u : 0u);
+            }
+            tc::commit(&empty[s]);
           }
-          tc::commit(&empty[s]);
           if (++s == ST) {
             s = 0;
             phase ^= 1u;
           }
         }
-        if (ok) tc::commit(&accf[buf]);
+        if (ok && lead) tc::commit(&accf[buf]);
       }
-      *s_consumed = it;
+      if (lane == 0) *s_consumed = it;
     }
   } else {
     const int quarter = warp & 3;

@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
   float* s_lse = s_scale + kScaleRing * 4 * 4 * 3;
   int32_t* s_pages = reinterpret_cast<int32_t*>(s_lse + kTiles * kM);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = tc::uniform_warp(), lane = threadIdx.x & 31;
   const int S = gridDim.y, part = blockIdx.y;
   // KV head fastest: the heaviest tiles of every head start in the first wave
   const int kvh = blockIdx.x % p.hkv;
@@ -323,45 +323,57 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
       // ------------------------------------------------------------ MMA issuers
       // Per tile: S(0), S(1), then for every block j PV(j), S(j + 2); one thread's MMAs run in order, so S(j + 2)
       // overwrites p'(j) only after PV(j) has read it.
+      // The whole warp runs the loop and one elected lane issues, so descriptors stay in uniform registers.
       const int t = warp - 1;
       const int nbx = nbt[t];
-      if (lane == 0 && nbx > 0) {
+      if (nbx > 0) {
         constexpr uint32_t kIdescS = tc::idesc_bf16_f32(kM, kN, false, false);
         constexpr uint32_t kIdescPV = idesc_f16_f32_bmn(kM, D);
-        bool ok = mbar_wait(q_full, 0, p.status);
+        const bool lead = tc::elect_one();
+        auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+          const bool ok = __all_sync(kFull, mbar_wait(bar, parity, p.status));
+          tc::fence_after_sync();
+          return ok;
+        };
+        bool ok = wait(q_full, 0);
         const uint64_t q_desc = tc::smem_desc_sw128(smem_addr(sQ + t * Cfg::kQBytes), 16, 1024);
         const uint64_t k_desc = tc::smem_desc_sw128(smem_addr(sKV), 16, 1024);
         const uint64_t v_desc = tc::smem_desc_sw128(smem_addr(sKV + kHalves * Cfg::kHalf), Cfg::kHalf, 1024);
         const uint32_t s_cols = tmem + t * 128, o_cols = tmem + kColO + t * 128;
+        int ss = 0, ps = 0;  // stages of the next S and PV
+        uint32_t s_phase = 0;
         auto issue_s = [&](int j) {
-          if (!mbar_wait(&kv_full[j % kStages], (j / kStages) & 1, p.status)) {
-            ok = false;
-            return;
-          }
-          tc::fence_after_sync();
-          const uint64_t kd = k_desc + static_cast<uint32_t>(((j % kStages) * Cfg::kKV) >> 4);
+          ok = wait(&kv_full[ss], s_phase);
+          if (!ok) return;
+          if (lead) {
+            const uint64_t kd = k_desc + static_cast<uint32_t>((ss * Cfg::kKV) >> 4);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t qo = ((kk >> 2) * (kM * 128) + (kk & 3) * 32) >> 4;
-            const uint32_t ko = ((kk >> 2) * Cfg::kHalf + (kk & 3) * 32) >> 4;
-            tc::mma_f16_ss(s_cols + (j & 1) * kN, q_desc + qo, kd + ko, kIdescS, kk > 0 ? 1u : 0u);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t qo = ((kk >> 2) * (kM * 128) + (kk & 3) * 32) >> 4;
+              const uint32_t ko = ((kk >> 2) * Cfg::kHalf + (kk & 3) * 32) >> 4;
+              tc::mma_f16_ss(s_cols + (j & 1) * kN, q_desc + qo, kd + ko, kIdescS, kk > 0 ? 1u : 0u);
+            }
+            tc::commit(&s_full[2 * t + (j & 1)]);
           }
-          tc::commit(&s_full[2 * t + (j & 1)]);
+          if (++ss == kStages) {
+            ss = 0;
+            s_phase ^= 1u;
+          }
         };
         auto issue_pv = [&](int j) {
-          const int sb = j & 1, s = j % kStages;
-          if (!mbar_wait(&p_full[2 * t + sb], (j >> 1) & 1, p.status)) {
-            ok = false;
-            return;
-          }
-          tc::fence_after_sync();
-          const uint64_t vd = v_desc + static_cast<uint32_t>((s * Cfg::kKV) >> 4);
+          const int sb = j & 1;
+          ok = wait(&p_full[2 * t + sb], (j >> 1) & 1);
+          if (!ok) return;
+          if (lead) {
+            const uint64_t vd = v_desc + static_cast<uint32_t>((ps * Cfg::kKV) >> 4);
 #pragma unroll
-          for (int ks = 0; ks < kN / 16; ++ks)
-            tc::mma_f16_ts(o_cols, s_cols + sb * kN + ks * 8, vd + ((ks * 2048) >> 4), kIdescPV,
-                           (j > 0 || ks > 0) ? 1u : 0u);
-          tc::commit(&o_done[2 * t + sb]);
-          tc::commit(&kv_empty[t * kStages + s]);
+            for (int ks = 0; ks < kN / 16; ++ks)
+              tc::mma_f16_ts(o_cols, s_cols + sb * kN + ks * 8, vd + ((ks * 2048) >> 4), kIdescPV,
+                             (j > 0 || ks > 0) ? 1u : 0u);
+            tc::commit(&o_done[2 * t + sb]);
+            tc::commit(&kv_empty[t * kStages + ps]);
+          }
+          if (++ps == kStages) ps = 0;
         };
         for (int j = 0; j < 2 && j < nbx && ok; ++j) issue_s(j);
         for (int j = 0; j < nbx && ok; ++j) {
