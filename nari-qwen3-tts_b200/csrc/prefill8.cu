@@ -17,7 +17,7 @@
 //   warp 3        brings the codes of a block by TMA (one box of 16 tokens, K and V, per lane) into a raw ring, and
 //                 the scale factors of four blocks at a time
 //   warps 4..7    converters: raw codes to 16 bits in the operands' 128-byte-swizzled layout
-//   warps 8..15   softmax, one query row per thread (8..11 tile A, 12..15 tile B)
+//   warps 8..23   softmax (8..15 tile A, 16..23 tile B), half of a query row's keys per thread
 // TMEM: S double-buffered per tile, p' over its own S buffer, O per tile.  The two tiles share every converted
 // block, which halves the conversions per product.  setmaxnreg gives the softmax warps the registers that the
 // others do not need; every role runs to its own end, with no code in common behind the split.
@@ -41,7 +41,7 @@ constexpr int kN = 64;        // keys per block
 constexpr int kStages = 3;     // converted blocks
 constexpr int kRaw = 3;        // raw blocks
 constexpr int kScaleRing = 4;  // groups of four blocks whose scale factors are kept
-constexpr int kThreads = 512;
+constexpr int kThreads = 768;
 constexpr int kPages = 1024;  // page ids of the row staged in shared memory
 constexpr int kRows = 512;    // rows of the batch whose tiles are put in order, longest first
 constexpr uint32_t kColO = 256;
@@ -56,7 +56,7 @@ struct P8Cfg {
   static constexpr int kRawBytes = 2 * p8::kN * D;             // [tile][K, V][16 tokens][D]
   static constexpr int kBars = 512;
   static constexpr int kScales = p8::kScaleRing * 4 * 4 * 3 * 4;  // [block][tile][score factor, log2 c, 1 / c]
-  static constexpr int kRowState = p8::kTiles * p8::kM * 4;    // log2-sum-exp of every row, for the join
+  static constexpr int kRowState = 3 * p8::kTiles * p8::kM * 4;  // of every row: log2-sum-exp, for the join; its halves' exchange
   static constexpr int kSmem =
       1024 + p8::kTiles * kQBytes + p8::kStages * kKV + p8::kRaw * kRawBytes + kBars + kScales + kRowState + 4 * p8::kPages;
 };
@@ -101,6 +101,17 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
+}
+// Whether `v` holds in any of the barrier's threads.
+__device__ __forceinline__ bool bar_any(int id, int n, bool v) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %3, 0;\n\tbarrier.cta.red.or.pred p, %1, %2, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(any)
+      : "r"(id), "r"(n), "r"(static_cast<uint32_t>(v))
+      : "memory");
+  return any != 0;
 }
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 template <int N>
@@ -241,7 +252,8 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
   int* found = reinterpret_cast<int*>(tmem_slot + 1);
   float* s_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(q_full) + Cfg::kBars);  // [block][4][3]
   float* s_lse = s_scale + kScaleRing * 4 * 4 * 3;
-  int32_t* s_pages = reinterpret_cast<int32_t*>(s_lse + kTiles * kM);
+  float* s_half = s_lse + kTiles * kM;  // [tile][half][row]
+  int32_t* s_pages = reinterpret_cast<int32_t*>(s_half + 2 * kTiles * kM);
 
   const int warp = tc::uniform_warp(), lane = threadIdx.x & 31;
   const int S = gridDim.y, part = blockIdx.y;
@@ -260,7 +272,7 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
     for (int s = 0; s < kTiles * kStages; ++s) mbar_init(&kv_empty[s], 1);
     for (int b = 0; b < 2 * kTiles; ++b) {
       mbar_init(&s_full[b], 1);
-      mbar_init(&p_full[b], 4);
+      mbar_init(&p_full[b], 8);
       mbar_init(&o_done[b], 1);
     }
     fence_barrier_init();
@@ -309,7 +321,7 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
   const bool have[kTiles] = {row >= 0 && t_first < qo_len, row >= 0 && t_first + tpt < qo_len};
 
   if (warp < 4) {
-    reg_dec<56>();
+    reg_dec<40>();
     if (warp == 0) {
       if (lane == 0 && nb > 0) {
         const int nq = nbt[1] > 0 ? kTiles : 1;
@@ -368,7 +380,7 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
             const uint64_t vd = v_desc + static_cast<uint32_t>((ps * Cfg::kKV) >> 4);
 #pragma unroll
             for (int ks = 0; ks < kN / 16; ++ks)
-              tc::mma_f16_ts(o_cols, s_cols + sb * kN + ks * 8, vd + ((ks * 2048) >> 4), kIdescPV,
+              tc::mma_f16_ts(o_cols, s_cols + sb * kN + (ks >> 1) * 32 + (ks & 1) * 8, vd + ((ks * 2048) >> 4), kIdescPV,
                              (j > 0 || ks > 0) ? 1u : 0u);
             tc::commit(&o_done[2 * t + sb]);
             tc::commit(&kv_empty[t * kStages + ps]);
@@ -467,7 +479,7 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------ converters
-    reg_dec<112>();
+    reg_inc<88>();
     {
       const int ct = threadIdx.x - 128;
       constexpr int kChunks = D / 16;       // 16-code chunks of a row
@@ -545,48 +557,50 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
     bar_sync(0, kThreads);
   } else {
     // ------------------------------------------------------------ softmax
-    reg_inc<168>();
-    const int t = (warp - 8) >> 2;
+    reg_inc<88>();
+    const int t = (warp - 8) >> 3, h = ((warp - 8) >> 2) & 1;
     const int nbx = nbt[t];
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;  // tile row = TMEM lane
+    const int pair = 5 + t * 4 + quarter;  // barrier of the two warps that share 32 rows
     const uint32_t t_row = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t col_s = t * 128, col_o = kColO + t * 128;
+    const uint32_t col_s = t * 128 + h * 32, col_o = kColO + t * 128 + h * (D / 2);
     uint64_t* sfull = s_full + 2 * t;
     uint64_t* pfull = p_full + 2 * t;
     uint64_t* odone = o_done + 2 * t;
-    const int lim = shift + t_first + t * tpt + r / G;  // last key that this row sees
+    float* mine = s_half + (t * 2 + h) * kM + r;
+    const float* other = s_half + (t * 2 + 1 - h) * kM + r;
+    const int lim = min(shift + t_first + t * tpt + r / G, kv_len - 1);  // last key that this row sees
     const float NEG_INF = -__int_as_float(0x7f800000);
     float m_used = NEG_INF, l = 0.f;
     bool ok = true;
+    // a warp whose wait gave up goes on to the barriers that its partner waits in
     for (int j = 0; j < nbx; ++j) {
       const int sb = j & 1, s = j % (4 * kScaleRing);
-      if ((j & 3) == 0) ok = mbar_wait(&sc_full[(j >> 2) % kScaleRing], ((j >> 2) / kScaleRing) & 1, p.status);
-      ok = mbar_wait(&sfull[sb], (j >> 1) & 1, p.status) && ok;
+      if (ok && (j & 3) == 0) ok = mbar_wait(&sc_full[(j >> 2) % kScaleRing], ((j >> 2) / kScaleRing) & 1, p.status);
+      if (ok) ok = mbar_wait(&sfull[sb], (j >> 1) & 1, p.status);
       ok = __all_sync(kFull, ok);
-      if (!ok) break;
       tc::fence_after_sync();
-      uint32_t sr[64];
-      tc::ld_32x32b_x32(t_row + col_s + sb * kN, *reinterpret_cast<uint32_t(*)[32]>(&sr[0]));
-      tc::ld_32x32b_x32(t_row + col_s + sb * kN + 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[32]));
-      float fk[4], fe[4], fv[4];
+      uint32_t sr[32];
+      tc::ld_32x32b_x32(t_row + col_s + sb * kN, sr);
+      float fk[2], fe[2], fv[2];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        fk[g] = s_scale[(s * 4 + g) * 3];
-        fe[g] = s_scale[(s * 4 + g) * 3 + 1];
-        fv[g] = s_scale[(s * 4 + g) * 3 + 2];
+      for (int g = 0; g < 2; ++g) {
+        const float* f = s_scale + (s * 4 + h * 2 + g) * 3;
+        fk[g] = f[0];
+        fe[g] = f[1];
+        fv[g] = f[2];
       }
       tc::wait_ld();
-      const int base = (j0 + j) * kN;
-      if (base + kN - 1 > lim || base + kN > kv_len) {
-        const int last = min(lim, kv_len - 1) - base;  // columns behind it are hidden
+      const int last = lim - (j0 + j) * kN - h * 32;  // columns behind it are hidden
+      if (last < 31) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
+        for (int c = 0; c < 32; ++c)
           if (c > last) sr[c] = __float_as_uint(NEG_INF);
       }
       float mx = NEG_INF;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+      for (int g = 0; g < 2; ++g) {
         const uint32_t* x = sr + g * 16;
         float a = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
         float b = max3(__uint_as_float(x[3]), __uint_as_float(x[4]), __uint_as_float(x[5]));
@@ -597,45 +611,46 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
         a = max3(a, __uint_as_float(x[14]), __uint_as_float(x[15]));
         mx = fmaxf(mx, fmaf(fmaxf(a, b), fk[g], fe[g]));
       }
-      const float m_new = fmaxf(m_used, mx);
-      const bool need = m_used != NEG_INF && m_new > m_used + 7.f;
-      if (__any_sync(kFull, need)) {
-        // the reference moves: rescale this warp's O rows once PV(j - 1) has landed
-        ok = mbar_wait(&odone[(j - 1) & 1], ((j - 1) >> 1) & 1, p.status);
-        ok = __all_sync(kFull, ok);
-        if (!ok) break;
-        tc::fence_after_sync();
-        const float alpha = need ? ex2(m_used - m_new) : 1.f;
+      // the reference moves where either half of a row asks for it; until it has one, at the first key
+      if (bar_any(pair, 64, ok && mx > m_used + 7.f)) {
+        *mine = mx;
+        bar_sync(pair, 64);
+        const float m_new = fmaxf(m_used, fmaxf(mx, *other));
+        const bool move = m_new > m_used + 7.f;
+        // rescale this warp's half of the O rows once PV(j - 1) has landed
+        if (j > 0) {
+          if (ok) ok = mbar_wait(&odone[(j - 1) & 1], ((j - 1) >> 1) & 1, p.status);
+          ok = __all_sync(kFull, ok);
+          tc::fence_after_sync();
+          const float alpha = move ? ex2(m_used - m_new) : 1.f;
 #pragma unroll
-        for (int ch = 0; ch < D / 32; ++ch) {
-          uint32_t o[32];
-          tc::ld_32x32b_x32(t_row + col_o + ch * 32, o);
-          tc::wait_ld();
+          for (int ch = 0; ch < D / 32; ++ch) {
+            uint32_t o[16];
+            tc::ld_32x32b_x16(t_row + col_o + ch * 16, o);
+            tc::wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tc::st_32x32b_x32(t_row + col_o + ch * 32, o);
-        }
-        tc::wait_st();
-        if (need) {
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tc::st_32x32b_x16(t_row + col_o + ch * 16, o);
+          }
+          tc::wait_st();
           l *= alpha;
-          m_used = m_new;
         }
+        if (move) m_used = m_new;
       }
-      if (m_used == NEG_INF) m_used = m_new;
       const float ref = m_used == NEG_INF ? 0.f : m_used;  // a row that has seen no key yet
-      uint32_t pk[32];
+      uint32_t pk[16];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+      for (int g = 0; g < 2; ++g) {
         const uint64_t c2 = pk2(fk[g], fk[g]);
         const float off = fe[g] - ref + 8.f;
         const uint64_t o2 = pk2(off, off);
         uint64_t sum = pk2(0.f, 0.f);
 #pragma unroll
-        for (int h = 0; h < 8; h += 4) {
+        for (int q = 0; q < 8; q += 4) {
           float pv[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int i = g * 16 + 2 * (h + e);
+            const int i = g * 16 + 2 * (q + e);
             float lo, hi;
             unpk2(fma2(pk2(sr[i], sr[i + 1]), c2, o2), lo, hi);
             pv[2 * e] = ex2(lo);
@@ -648,16 +663,20 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
         unpk2(sum, lo, hi);
         l = fmaf(lo + hi, fv[g], l);
       }
-      tc::st_32x32b_x32(t_row + col_s + sb * kN, pk);
+      tc::st_32x32b_x16(t_row + col_s + sb * kN, pk);
       tc::wait_st();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&pfull[sb]);
+      if (lane == 0 && ok) mbar_arrive(&pfull[sb]);
     }
     // epilogue: O / l
     ok = nbx > 0 && ok && mbar_wait(&odone[(nbx - 1) & 1], ((nbx - 1) >> 1) & 1, p.status);
     ok = __all_sync(kFull, ok);
     tc::fence_after_sync();
+    bar_sync(pair, 64);  // the exchange's last readers
+    *mine = l;
+    bar_sync(pair, 64);
+    l = h == 0 ? l + *other : *other + l;
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     if (S == 1) {
       if (have[t]) {
@@ -665,12 +684,10 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
         // all its tokens leaves through one TMA store per 64 dims, a ragged one row by row
         uint8_t* sO = sQ + t * Cfg::kQBytes;
 #pragma unroll
-        for (int ch = 0; ch < D / 32; ++ch) {
+        for (int ch = 0; ch < D / 64; ++ch) {
           uint32_t o[32];
-          if (ok) {
-            tc::ld_32x32b_x32(t_row + col_o + ch * 32, o);
-            tc::wait_ld();
-          }
+          tc::ld_32x32b_x32(t_row + col_o + ch * 32, o);
+          tc::wait_ld();
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             uint4 w = make_uint4(0u, 0u, 0u, 0u);
@@ -680,15 +697,15 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
               w.z = pack_bf16x2(__uint_as_float(o[v * 8 + 4]) * inv, __uint_as_float(o[v * 8 + 5]) * inv);
               w.w = pack_bf16x2(__uint_as_float(o[v * 8 + 6]) * inv, __uint_as_float(o[v * 8 + 7]) * inv);
             }
-            const int c = (ch & 1) * 4 + v;
-            *reinterpret_cast<uint4*>(sO + (ch >> 1) * (kM * 128) + r * 128 + ((c ^ (r & 7)) << 4)) = w;
+            const int c = h * (D / 16) + ch * 4 + v;  // 16-byte piece of the row
+            *reinterpret_cast<uint4*>(sO + (c >> 3) * (kM * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = w;
           }
         }
         const bool full = p.tma_out && t_first + (t + 1) * tpt <= qo_len;
         if (full) fence_proxy_async_smem();
-        bar_sync(2 + t, 128);
+        bar_sync(2 + t, 256);
         if (full) {
-          if (quarter == 0 && lane == 0) {
+          if (h == 0 && quarter == 0 && lane == 0) {
             for (int half = 0; half < kHalves; ++half)
               tma_store_3d(&omap, sO + half * (kM * 128), half * 64, kvh * G, q0 + t_first + t * tpt);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -696,7 +713,7 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
           }
         } else {
           constexpr int kC = D / 8;  // 16-byte pieces of an output row
-          for (int i = r; i < kM * kC; i += kM) {
+          for (int i = h * kM + r; i < kM * kC; i += 2 * kM) {
             const int rr = i / kC, c = i % kC;
             const int tok = t_first + t * tpt + rr / G;
             if (rr < tpt * G && tok < qo_len) {
@@ -718,24 +735,22 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
     } else {
       // the row's part: normalised O in fp32 over the KV stages (every reader of them is done once both tiles'
       // last products are: bar 4) and its log2-sum-exp; -inf for a part that saw no key
-      bar_sync(4, 256);
+      bar_sync(4, 512);
       uint8_t* sO = sKV + t * (kM * D * 4);
       const bool any = ok && inv != 0.f;
-      s_lse[t * kM + r] = any ? m_used - 8.f + log2f(l) : NEG_INF;
+      if (h == 0) s_lse[t * kM + r] = any ? m_used - 8.f + log2f(l) : NEG_INF;
 #pragma unroll
-      for (int ch = 0; ch < D / 32; ++ch) {
+      for (int ch = 0; ch < D / 64; ++ch) {
         uint32_t o[32];
-        if (ok) {
-          tc::ld_32x32b_x32(t_row + col_o + ch * 32, o);
-          tc::wait_ld();
-        }
+        tc::ld_32x32b_x32(t_row + col_o + ch * 32, o);
+        tc::wait_ld();
 #pragma unroll
         for (int f = 0; f < 8; ++f) {
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
           if (any)
             v = make_float4(__uint_as_float(o[f * 4]) * inv, __uint_as_float(o[f * 4 + 1]) * inv,
                             __uint_as_float(o[f * 4 + 2]) * inv, __uint_as_float(o[f * 4 + 3]) * inv);
-          *reinterpret_cast<float4*>(sO + r * (D * 4) + (((ch * 8 + f) ^ (r & 7)) << 4)) = v;
+          *reinterpret_cast<float4*>(sO + r * (D * 4) + (((h * (D / 8) + ch * 8 + f) ^ (r & 7)) << 4)) = v;
         }
       }
       // join: CTA `part` finishes every S-th slice of the 256 rows
@@ -743,7 +758,7 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
       gemm_detail::cluster_wait();
       constexpr int kF = D / 4;
       const int rows = kTiles * kM / S;
-      for (int i = static_cast<int>(threadIdx.x) - 256; i < rows * kF; i += 256) {
+      for (int i = static_cast<int>(threadIdx.x) - 256; i < rows * kF; i += 512) {
         const int rr = part * rows + i / kF, f = i % kF;
         const int jt = rr / kM, jr = rr % kM;
         const int tok = t_first + jt * tpt + jr / G;
