@@ -59,6 +59,7 @@ struct P8Cfg {
   static constexpr int kRowState = 3 * p8::kTiles * p8::kM * 4;  // of every row: log2-sum-exp, for the join; its halves' exchange
   static constexpr int kSmem =
       1024 + p8::kTiles * kQBytes + p8::kStages * kKV + p8::kRaw * kRawBytes + kBars + kScales + kRowState + 4 * p8::kPages;
+  static_assert(p8::kStages * kKV + p8::kRaw * kRawBytes >= p8::kTiles * p8::kM * D * 4, "the join stages O over them");
 };
 
 struct Prefill8Args {
