@@ -175,17 +175,18 @@ __device__ __forceinline__ bool count_in(int32_t* ticket, int others, int lane) 
 }
 
 // Joins `count` parts of one row and KV head: sum_i 2^(lse_i - M) O_i / sum_i 2^(lse_i - M) for every query head of
-// the group, by one warp.  slot(i): the slot of part i.  Goes to `out` (last) or to slot `dst` as a part.  The loads
-// of two sets of heads and eight parts are in flight at once: a join is a chain of trips to L2.
-template <int D, typename Slot>
+// the group, by WARPS warps of which this is number `sub`.  slot(i): the slot of part i.  Goes to `out` (last) or to slot
+// `dst` as a part.  The loads of two sets of heads and eight parts are in flight at once: a join is a chain of trips to
+// L2.
+template <int D, int WARPS, typename Slot>
 __device__ __forceinline__ void join_parts(const Decode8Args& p, int row, int kvh, int count, Slot slot, bool last,
-                                           int dst, int lane) {
+                                           int dst, int sub, int lane) {
   constexpr int QD = D / 4;    // float4 of a head
   constexpr int HP = 32 / QD;  // heads of a set: the warp's lanes
   constexpr int kBatch = 8;
   const float NEG_INF = -__int_as_float(0x7f800000);
   const int col = lane % QD;
-  for (int g0 = 0; g0 < p.group; g0 += 2 * HP) {
+  for (int g0 = 2 * HP * sub; g0 < p.group; g0 += 2 * HP * WARPS) {
     int head[2];
     bool live[2];
     float m[2], sum[2];
@@ -291,6 +292,7 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
   __shared__ int s_warp_sum[kWarps + 1];
   __shared__ int s_issued;
   __shared__ int s_progress[kWarps];
+  __shared__ int s_fix[HPC][2];  // what a head's first warp tells the others
 
   // see nqt_decode_attention_ex: by default everything waits for the previous grid; with `early` only q, each
   // row's last tile and its scales, the workspace and all writes do
@@ -733,8 +735,20 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
       i0 = i1;
     }
 
-    // joins, behind the tile loop: its accumulators are dead here
-    __syncwarp();
+    // joins, behind the tile loop: its accumulators are dead here; a head's warps share the query heads
+    auto head_sync = [&]() {
+      if (kPerHead > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + hw), "n"(kPerHead * 32) : "memory");
+      else __syncwarp();
+    };
+    if (kPerHead > 1) {
+      if (sub == 0 && lane == 0) {
+        s_fix[hw][0] = fix_a;
+        s_fix[hw][1] = fix_b;
+      }
+      head_sync();
+      fix_a = s_fix[hw][0];
+      fix_b = s_fix[hw][1];
+    }
     for (int f = 0; f < 2; ++f) {
       const int r = f == 0 ? fix_a : fix_b;
       if (r < 0) continue;
@@ -743,14 +757,25 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
       const int lo = c - (c - ca) % kGroup8, hi = min(cb, lo + kGroup8 - 1);
       const bool late = first_tile(total, ca, n) < r0;
       const int groups = (cb - ca) / kGroup8;  // less one
-      join_parts<D>(p, r, kvh, hi - lo + 1, [&](int i) { return part_slot(lo + i, ca, late); }, groups == 0,
-                    part_slot(lo, ca, late), lane);
+      join_parts<D, kPerHead>(p, r, kvh, hi - lo + 1, [&](int i) { return part_slot(lo + i, ca, late); }, groups == 0,
+                              part_slot(lo, ca, late), sub, lane);
       if (groups == 0) continue;
-      __syncwarp();
-      if (count_in(p.tickets + static_cast<int64_t>(r) * p.hq + kvh, groups, lane))
-        join_parts<D>(
-            p, r, kvh, groups + 1,
-            [&](int i) { return part_slot(ca + i * kGroup8, ca, late); }, true, 0, lane);
+      head_sync();
+      int32_t* ticket = p.tickets + static_cast<int64_t>(r) * p.hq + kvh;
+      bool whole;
+      if (kPerHead > 1) {
+        if (sub == 0) {
+          const bool w = count_in(ticket, groups, lane);
+          if (lane == 0) s_fix[hw][f] = w;
+        }
+        head_sync();
+        whole = s_fix[hw][f] != 0;
+      } else {
+        whole = count_in(ticket, groups, lane);
+      }
+      if (whole)
+        join_parts<D, kPerHead>(
+            p, r, kvh, groups + 1, [&](int i) { return part_slot(ca + i * kGroup8, ca, late); }, true, 0, sub, lane);
     }
     if (lane == 0) s_progress[warp] = stop;
   }
