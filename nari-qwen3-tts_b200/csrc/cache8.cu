@@ -222,10 +222,11 @@ __global__ void __launch_bounds__(kWarps8 * 32, 4) write8_kernel(const __grid_co
     __syncthreads();
   }
 
-  // this CTA's units: query heads, then K heads, then V heads
+  // this CTA's units: query heads, then K heads, then V heads; the dearer K and V start first (4893 tokens, 16 + 8 heads
+  // of 128: 31 us, against 34 the other way round, and 46 with the kinds mixed in every CTA)
   const int units = a.hq + 2 * a.hkv;
   const int per = (units + gridDim.y - 1) / gridDim.y;
-  const int u0 = blockIdx.y * per, u1 = min(units, u0 + per);
+  const int u0 = (gridDim.y - 1 - blockIdx.y) * per, u1 = min(units, u0 + per);
 
   const int sub = lane / kLanes, l8 = lane % kLanes;  // row of the warp's four, place in it
   {
