@@ -721,7 +721,7 @@ class Int8Weight:
             data[:, :half, :k] = q.view(2, half, k) if q.is_contiguous() else torch.stack([q[:half], q[half:]])
             self.data = data.view(2, groups, 16, pitch).transpose(0, 1).reshape(-1, pitch)
             scales = torch.zeros((2, groups * 16), dtype=torch.float32, device=q.device)
-            scales[:, :half] = scale.view(2, half)
+            scales[:, :half] = scale.reshape(2, half)
             self.data_scale = scales.view(2, groups, 16).transpose(0, 1).reshape(-1)
         elif q.stride(1) == 1 and _row_pitch(q) % 16 == 0 and _row_pitch(q) >= k and q.data_ptr() % 16 == 0:
             self.data, self.data_scale = q, scale.contiguous()
