@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
 #include <utility>
 
 #include "../../include/nqt.h"
@@ -69,6 +70,17 @@ cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, 
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
+
+// Once for each device: a function's attributes belong to the device that was current when they were set.
+struct DeviceOnce {
+  std::once_flag flags[64];
+  template <typename F>
+  void operator()(F&& f) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::call_once(flags[dev & 63], f);
+  }
+};
 
 int num_sms();
 

@@ -814,7 +814,7 @@ int launch8(const void* layer, Decode8Args a, cudaStream_t s) {
     return NQT_ERR_CUDA;
   }
   static int few_occ = 1;
-  static std::once_flag once;
+  static DeviceOnce once;
   auto occupancy = [](int smem) {
     int occ = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, decode8_kernel<D, HPC, STAGES, E4M3>, Cfg::kThreads, smem) !=
@@ -823,7 +823,7 @@ int launch8(const void* layer, Decode8Args a, cudaStream_t s) {
       occ = 1;
     return occ;
   };
-  std::call_once(once, [&] {
+  once([&] {
     cudaFuncSetAttribute(decode8_kernel<D, HPC, STAGES, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          Cfg::smem(kMaxRows8));
     few_occ = occupancy(Cfg::smem(kFewRows8));

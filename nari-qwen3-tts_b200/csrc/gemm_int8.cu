@@ -716,8 +716,8 @@ __global__ void __launch_bounds__(256, 2) gemv_int8_kernel(const __grid_constant
 
 template <int M>
 int launch_gemv(const GemvArgs& a, cudaStream_t s) {
-  static std::once_flag once;
-  std::call_once(once, [] {
+  static DeviceOnce once;
+  once([] {
     cudaFuncSetAttribute(gemv_int8_kernel<M>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemvSmem);
   });
   const int pairs = (a.n + 1) / 2;
@@ -749,9 +749,9 @@ int run_gemv(const GemvArgs& a, cudaStream_t s) {
 // ------------------------------------------------------------------ host
 // CTAs that run at once in clusters of `split` (each CTA takes its SM whole; clusters leave some SMs over).
 int max_ctas(int split) {
-  static std::once_flag once;
+  static DeviceOnce once;
   static int most[kMaxSplit + 1];
-  std::call_once(once, [] {
+  once([] {
     for (auto kernel : {gemm_int8_kernel<false, 1>, gemm_int8_kernel<false, 2>, gemm_int8_kernel<true, 1>,
                         gemm_int8_kernel<true, 2>})
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem8);

@@ -836,8 +836,8 @@ template <int D, bool E4M3>
 int launch_prefill8(const CUtensorMap& qmap, const CUtensorMap& kvmap, const CUtensorMap& omap,
                     const Prefill8Args& a, int total_q, cudaStream_t s) {
   using Cfg = P8Cfg<D>;
-  static std::once_flag once;
-  std::call_once(once, [] {
+  static DeviceOnce once;
+  once([] {
     cudaFuncSetAttribute(prefill8_kernel<D, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   });
   const int tokens_per_cta = p8::kTiles * (p8::kM / a.group);
