@@ -160,7 +160,7 @@ PyObject* decode8(PyObject* const* a) {
   const long long cap = a[7] == Py_None ? rows : integer(a[7]);
   const double scale = a[8] == Py_None ? 1.0 / std::sqrt(static_cast<double>(q.size(2))) : number(a[8]);
   const long long flags = integer(a[10]);
-  if (cap < rows) value_error("batch_capacity must cover the rows");
+  if (cap < rows || cap > 0x7fffffff) value_error("batch_capacity must cover the rows");
   if (!ws.is_contiguous()) value_error("the decode workspace must be contiguous");
   Device dev;
   for (int i = 0; i < 7; ++i) dev.add(tensor(a[i]));
@@ -194,8 +194,9 @@ PyObject* prefill8(PyObject* const* a) {
   dev.add(out);
   if (!out) out = contiguous_like(q0);
   if (rows == 0 || q0.size(0) == 0) return THPVariable_Wrap(*out);
-  at::Tensor q = q0;
-  if (reinterpret_cast<uintptr_t>(q.const_data_ptr()) % 16 || q.stride(0) % 8 || q.stride(1) % 8)
+  at::Tensor q = q0;  // a tensor map needs 16-byte strides, and none of zero (a broadcast query)
+  if (reinterpret_cast<uintptr_t>(q.const_data_ptr()) % 16 || q.stride(0) % 8 || q.stride(1) % 8 || q.stride(0) == 0 ||
+      q.stride(1) == 0)
     q = q.clone(at::MemoryFormat::Contiguous);
   return result(on_device(dev, [&](int32_t* status, void* stream) {
     return f_prefill8(q.const_data_ptr(), q.stride(0), q.stride(1), cache.const_data_ptr(),

@@ -244,7 +244,7 @@ def batch_prefill_paged8(
 ) -> torch.Tensor:
     """``batch_prefill_paged`` over an 8-bit cache: ragged causal chunks, query i of a chunk of n sees the keys up
     to kv_len - n + i.  Queries that see no key give zeros; tokens behind ``qo_indptr[batch]`` are not written.  A
-    query whose rows are not 16-byte aligned is copied first."""
+    query that is broadcast or whose rows are not 16-byte aligned is copied first."""
 
     args = (query, layer_cache, layer_scales, qo_indptr, kv_indptr, kv_indices, last_page_len, batch, sm_scale, out)
     fn = (_lib._bind or _lib.bind()).prefill8

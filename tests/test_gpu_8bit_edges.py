@@ -184,3 +184,34 @@ def test_products_behind_32_bit_offsets(nqt, cuda):
     for rows in (slice(0, 3), slice(m - 130, m)):
         want = x[rows].cpu().double() @ wq.double().t() * (0.5 * float(torch.tensor(0.01)))
         assert ((out[rows].cpu().double() - want).abs() <= (2.0**-8 + 2.0**-21) * want.abs()).all()
+
+
+def test_broadcast_queries(nqt, cuda):
+    """One query for every row, or one head for all, without a copy in memory."""
+
+    codes, scales, indptr, indices, last = make_cache8([40, 33, 90], seed=21)
+    dev = [t.to(cuda) for t in (codes, scales, indptr, indices, last)]
+    ws = nqt.decode_paged8_workspace(3, 16, 128, cuda)
+    qo = torch.tensor([0, 1, 2, 3], dtype=torch.int32)
+    for q in (_q(1, 16, 128, 22).expand(3, 16, 128), _q(3, 1, 128, 23).expand(3, 16, 128)):
+        want = oc8.attention(q, numbers(codes), scales.double(), indptr, indices, last)
+        base = q.to(cuda)[:1, :, :] if q.stride(0) == 0 else q.to(cuda)[:, :1]
+        dq = base.expand(3, 16, 128)
+        assert 0 in dq.stride()
+        _close(nqt.batch_decode_paged8(dq, *dev, ws), *want)
+        _close(nqt.batch_prefill_paged8(dq, *dev[:2], qo.to(cuda), *dev[2:]), *want)
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 6, 7, 8])
+def test_prefill_groups_over_long_keys(nqt, cuda, group):
+    """Every group size, tiles with rows left over, keys beyond one stage of the rings, chunks that end inside a tile."""
+
+    chunks, lens = [150, 1, 61], [400, 1000, 61]
+    codes, scales, indptr, indices, last = make_cache8(lens, kind="e4m3", hkv=2, d=128, page_size=32, seed=group)
+    q = _q(sum(chunks), 2 * group, 128, 31)
+    qo = torch.tensor([0, 150, 151, 212], dtype=torch.int32)
+    want = oc8.attention(q, numbers(codes), scales.double(), indptr, indices, last, qo)
+    dev = [t.to(cuda) for t in (q, codes, scales, qo, indptr, indices, last)]
+    first = nqt.batch_prefill_paged8(*dev)
+    assert torch.equal(first, nqt.batch_prefill_paged8(*dev))
+    _close(first, *want)
