@@ -215,3 +215,31 @@ def test_prefill_groups_over_long_keys(nqt, cuda, group):
     first = nqt.batch_prefill_paged8(*dev)
     assert torch.equal(first, nqt.batch_prefill_paged8(*dev))
     _close(first, *want)
+
+
+def test_prefill_more_work_than_the_gpu_holds_at_once(nqt, cuda):
+    """Far more tiles than SMs, of very different costs: CTAs take over one another's work; rows without queries or keys
+    among them.  Equal from launch to launch, with tokens behind the last chunk left as they were."""
+
+    g = torch.Generator().manual_seed(41)
+    chunks = [int(n) for n in torch.randint(0, 260, (48,), generator=g)] + [0, 3, 700, 0]
+    lens = [n + int(e) for n, e in zip(chunks, torch.randint(0, 200, (52,), generator=g), strict=True)]
+    lens[5], chunks[7] = 0, 0  # queries without keys, keys without queries
+    codes, scales, indptr, indices, last = make_cache8(lens, kind="int8", hkv=8, d=64, seed=43)
+    total = sum(chunks)
+    q = _q(total + 5, 8, 64, 44)
+    qo = torch.tensor([0, *torch.tensor(chunks).cumsum(0).tolist()], dtype=torch.int32)
+    dev = [t.to(cuda) for t in (q, codes, scales, qo, indptr, indices, last)]
+    out = torch.full((total + 5, 8, 64), 7.0, dtype=torch.bfloat16, device=cuda)
+    nqt.kernels.clear_status(cuda)
+    first = nqt.batch_prefill_paged8(*dev, out=out).clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        nqt.batch_prefill_paged8(*dev, out=out)
+    for _ in range(20):
+        out[:total] = 0
+        graph.replay()
+        assert torch.equal(out, first)
+    assert nqt.kernels.read_status(cuda) == 0 and (first[total:] == 7).all()
+    want, mag = oc8.attention(q[:total], numbers(codes), scales.double(), indptr, indices, last, qo)
+    _close(first[:total], want, mag)
