@@ -161,9 +161,27 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
+// One look at an mbarrier phase that does not suspend the thread (try_wait may, until the phase completes).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Bounded wait on an mbarrier phase.  Returns false (and reports a timeout)
-// when the phase did not complete within kWaitLimitNs.
+// when the phase did not complete within the limit; a limit of zero is one look.
 __device__ __forceinline__ bool mbar_wait_ns(uint64_t* bar, uint32_t parity, int32_t* status, uint64_t limit_ns) {
+  if (limit_ns == 0) {
+    const bool done = mbar_test(bar, parity);
+    if (!done) report(status, NQT_DEV_TIMEOUT);
+    return done;
+  }
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t start = global_timer_ns();
   while (true) {

@@ -121,19 +121,9 @@ __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint
       : "memory");
 }
 
-// Bounded pipeline wait; with NQT_DECODE_SHORT_WAIT (limit 0) one look at the barrier that does not suspend.
+// Bounded pipeline wait; with NQT_DECODE_SHORT_WAIT (limit 0) one look at the barrier.
 __device__ __forceinline__ bool pipe_wait(uint64_t* bar, uint32_t parity, const Decode8Args& p) {
-  if (p.wait_ns != 0) return mbar_wait_ns(bar, parity, p.status, p.wait_ns);
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity)
-      : "memory");
-  if (!ok) report(p.status, NQT_DEV_TIMEOUT);
-  return ok != 0;
+  return mbar_wait_ns(bar, parity, p.status, p.wait_ns);
 }
 
 __device__ __forceinline__ int atomic_inc_acq_rel(int32_t* addr) {
