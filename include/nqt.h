@@ -613,8 +613,8 @@ int nqt_decode_attention8(
 /*
  * Ragged causal prefill attention over an 8-bit layer: nqt_prefill_attention's
  * contract for head_dim 64 and 128, any num_qo_heads / num_kv_heads <= 8 and
- * sm_scale >= 0.  q 16-byte aligned with strides that are multiples of 8; out any
- * alignment (16-byte aligned rows leave faster).  Queries that see no key, and
+ * sm_scale >= 0.  q 16-byte aligned with positive strides that are multiples of 8;
+ * out any alignment (rows on multiples of 32 or 16 bytes leave faster).  Queries that see no key, and
  * rows without pages, give zeros; tokens behind qo_indptr[batch] are left as
  * they are.  No workspace: when the query tiles do not fill the GPU, clusters
  * of CTAs share the keys of one tile and join in shared memory.
@@ -643,8 +643,9 @@ int nqt_prefill_attention8(
  * Any m, n >= 1 and 1 <= k <= 131072; xq and w 16-byte aligned with row pitches
  * (bytes) that are multiples of 16; y any row pitch.  No workspace.
  *
- * nqt_linear_int8: both for bf16 x, with xq [m, ldxq] and xscale [m] as scratch.
- * Launched with programmatic stream serialization.
+ * nqt_linear_int8: both for bf16 x, with xq [m, ldxq] and xscale [m] as scratch
+ * (up to 8 rows one launch that does not use them, else two).
+ * All are launched with programmatic stream serialization.
  */
 int nqt_int8_quantize_rows(const void* x, int64_t ldx, int m, int k, void* q, int64_t ldq, float* scale,
                            void* stream);

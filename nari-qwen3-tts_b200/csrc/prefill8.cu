@@ -30,9 +30,9 @@
 // walking over a part of its keys; the parts are joined in the cluster's shared memory in CTA order, so there is no
 // workspace and nothing depends on timing.
 //
-// Bound by the softmax warps' instructions: a block costs about 2150 clocks, of which the tensor pipe and MUFU each need
-// about 1024.  On one B200 (16 query and 8 KV heads of 128): eight prompts of 2048 tokens 187 us, eight first chunks of 128
-// to 1024 53 us, chunks of 301 and 515 behind 9000 to 16001 tokens 166 us.
+// Bound by the softmax warps' instructions: a block costs about 2150 clocks, of which the tensor pipe and MUFU each
+// need about 1024.  On one B200 (16 query and 8 KV heads of 128, captured graphs): eight prompts of 2048 tokens 187 us,
+// eight first chunks of 128 to 1024 53 us, two chunks of 301 to 515 behind 9000 to 16001 tokens 166 us.
 #include "cache8.cuh"
 #include "gemm_common.cuh"
 #include "tcgen05.cuh"
@@ -1121,6 +1121,7 @@ extern "C" int nqt_prefill_attention8(const void* q, int64_t q_stride_tok, int64
   const int group = num_qo_heads / num_kv_heads;
   if (group > 8) return NQT_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(q) & 15) || q_stride_tok % 8 || q_stride_head % 8) return NQT_ERR_ARG;
+  if (q_stride_tok <= 0 || q_stride_head <= 0) return NQT_ERR_ARG;
   if (total_q_tokens == 0) return NQT_OK;
   CUtensorMap qmap, kvmap;
   rc = encode_rows(&qmap, q, q_stride_tok, q_stride_head, total_q_tokens, num_qo_heads, group, head_dim);
