@@ -33,7 +33,7 @@
 // time (gate and up of one column) with dp4a.
 //
 // One B200, captured graphs, weights from HBM, with the quantiser: 1 x 2048 x 2048
-// with bias 3.9 us; 64 x 12288 x 2048 with SwiGLU 7.9; 64 x 2048 x 6144 9.8;
+// with bias 3.9 us; 64 x 12288 x 2048 with SwiGLU 7.8; 64 x 2048 x 6144 9.1;
 // 4613 x 2048 x 6144 56.5, of which the product 42 (2.8 POP/s, tensor pipe 66 %
 // busy).
 #include <algorithm>
@@ -787,11 +787,11 @@ int max_ctas(int split) {
 int boxes_per_stage(int rows, int tn) { return 3 * 2 * (rows + tn) * kBlockK <= kRing8 ? 2 : 1; }
 
 // Weight rows per tile, and the CTAs that share a tile's K.  The times of a wave's tiles in ns, fitted to a sweep over
-// 16 to 4613 tokens and four weights on one B200.  A box of K costs its barriers and the issue of its products, about
-// 200 with two boxes a stage and 270 with one, and wide tiles what they bring into shared memory.  So tiles are as
-// narrow as one wave allows (64 tokens x 12288 x 2048: width 96, 8.5 us, against 128, 8.8, and 192, 10.4), and K is
+// 16 to 4613 tokens and five weights on one B200.  A box of K costs its barriers and the issue of its products, about
+// 120 with two boxes a stage and 270 with one, and wide tiles what they bring into shared memory.  So tiles are as
+// narrow as one wave allows (64 tokens x 12288 x 2048: width 96, 7.8 us, against 128, 8.5, and 192, 10.0), and K is
 // shared where that saves more boxes than the cluster's two barriers and the exchange of rows x tn sums cost
-// (64 tokens x 2048 x 6144: 7.5 us, against 12.6 undivided; 64 x 4096 x 2048: 7.0 against 6.3, so undivided).
+// (128 tokens x 2048 x 6144: 7.6 us, against 8.7 undivided; 64 x 2048 x 2048: 5.5 against 4.7, so undivided).
 struct Tiling {
   int tn, split;
 };
@@ -806,12 +806,12 @@ Tiling pick_tiling(int m, int n, int boxes, int epilogue) {
   for (int tn : widths) {
     if (epilogue == kSiluMul && tn % 32) continue;  // a group of gate and up rows stays together
     const int64_t tiles = m_tiles * ((n + tn - 1) / tn);
-    const int64_t box = boxes_per_stage(rows, tn) == 2 ? std::max(200, (rows + tn) * 17 / 20)
+    const int64_t box = boxes_per_stage(rows, tn) == 2 ? std::max(120, (rows + tn) * 41 / 50)
                                                        : std::max(270, (rows + tn) * 9 / 10);
     for (int split = 1; split <= kMaxSplit; split *= 2) {
       if (split > 1 && (2 * split > boxes || tiles * split > max_ctas(split))) break;
       const int64_t cost = split == 1 ? (tiles + sms - 1) / sms * boxes * box
-                                      : (boxes + split - 1) / split * box + 1500 + rows * tn / 6;
+                                      : (boxes + split - 1) / split * box + 1300 + 75 * split + rows * tn / 6;
       if (cost <= best_cost) {
         best = {tn, split};
         best_cost = cost;
