@@ -17,7 +17,9 @@
 //
 // Work split.  The KV of one KV-head group is a flat list of 16-token tiles;
 // CTA c of n streams tiles [T c / n, T (c + 1) / n) across sequence borders, so
-// every CTA moves the same bytes whatever the lengths are.  The tile prefix is
+// every CTA moves the same bytes whatever the lengths are.  Few rows (up to a fifth
+// of the CTAs) are cut one by one into equal parts instead: no CTA then loads a
+// second query or joins twice.  The tile prefix is
 // computed by every CTA from the row lengths (one read and a scan, which costs
 // no more than reading a prefix that a plan kernel left), so the call is one
 // launch.  A row that several CTAs cover leaves fp32 partials in the workspace.
@@ -86,7 +88,8 @@ struct Decode8Args {
   float *part_lse, *part_o;
   int32_t* status;
   int batch, hq, hkv, group, page_size, total_pages, n_ctas;
-  int early;  // NQT_DECODE_OVERLAP_KV_WRITE
+  int early;   // NQT_DECODE_OVERLAP_KV_WRITE
+  int by_row;  // few rows: no CTA's range crosses into another row
   float scale_log2;
   uint64_t wait_ns;
 };
@@ -267,7 +270,7 @@ struct Cfg8 {
   static constexpr int kState = 32 * (D / 4 + 4) * 4;  // a warp's O, m and l
   static constexpr int kJoin = HPC * (kPerHead - 1) * kState;
   static __host__ __device__ constexpr int smem(int rows) {
-    return STAGES * kStage + 1024 + 2 * STAGES * 8 + kJoin + 4 * (2 * (rows + 1)) + (rows + 3) / 4 * 4;
+    return STAGES * kStage + 1024 + 2 * STAGES * 8 + kJoin + 4 * ((rows <= kFewRows8 ? 3 : 2) * (rows + 1)) + (rows + 3) / 4 * 4;
   }
 };
 
@@ -284,7 +287,8 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
   float* s_join = reinterpret_cast<float*>(empty + STAGES);  // [head][warp - 1][O, m, l][lane]
   int32_t* s_prefix = reinterpret_cast<int32_t*>(s_join + Cfg::kJoin / 4);  // [batch + 1] first tile of every row
   int32_t* s_base = s_prefix + p.batch + 1;       // [batch + 1] kv_indptr
-  uint8_t* s_valid = reinterpret_cast<uint8_t*>(s_base + p.batch + 1);  // [batch] tokens of the row's last tile
+  int32_t* s_first = s_base + p.batch + 1;        // [batch + 1] first CTA of every row (by_row)
+  uint8_t* s_valid = reinterpret_cast<uint8_t*>(s_first + (p.by_row ? p.batch + 1 : 0));  // [batch] tokens of the row's last tile
   __shared__ int s_warp_sum[kWarps + 1];
   __shared__ int s_issued;
   __shared__ int s_progress[kWarps];
@@ -299,44 +303,50 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
   const int lane = threadIdx.x & 31;
   const int tpp = p.page_size / kBlock;
 
-  // tile prefix of the batch: exclusive scan of the rows' tile counts
-  int carry = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += Cfg::kThreads) {
-    const int b = b0 + threadIdx.x;
-    int tiles = 0;
-    if (b < p.batch) {
-      const int i0 = p.indptr[b], np = p.indptr[b + 1] - i0;
-      int valid = 0;
-      if (np > 0) {
-        int ll = p.last_len[b];
-        ll = ll < 1 ? 1 : (ll > p.page_size ? p.page_size : ll);
-        tiles = (np - 1) * tpp + (ll + kBlock - 1) / kBlock;
-        valid = ll - (ll - 1) / kBlock * kBlock;
+  // exclusive scan over the batch by the whole CTA; its sum
+  auto scan = [&](auto value, int32_t* prefix) -> int {
+    int carry = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += Cfg::kThreads) {
+      const int b = b0 + threadIdx.x;
+      const int mine = b < p.batch ? value(b) : 0;
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(kFull, incl, o);
+        if (lane >= o) incl += y;
       }
-      s_base[b] = i0;
-      s_valid[b] = static_cast<uint8_t>(valid);
-    }
-    int incl = tiles;
+      if (lane == 31) s_warp_sum[warp] = incl;
+      __syncthreads();
+      int before = carry, sum = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(kFull, incl, o);
-      if (lane >= o) incl += y;
+      for (int w = 0; w < kWarps + 1; ++w) {
+        if (w < warp) before += s_warp_sum[w];
+        sum += s_warp_sum[w];
+      }
+      if (b < p.batch) prefix[b] = before + incl - mine;
+      carry += sum;
+      __syncthreads();
     }
-    if (lane == 31) s_warp_sum[warp] = incl;
-    __syncthreads();
-    int before = carry, sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps + 1; ++w) {
-      if (w < warp) before += s_warp_sum[w];
-      sum += s_warp_sum[w];
-    }
-    if (b < p.batch) s_prefix[b] = before + incl - tiles;
-    carry += sum;
-    __syncthreads();
-  }
-  const int64_t total = carry;
+    if (threadIdx.x == 0) prefix[p.batch] = carry;
+    return carry;
+  };
+  // the rows' first tiles
+  const int64_t total = scan(
+      [&](int b) -> int {
+        const int i0 = p.indptr[b], np = p.indptr[b + 1] - i0;
+        int tiles = 0, valid = 0;
+        if (np > 0) {
+          int ll = p.last_len[b];
+          ll = ll < 1 ? 1 : (ll > p.page_size ? p.page_size : ll);
+          tiles = (np - 1) * tpp + (ll + kBlock - 1) / kBlock;
+          valid = ll - (ll - 1) / kBlock * kBlock;
+        }
+        s_base[b] = i0;
+        s_valid[b] = static_cast<uint8_t>(valid);
+        return tiles;
+      },
+      s_prefix);
   if (threadIdx.x == 0) {
-    s_prefix[p.batch] = carry;
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], HPC);
@@ -355,11 +365,36 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
       p.out[b * p.o_st + static_cast<int64_t>(kv0 * p.group + i / D) * p.o_sh + i % D] = __float2bfloat16_rn(0.f);
   }
   // few tiles: fewer CTAs, so that each has some; every range is non-empty (n <= total)
-  const int64_t want = (total + kMinTiles8 - 1) / kMinTiles8;
-  const int n = want < p.n_ctas ? static_cast<int>(want) : p.n_ctas;
-  if (c >= n) return;  // uniform over the block
-  const int64_t t_begin = first_tile(total, c, n);
-  const int64_t t_end = first_tile(total, c + 1, n);
+  int n, per = 0;
+  int64_t t_begin, t_end;
+  if (p.by_row) {
+    per = static_cast<int>((total + p.n_ctas - p.batch - 1) / (p.n_ctas - p.batch));
+    per = per < kMinTiles8 ? kMinTiles8 : per;
+    n = scan([&](int b) -> int { return (s_prefix[b + 1] - s_prefix[b] + per - 1) / per; }, s_first);
+    __syncthreads();
+    if (c >= n) return;  // uniform over the block
+    const int r = row_of_tile(s_first, p.batch, c);
+    t_begin = s_prefix[r] + static_cast<int64_t>(c - s_first[r]) * per;
+    t_end = t_begin + per < s_prefix[r + 1] ? t_begin + per : s_prefix[r + 1];
+  } else {
+    const int64_t want = (total + kMinTiles8 - 1) / kMinTiles8;
+    n = want < p.n_ctas ? static_cast<int>(want) : p.n_ctas;
+    if (c >= n) return;
+    t_begin = first_tile(total, c, n);
+    t_end = first_tile(total, c + 1, n);
+  }
+  // the CTAs of a row, and whether it starts inside the first one's range
+  auto owners = [&](int row, int& ca, int& cb) -> bool {
+    if (p.by_row) {
+      ca = s_first[row];
+      cb = s_first[row + 1] - 1;
+      return false;
+    }
+    const int64_t t0 = s_prefix[row], t1 = s_prefix[row + 1];
+    ca = tile_owner(total, n, t0);
+    cb = tile_owner(total, n, t1 - 1);
+    return first_tile(total, ca, n) < t0;
+  };
   const int n_tiles = static_cast<int>(t_end - t_begin);
 
   if (warp == kWarps) {
@@ -705,8 +740,8 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
                   __floats2bfloat162_rn(o[ch][1] * v1, o[ch][3] * v1);
           }
         } else {
-          const int ca = tile_owner(total, n, row_t0), cb = tile_owner(total, n, row_t1 - 1);
-          const bool late = first_tile(total, ca, n) < row_t0;
+          int ca, cb;
+          const bool late = owners(row, ca, cb);
           const int slot = part_slot(c, ca, late);
           float* po = p.part_o + (static_cast<int64_t>(slot) * p.hq + ha) * D + 2 * g;
           float* pl = p.part_lse + static_cast<int64_t>(slot) * p.hq + ha;
@@ -748,10 +783,9 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
     for (int f = 0; f < 2; ++f) {
       const int r = f == 0 ? fix_a : fix_b;
       if (r < 0) continue;
-      const int64_t r0 = s_prefix[r], r1 = s_prefix[r + 1];
-      const int ca = tile_owner(total, n, r0), cb = tile_owner(total, n, r1 - 1);
+      int ca, cb;
+      const bool late = owners(r, ca, cb);
       const int lo = c - (c - ca) % kGroup8, hi = min(cb, lo + kGroup8 - 1);
-      const bool late = first_tile(total, ca, n) < r0;
       const int groups = (cb - ca) / kGroup8;  // less one
       join_parts<D, kPerHead>(p, r, kvh, hi - lo + 1, [&](int i) { return part_slot(lo + i, ca, late); }, groups == 0,
                               part_slot(lo, ca, late), sub, lane);
@@ -830,6 +864,7 @@ int launch8(const void* layer, Decode8Args a, cudaStream_t s) {
   int n = num_sms() * occ / groups;
   n = n < 1 ? 1 : (n > kMaxCtas ? kMaxCtas : n);
   a.n_ctas = n;
+  a.by_row = 5 * a.batch <= n && a.batch <= kFewRows8;
   const cudaError_t err = launch_pdl(decode8_kernel<D, HPC, STAGES, E4M3>, dim3(n, groups), dim3(Cfg::kThreads), smem,
                                      s, map, a);
   if (err != cudaSuccess) {
