@@ -17,9 +17,9 @@
 //
 // Work split.  The KV of one KV-head group is a flat list of 16-token tiles;
 // CTA c of n streams tiles [T c / n, T (c + 1) / n) across sequence borders, so
-// every CTA moves the same bytes whatever the lengths are.  Few rows (up to a fifth
-// of the CTAs) are cut one by one into equal parts instead: no CTA then loads a
-// second query or joins twice.  The tile prefix is
+// every CTA moves the same bytes whatever the lengths are.  Where that makes no range
+// much longer the rows are cut one by one instead: no CTA then loads a second query
+// or joins twice.  The tile prefix is
 // computed by every CTA from the row lengths (one read and a scan, which costs
 // no more than reading a prefix that a plan kernel left), so the call is one
 // launch.  A row that several CTAs cover leaves fp32 partials in the workspace.
@@ -89,7 +89,7 @@ struct Decode8Args {
   int32_t* status;
   int batch, hq, hkv, group, page_size, total_pages, n_ctas;
   int early;   // NQT_DECODE_OVERLAP_KV_WRITE
-  int by_row;  // few rows: no CTA's range crosses into another row
+  int by_row;  // few rows: they may be cut one by one
   float scale_log2;
   uint64_t wait_ns;
 };
@@ -365,10 +365,14 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
       p.out[b * p.o_st + static_cast<int64_t>(kv0 * p.group + i / D) * p.o_sh + i % D] = __float2bfloat16_rn(0.f);
   }
   // few tiles: fewer CTAs, so that each has some; every range is non-empty (n <= total)
-  int n, per = 0;
+  int n;
   int64_t t_begin, t_end;
-  if (p.by_row) {
-    per = static_cast<int>((total + p.n_ctas - p.batch - 1) / (p.n_ctas - p.batch));
+  // Rows cut one by one make the longest range up to total / (n - rows) tiles, total * rows / (n (n - rows)) more than a
+  // cut across rows, at some 0.5 us each, and save 3 us.  (One B200, 64 rows: of 33 to 100 tokens 11.9 us against 15.5,
+  // of 333 to 1000 26.9 against 27.5, of 1000 to 3000 57.4 against 52.9.)
+  const bool by_row = p.by_row && total * p.batch <= 5ll * p.n_ctas * (p.n_ctas - p.batch);
+  if (by_row) {
+    int per = static_cast<int>((total + p.n_ctas - p.batch - 1) / (p.n_ctas - p.batch));
     per = per < kMinTiles8 ? kMinTiles8 : per;
     n = scan([&](int b) -> int { return (s_prefix[b + 1] - s_prefix[b] + per - 1) / per; }, s_first);
     __syncthreads();
@@ -385,7 +389,7 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
   }
   // the CTAs of a row, and whether it starts inside the first one's range
   auto owners = [&](int row, int& ca, int& cb) -> bool {
-    if (p.by_row) {
+    if (by_row) {
       ca = s_first[row];
       cb = s_first[row + 1] - 1;
       return false;
@@ -864,7 +868,7 @@ int launch8(const void* layer, Decode8Args a, cudaStream_t s) {
   int n = num_sms() * occ / groups;
   n = n < 1 ? 1 : (n > kMaxCtas ? kMaxCtas : n);
   a.n_ctas = n;
-  a.by_row = 5 * a.batch <= n && a.batch <= kFewRows8;
+  a.by_row = 2 * a.batch <= n && a.batch <= kFewRows8;
   const cudaError_t err = launch_pdl(decode8_kernel<D, HPC, STAGES, E4M3>, dim3(n, groups), dim3(Cfg::kThreads), smem,
                                      s, map, a);
   if (err != cudaSuccess) {

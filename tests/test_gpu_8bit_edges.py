@@ -243,3 +243,19 @@ def test_prefill_more_work_than_the_gpu_holds_at_once(nqt, cuda):
     assert nqt.kernels.read_status(cuda) == 0 and (first[total:] == 7).all()
     want, mag = oc8.attention(q[:total], numbers(codes), scales.double(), indptr, indices, last, qo)
     _close(first[:total], want, mag)
+
+
+@pytest.mark.parametrize(("rows", "lo", "hi"), [(3, 0, 40), (30, 1, 600), (64, 20, 120), (64, 900, 3100), (110, 0, 90),
+                                                (130, 1, 50), (255, 0, 40), (256, 1, 30)])
+def test_decode_rows_cut_one_by_one_or_across(nqt, cuda, rows, lo, hi):
+    """Row counts and lengths on both sides of the rules that decide how the tiles are cut."""
+
+    lens = torch.randint(lo, hi, (rows,), generator=torch.Generator().manual_seed(rows + hi)).tolist()
+    codes, scales, indptr, indices, last = make_cache8(lens, hkv=2, d=64, seed=rows)
+    q = _q(rows, 4, 64, 9)
+    want = oc8.attention(q, numbers(codes), scales.double(), indptr, indices, last)
+    dev = [t.to(cuda) for t in (q, codes, scales, indptr, indices, last)]
+    ws = nqt.decode_paged8_workspace(rows, 4, 64, cuda)
+    first = nqt.batch_decode_paged8(*dev, ws)
+    assert torch.equal(first, nqt.batch_decode_paged8(*dev, ws))
+    _close(first, *want)
