@@ -45,9 +45,9 @@
 //
 // Bound by HBM for large batches and by a chain of dependent trips (row lengths,
 // page ids, TMA, tickets: about 6 us) for small ones.  One B200, captured graphs:
-// 1 row of 300 tokens 9.5 us; 64 rows of 64 to 2048 tokens (16 query and 8 KV
-// heads of 128) 36 us, 144 MB; 240 rows of 32 to 4096 177 us, 6.0 TB/s; five rows
-// of 20001 to 98765 tokens (14 and 2 heads of 64) 30 us, 81 MB.
+// 1 row of 300 tokens 9.0 us; 64 rows of 64 to 2048 tokens (16 query and 8 KV
+// heads of 128) 35 us, 144 MB; 240 rows of 32 to 4096 172 to 177 us, 6.1 TB/s; five
+// rows of 20001 to 98765 tokens (14 and 2 heads of 64) 30 us, 81 MB.
 #include "cache8.cuh"
 
 namespace nqt {
