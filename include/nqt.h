@@ -598,8 +598,10 @@ int nqt_read_paged_cache8(const void* layer_cache, const float* layer_scales, in
  * a plan: the split is computed inside the launch from kv_indptr and
  * last_page_len.  batch <= 8192; rows without pages give zeros.  The workspace
  * (16-byte aligned, nqt_decode8_workspace_bytes) must be zero before its first
- * use and belongs to this entry point: every launch leaves its tickets at zero.
- * One launch at a time per workspace; any shape within its capacity.
+ * use and belongs to this entry point: every launch leaves its tickets, which lie
+ * at the same place for every shape, at zero.  One launch at a time per
+ * workspace; launches of any rows, heads and head sizes may follow one another on
+ * it as long as it holds nqt_decode8_workspace_bytes for each.
  */
 size_t nqt_decode8_workspace_bytes(int batch_capacity, int num_qo_heads, int head_dim);
 int nqt_decode_attention8(

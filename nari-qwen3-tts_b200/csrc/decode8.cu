@@ -55,7 +55,8 @@ namespace {
 
 using namespace c8;
 
-constexpr int kMaxCtas = 1184;     // split CTAs per head group (8 per SM on 148 SMs)
+constexpr int kMaxCtas = 1184;     // split CTAs of all head groups (8 per SM on 148 SMs)
+constexpr int kMaxHpc = 4;         // KV heads of a CTA at most
 constexpr int kMaxRows8 = 8192;    // rows whose prefix a CTA holds in shared memory
 constexpr int kFewRows8 = 255;     // up to here the shared memory is sized alike, so its occupancy is asked for once
 constexpr int kGroup8 = 16;        // CTAs whose parts are joined at once
@@ -63,15 +64,20 @@ constexpr int kMinTiles8 = 4;      // tiles of a CTA at least: shorter parts cos
 
 constexpr size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
+// The workspace: tickets, zero between launches, then the split rows' parts.  A ticket belongs to a part's slot and KV
+// head: those of a row's groups of CTAs to each group's first slot, the row's own to the row's first slot.  A launch has
+// up to kMaxCtas CTAs of up to kMaxHpc KV heads with two slots each, so the tickets take the same bytes whatever the
+// call's rows, heads and head size are, and no call's parts lie where another call's tickets do.
+constexpr size_t kTickets8 = static_cast<size_t>(2) * kMaxCtas * kMaxHpc;
+
 struct Ws8 {
-  // tickets come first, zero between launches: i32 [batch_cap * hq] of the rows, then [2 * kMaxCtas * hq] of groups
-  size_t groups, lse, o, total;
+  size_t groups, lse, o, total;  // the rows' tickets are at 0
 };
 
-constexpr Ws8 ws8_layout(int batch_cap, int hq, int d) {
+constexpr Ws8 ws8_layout(int hq, int d) {
   Ws8 w{};
-  w.groups = up256(4 * static_cast<size_t>(batch_cap) * hq);
-  w.lse = up256(w.groups + 4 * static_cast<size_t>(2 * kMaxCtas) * hq);
+  w.groups = 4 * kTickets8;
+  w.lse = up256(2 * w.groups);
   w.o = up256(w.lse + 4 * static_cast<size_t>(2 * kMaxCtas) * hq);
   w.total = up256(w.o + 4 * static_cast<size_t>(2 * kMaxCtas) * hq * d);
   return w;
@@ -760,8 +766,7 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
           }
           __syncwarp();
           const int lo = c - (c - ca) % kGroup8, hi = min(cb, lo + kGroup8 - 1);  // the CTAs joined with this one
-          if (count_in(p.group_tickets + static_cast<int64_t>(part_slot(lo, ca, late)) * p.hq + kvh, hi - lo,
-                       lane)) {
+          if (count_in(p.group_tickets + part_slot(lo, ca, late) * p.hkv + kvh, hi - lo, lane)) {
             if (fix_a < 0) fix_a = row;  // only a range's first and last rows can be split
             else fix_b = row;
           }
@@ -795,7 +800,7 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
                               part_slot(lo, ca, late), sub, lane);
       if (groups == 0) continue;
       head_sync();
-      int32_t* ticket = p.tickets + static_cast<int64_t>(r) * p.hq + kvh;
+      int32_t* ticket = p.tickets + part_slot(ca, ca, late) * p.hkv + kvh;
       bool whole;
       if (kPerHead > 1) {
         if (sub == 0) {
@@ -866,7 +871,9 @@ int launch8(const void* layer, Decode8Args a, cudaStream_t s) {
   const int occ = a.batch <= kFewRows8 ? few_occ : occupancy(smem);
   const int groups = a.hkv / HPC;
   int n = num_sms() * occ / groups;
-  n = n < 1 ? 1 : (n > kMaxCtas ? kMaxCtas : n);
+  static_assert(HPC <= kMaxHpc, "the tickets' place");
+  n = n > kMaxCtas / groups ? kMaxCtas / groups : n;  // hkv <= 256: at least 4
+  n = n < 1 ? 1 : n;
   a.n_ctas = n;
   a.by_row = 2 * a.batch <= n && a.batch <= kFewRows8;
   const cudaError_t err = launch_pdl(decode8_kernel<D, HPC, STAGES, E4M3>, dim3(n, groups), dim3(Cfg::kThreads), smem,
@@ -893,7 +900,7 @@ using namespace nqt;
 
 extern "C" size_t nqt_decode8_workspace_bytes(int batch_capacity, int num_qo_heads, int head_dim) {
   if (batch_capacity < 1 || num_qo_heads < 1 || head_dim < 1) return 0;
-  return ws8_layout(batch_capacity, num_qo_heads, head_dim).total;
+  return ws8_layout(num_qo_heads, head_dim).total;
 }
 
 extern "C" int nqt_decode_attention8(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
@@ -912,7 +919,7 @@ extern "C" int nqt_decode_attention8(const void* q, int64_t q_stride_tok, int64_
   if ((q_stride_tok & 1) || (q_stride_head & 1) || (out_stride_tok & 1) || (out_stride_head & 1)) return NQT_ERR_ARG;
   if (flags & ~(NQT_DECODE_OVERLAP_KV_WRITE | NQT_DECODE_SHORT_WAIT)) return NQT_ERR_ARG;
   if (batch > kMaxRows8) return NQT_ERR_CAPACITY;
-  const Ws8 w = ws8_layout(batch_capacity, num_qo_heads, head_dim);
+  const Ws8 w = ws8_layout(num_qo_heads, head_dim);
   if (workspace_bytes < w.total) return NQT_ERR_CAPACITY;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return NQT_ERR_ARG;
   if (batch == 0) return NQT_OK;

@@ -191,7 +191,8 @@ def batch_prefill_paged(
 def decode_paged8_workspace(batch_capacity: int, num_qo_heads: int, head_dim: int,
                             device: torch.device) -> torch.Tensor:
     """The zeroed workspace of ``batch_decode_paged8`` for up to ``batch_capacity`` rows: make it once, outside
-    graph capture, and use it for one launch at a time."""
+    graph capture, and use it for one launch at a time.  Calls of other rows, heads and head sizes may take turns on
+    it; one that needs more than it holds is refused."""
 
     nbytes = _lib.lib().nqt_decode8_workspace_bytes(batch_capacity, num_qo_heads, head_dim)
     if nbytes == 0:
