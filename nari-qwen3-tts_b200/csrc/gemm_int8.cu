@@ -53,18 +53,24 @@ using namespace gemm_detail;
 // The rule of a row whose largest |bf16| bits are `mx`: scale, factor and the codes of its values.  A value times the
 // factor plus 1.5 2^23 is the rounded code in the sum's low bits: one rounding, no conversion (1024 x 6144: 5.0 -> 3.8
 // us).
+//
+// The codes are exactly round(x 127 / amax), ties to even, because the factor 127 / amax is rounded up.  Write x and amax
+// as 8-bit integers times powers of two: a quotient q that is no tie is q / (254 255) or more away from one, and the factor
+// moves it by 2^-23 q.  A tie 254 x = (2 j + 1) amax needs 127 to divide 2 j + 1, which is then 127, or amax's integer,
+// and then the factor is a power of two.  So the only tie with an inexact factor is x = amax / 2, 63.5, whose even
+// neighbour 64 is the upper one.
 struct RowRule {
-  float s, f;
-  bool plain;  // else 127 / amax overflows (divide by the subnormal scale), or the row holds an infinity or a NaN
+  float s, f, amax;
+  bool plain;  // else 127 / amax overflows (a division each), or the row holds an infinity or a NaN
   __device__ __forceinline__ explicit RowRule(uint32_t mx) {
-    const float amax = __uint_as_float(mx << 16);
+    amax = __uint_as_float(mx << 16);
     s = __fdiv_rn(amax, 127.f);
-    f = amax == 0.f ? 0.f : __fdiv_rn(127.f, amax);
+    f = amax == 0.f ? 0.f : __fdiv_ru(127.f, amax);
     plain = f <= 3.0e38f && mx < 0x7f80u;
   }
   __device__ __forceinline__ uint32_t odd(uint32_t bf16_bits) const {
     const float v = __uint_as_float(bf16_bits << 16);
-    const float t = f > 3.0e38f ? fminf(fmaxf(__fdiv_rn(v, s), -127.f), 127.f) : v * f;
+    const float t = f > 3.0e38f ? __fdiv_rn(v * 127.f, amax) : v * f;
     return static_cast<uint32_t>(__float2int_rn(t)) & 0xffu;
   }
   __device__ __forceinline__ uint32_t sum(uint32_t f32_bits) const {

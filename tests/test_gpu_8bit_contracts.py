@@ -55,3 +55,45 @@ def test_a_workspace_serves_every_capacity(nqt, cuda):
         out = torch.full_like(want, 7.0)
         nqt.batch_decode_paged8(*case, ws, batch_capacity=capacity, out=out)
         assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------------------------------------ quantiser
+def _tie_rows(exponent):
+    """Rows whose largest value has each mantissa once, with every smaller bf16 down to 2^-10 of it: the ties of
+    x * 127 / amax among them."""
+
+    mantissa = torch.arange(128, 256).double()
+    x = torch.cat([mantissa * 2.0**-e for e in range(11)])
+    rows = torch.where(x[None] <= mantissa[:, None], x[None], 0.0)
+    return torch.cat([rows, -rows], 1) * 2.0**exponent
+
+
+@pytest.mark.parametrize("exponent", [0, -60, 100, -118, -134])
+@pytest.mark.parametrize("odd", [False, True])
+def test_quantize_rows_ties_to_even(nqt, cuda, exponent, odd):
+    """Every code is round(x * 127 / amax), ties to even; the rows of -134 are subnormal numbers."""
+
+    x = _tie_rows(exponent).to(torch.bfloat16)
+    if odd:
+        x = torch.cat([x, x[:, :1] * 0], 1)  # a length that takes the narrow loads
+    exact = x.double() * 127
+    # in 64 bits a tie is exact and nothing else comes near one: 8-bit significands keep quotients 2^-19 apart from it
+    want = (exact / x.double().abs().amax(1, keepdim=True)).round()
+    q, s = nqt.kernels.int8_quantize_rows(x.to(cuda))
+    assert torch.equal(q.cpu().double(), want)
+    top = x.double().abs().amax(1) / 127
+    assert ((s.cpu().double() - top).abs() <= 2.0**-24 * top + 2.0**-150).all()
+
+
+def test_product_of_few_tokens_quantises_ties_alike(nqt, cuda):
+    """The launch for up to 8 tokens quantises by itself: every code it multiplies is the row quantiser's."""
+
+    rows = _tie_rows(0).to(torch.bfloat16)[40:48]
+    x = torch.cat([rows[:, 128:828], rows.amax(1, keepdim=True)], 1)
+    k = x.shape[1]
+    weight = nqt.kernels.Int8Weight.from_quantized(torch.eye(k, dtype=torch.int8, device=cuda), torch.ones(k, device=cuda))
+    amax = x.double().abs().amax(1, keepdim=True)
+    scale = (amax / 127).float().double()
+    want = ((x.double() * 127 / amax).round() * scale).to(torch.float32).to(torch.bfloat16)
+    for m in (1, 2, 3, 8):
+        assert torch.equal(nqt.kernels.linear_int8(x[:m].to(cuda), weight).cpu(), want[:m])
