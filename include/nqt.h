@@ -556,9 +556,11 @@ int nqt_step_finish(const int32_t* row_slot, int rows, int slots, const int64_t*
  * [total_pages, 2, page_size, num_kv_heads, head_dim] (kind 0 = K, 1 = V), and
  * `layer_scales`, contiguous f32 [total_pages, 2, page_size / 16, num_kv_heads]:
  * one scale for every block of 16 tokens of a page, kind and KV head.  An
- * element stands for code * scale; `code` is NQT_I8 or NQT_E4M3.  page_size is a
- * multiple of 16 up to 256, head_dim 64 or 128, num_kv_heads <= 256; the cache
- * is 16-byte aligned.
+ * element stands for code * scale; `code` is NQT_I8 or NQT_E4M3.  The attention
+ * takes value scales below 2^-80 as 2^-80.  A NaN scale of a block, of K or of V,
+ * makes NaN of every query that sees one of its tokens, and of no other.
+ * page_size is a multiple of 16 up to 256, head_dim 64 or 128, num_kv_heads <=
+ * 256; the cache is 16-byte aligned.
  *
  * nqt_qk_norm_rope_paged_cache8: the step's QK RMSNorm + RoPE with the quantised
  * K/V write, the 8-bit counterpart of nqt_qk_norm_rope_paged_kv_write (bf16
@@ -618,7 +620,9 @@ int nqt_decode_attention8(
  * sm_scale >= 0.  q 16-byte aligned with positive strides that are multiples of 8;
  * out any alignment (rows on multiples of 32 or 16 bytes leave faster).  Queries that see no key, and
  * rows without pages, give zeros; tokens behind qo_indptr[batch] are left as
- * they are.  No workspace: when the query tiles do not fill the GPU, clusters
+ * they are.  A NaN code of V (NQT_E4M3) in a chunk may reach the chunk's earlier
+ * queries too: where it is hidden it still meets a weight of zero, as a NaN V does
+ * in nqt_prefill_attention.  No workspace: when the query tiles do not fill the GPU, clusters
  * of CTAs share the keys of one tile and join in shared memory.
  */
 int nqt_prefill_attention8(

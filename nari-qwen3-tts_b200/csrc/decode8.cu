@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(160, 3) decode8_kernel(const __grid_constant__
     // what a tile needs of its scales, per lane of the chunk: score factor, log2 c, 1 / c
     float ks_c, lc_c, rc_c;
     auto take = [&](float ks, float vs) {
-      const float c = fmaxf(vs, 8.271806e-25f);  // 2^-80
+      const float c = vs < 8.271806e-25f ? 8.271806e-25f : vs;  // 2^-80; NaN stays NaN
       ks_c = ks;
       lc_c = log2f(c);
       rc_c = __frcp_rn(c);

@@ -654,11 +654,12 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
             // a group's factors are read before its slot comes round: this warp is at most kRaw + kVStages blocks ahead
             float* f = s_scale + (((group % kScaleRing) * 16 + (lane >> 1)) * 3);
             if (lane & 1) {
-              const float c = fmaxf(sc, 8.271806e-25f);  // 2^-80
+              const float c = sc < 8.271806e-25f ? 8.271806e-25f : sc;  // 2^-80; NaN stays NaN
               f[1] = log2f(c);
               f[2] = __fdiv_rn(1.f, c);
             } else {
-              f[0] = fmaxf(sc * p.scale_log2, 1.17549435e-38f);  // a masked -inf times it stays -inf
+              const float k = sc * p.scale_log2;
+              f[0] = k < 1.17549435e-38f ? 1.17549435e-38f : k;  // a masked -inf times it stays -inf
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sc_full[group % kScaleRing]);
@@ -835,6 +836,13 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (e > last) sr[e] = __float_as_uint(NEG_INF);
+          // a NaN scale is for those who see one of its keys
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+            if (last < g * 16) {
+              fk[g] = 1.f;
+              fe[g] = fv[g] = 0.f;
+            }
         }
         float mx = NEG_INF;
 #pragma unroll

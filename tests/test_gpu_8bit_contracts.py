@@ -97,3 +97,47 @@ def test_product_of_few_tokens_quantises_ties_alike(nqt, cuda):
     want = ((x.double() * 127 / amax).round() * scale).to(torch.float32).to(torch.bfloat16)
     for m in (1, 2, 3, 8):
         assert torch.equal(nqt.kernels.linear_int8(x[:m].to(cuda), weight).cpu(), want[:m])
+
+
+# ------------------------------------------------------------------------------------------------ NaN scales
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("what", [0, 1])
+@pytest.mark.parametrize(("hq", "hkv", "lens"), [(16, 8, [300, 77, 40]), (7, 1, [6000, 33, 1]), (4, 2, [300, 9000])])
+def test_decode_shows_nan_scales(nqt, cuda, kind, what, hq, hkv, lens):
+    """A NaN scale of K (0) or V (1) of a block that row 0 holds makes that row and KV head NaN, and nothing else."""
+
+    codes, scales, indptr, indices, last = make_cache8(lens, kind=kind, hkv=hkv, seed=5)
+    dev = [t.to(cuda) for t in (_q(len(lens), hq, 128, 6), codes, scales, indptr, indices, last)]
+    ws = nqt.decode_paged8_workspace(len(lens), hq, 128, cuda)
+    clean = nqt.batch_decode_paged8(*dev, ws)
+    for block in (0, 7, (lens[0] - 1) // 16):
+        bad = scales.clone()
+        bad[int(indices[block]), what, 0, hkv - 1] = float("nan")
+        out = nqt.batch_decode_paged8(dev[0], dev[1], bad.to(cuda), *dev[3:], ws)
+        first = hq - hq // hkv
+        assert out[0, first:].isnan().all()
+        assert torch.equal(out[0, :first], clean[0, :first]) and torch.equal(out[1:], clean[1:])
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("what", [0, 1])
+@pytest.mark.parametrize(("hq", "hkv", "copies"), [(16, 8, 30), (2, 1, 1), (7, 1, 1)])
+def test_prefill_shows_nan_scales_to_those_who_see_them(nqt, cuda, kind, what, hq, hkv, copies):
+    """A block with a NaN scale makes the queries NaN that see one of its keys; the others keep every bit.  Many rows
+    and few: with and without keys shared by a cluster."""
+
+    lens, chunks = [300] * copies, [200] * copies
+    codes, scales, indptr, indices, last = make_cache8(lens, kind=kind, hkv=hkv, d=64, seed=7)
+    qo = (200 * torch.arange(copies + 1)).to(torch.int32)
+    q = _q(200 * copies, hq, 64, 8)
+    dev = [t.to(cuda) for t in (q, codes, scales, qo, indptr, indices, last)]
+    clean = nqt.batch_prefill_paged8(*dev)
+    first = hq - hq // hkv
+    for block in (0, 6, 9, 10, 18):
+        bad = scales.clone()
+        bad[int(indices[block]), what, 0, hkv - 1] = float("nan")
+        out = nqt.batch_prefill_paged8(dev[0], dev[1], bad.to(cuda), *dev[3:])
+        seen = max(0, 16 * block - 100)  # the first query that sees the block
+        assert out[seen:200, first:].isnan().all()
+        assert torch.equal(out[:seen], clean[:seen]) and torch.equal(out[200:], clean[200:])
+        assert torch.equal(out[:, :first], clean[:, :first])
