@@ -176,12 +176,14 @@ __device__ __forceinline__ bool count_in(int32_t* ticket, int others, int lane) 
     arrived = atomic_inc_acq_rel(ticket);
     if (arrived == others) *ticket = 0;
   }
-  return __shfl_sync(kFull, arrived, 0) == others;
+  const bool last = __shfl_sync(kFull, arrived, 0) == others;
+  __syncwarp();  // what lane 0 acquired is there for all
+  return last;
 }
 
 // Joins `count` parts of one row and KV head: sum_i 2^(lse_i - M) O_i / sum_i 2^(lse_i - M) for every query head of
 // the group, by WARPS warps of which this is number `sub`.  slot(i): the slot of part i.  Goes to `out` (last) or to slot
-// `dst` as a part.  The loads of two sets of heads and eight parts are in flight at once: a join is a chain of trips to
+// `dst`, which may be slot(0), as a part.  The loads of two sets of heads and eight parts are in flight at once: a join is a chain of trips to
 // L2.
 template <int D, int WARPS, typename Slot>
 __device__ __forceinline__ void join_parts(const Decode8Args& p, int row, int kvh, int count, Slot slot, bool last,
@@ -245,6 +247,7 @@ __device__ __forceinline__ void join_parts(const Decode8Args& p, int row, int kv
         }
       }
     }
+    __syncwarp();  // slot `dst` may be one of the parts, and another lane may still be reading its log2-sum-exp
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if (!live[u]) continue;
