@@ -649,8 +649,10 @@ int nqt_prefill_attention8(
  * Any m, n >= 1 and 1 <= k <= 131072; xq and w 16-byte aligned with row pitches
  * (bytes) that are multiples of 16; y any row pitch.  No workspace.
  *
- * nqt_linear_int8: both for bf16 x, with xq [m, ldxq] and xscale [m] as scratch
- * (up to 8 rows one launch that does not use them, else two).
+ * nqt_linear_int8: both for bf16 x.  Where nqt_linear_int8_launches(m, k) is 1
+ * (up to 8 rows of a k that their launch can hold) xq and xscale are not used and
+ * may be null; where it is 2, xq [m, ldxq] and xscale [m] are written as scratch.
+ * It is 0 for m or k below 1.
  * All are launched with programmatic stream serialization.
  */
 int nqt_int8_quantize_rows(const void* x, int64_t ldx, int m, int k, void* q, int64_t ldq, float* scale,
@@ -658,6 +660,7 @@ int nqt_int8_quantize_rows(const void* x, int64_t ldx, int m, int k, void* q, in
 int nqt_gemm_int8(const void* xq, int64_t ldxq, const float* xscale, const void* w, int64_t ldw, const float* wscale,
                   const void* bias, void* y, int64_t ldy, int m, int n, int cols, int k, int epilogue,
                   int32_t* status, void* stream);
+int nqt_linear_int8_launches(int m, int k);
 int nqt_linear_int8(const void* x, int64_t ldx, void* xq, int64_t ldxq, float* xscale, const void* w, int64_t ldw,
                     const float* wscale, const void* bias, void* y, int64_t ldy, int m, int n, int cols, int k,
                     int epilogue, int32_t* status, void* stream);

@@ -125,6 +125,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "nqt_int8_quantize_rows": (I, [P, L, I, I, P, L, P, P]),
     "nqt_gemm_int8": (I, [P, L, P, P, L, P, P, P, L, I, I, I, I, I, P, P]),
+    "nqt_linear_int8_launches": (I, [I, I]),
     "nqt_linear_int8": (I, [P, L, P, L, P, P, L, P, P, P, L, I, I, I, I, I, P, P]),
     "nqt_step_stage": (I, [P, I, I, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P]),
     "nqt_talker_logits_mask": (I, [P, I, L, I, I, I, I, P, P]),
@@ -175,7 +176,7 @@ def lib() -> ctypes.CDLL:
 
 # entry points that the C++ binding (csrc/bind.cpp) calls, in its order
 _BOUND = ("nqt_decode_attention8", "nqt_prefill_attention8", "nqt_qk_norm_rope_paged_cache8", "nqt_read_paged_cache8",
-          "nqt_gemm_int8", "nqt_linear_int8")
+          "nqt_gemm_int8", "nqt_linear_int8", "nqt_linear_int8_launches")
 _bind = None
 
 
@@ -221,7 +222,6 @@ def exported_symbols() -> list[str]:
 # kernels each entry point launches (nqt_plan_step adds the split-KV plan when given a workspace)
 KERNELS_PER_CALL = {
     "nqt_decode_attention_noalloc": 2,
-    "nqt_linear_int8": 2,
 }
 _launches = 0
 

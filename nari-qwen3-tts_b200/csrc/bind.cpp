@@ -30,6 +30,8 @@ decltype(&nqt_qk_norm_rope_paged_cache8) f_write8;
 decltype(&nqt_read_paged_cache8) f_read8;
 decltype(&nqt_gemm_int8) f_gemm_int8;
 decltype(&nqt_linear_int8) f_linear_int8;
+decltype(&nqt_linear_int8_launches) f_linear_int8_launches;
+constexpr int kEntryPoints = 7;
 
 int32_t* g_status[kMaxDevices];
 long long g_launches;
@@ -329,11 +331,16 @@ PyObject* linear8(PyObject* const* a) {
                          static_cast<int>(cols), static_cast<int>(k), epilogue, status, stream);
     }), *out);
   const int64_t pitch = (k + 15) / 16 * 16;
-  const at::Tensor scratch = at::empty({m * (pitch + 4)}, x.options().dtype(at::kByte));
-  uint8_t* q = static_cast<uint8_t*>(scratch.data_ptr());
+  const bool quantises = f_linear_int8_launches(static_cast<int>(m), static_cast<int>(k)) == 2;
+  at::Tensor scratch;
+  uint8_t* q = nullptr;
+  if (quantises) {
+    scratch = at::empty({m * (pitch + 4)}, x.options().dtype(at::kByte));
+    q = static_cast<uint8_t*>(scratch.data_ptr());
+  }
   return result(on_device(dev, [&](int32_t* status, void* stream) {
-    if (m > 8) ++g_launches;  // the quantiser's
-    return f_linear_int8(x.const_data_ptr(), pitch_of(x), q, pitch, reinterpret_cast<float*>(q + m * pitch),
+    if (quantises) ++g_launches;
+    return f_linear_int8(x.const_data_ptr(), pitch_of(x), q, pitch, quantises ? reinterpret_cast<float*>(q + m * pitch) : nullptr,
                          w.const_data_ptr(), pitch_of(w), ws.const_data_ptr<float>(), b, out->data_ptr(), pitch_of(*out),
                          static_cast<int>(m), rows, static_cast<int>(cols), static_cast<int>(k), epilogue, status, stream);
   }), *out);
@@ -357,12 +364,12 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // init(addresses of the entry points, in the order below)
 PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 6) {
-    PyErr_SetString(PyExc_TypeError, "init takes six addresses");
+  if (n != kEntryPoints) {
+    PyErr_SetString(PyExc_TypeError, "init takes the entry points' addresses");
     return nullptr;
   }
-  void* p[6];
-  for (int i = 0; i < 6; ++i) {
+  void* p[kEntryPoints];
+  for (int i = 0; i < kEntryPoints; ++i) {
     p[i] = PyLong_AsVoidPtr(args[i]);
     if (p[i] == nullptr) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null entry point");
@@ -375,6 +382,7 @@ PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
   f_read8 = reinterpret_cast<decltype(f_read8)>(p[3]);
   f_gemm_int8 = reinterpret_cast<decltype(f_gemm_int8)>(p[4]);
   f_linear_int8 = reinterpret_cast<decltype(f_linear_int8)>(p[5]);
+  f_linear_int8_launches = reinterpret_cast<decltype(f_linear_int8_launches)>(p[6]);
   Py_RETURN_NONE;
 }
 

@@ -871,14 +871,16 @@ int launch_i8(const void* xq, int64_t ldxq, const void* w, int64_t ldw, int k, I
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-int check_gemm(const void* xq, int64_t ldxq, const float* xscale, const void* w, int64_t ldw, const float* wscale,
-               const void* bias, const void* y, int64_t ldy, int m, int n, int cols, int k, int epilogue) {
+// `codes`: whether the call reads (or writes and reads) xq and xscale.
+int check_gemm(bool codes, const void* xq, int64_t ldxq, const float* xscale, const void* w, int64_t ldw,
+               const float* wscale, const void* bias, const void* y, int64_t ldy, int m, int n, int cols, int k,
+               int epilogue) {
   if (!w || !wscale || !y || m < 0 || n < 1 || k < 1 || cols < 1) return NQT_ERR_ARG;
   if (epilogue != kPlain && epilogue != kBias && epilogue != kSiluMul) return NQT_ERR_ARG;
   if (epilogue == kBias && !bias) return NQT_ERR_ARG;
   if (epilogue == kSiluMul ? (n % 32 != 0 || cols > n / 2) : cols != n) return NQT_ERR_ARG;
   if (k > 131072) return NQT_ERR_UNSUPPORTED;  // the int32 sums could overflow
-  if (!xq || !xscale || !aligned(xq, 16) || ldxq % 16 || ldxq < k) return NQT_ERR_ARG;
+  if (codes && (!xq || !xscale || !aligned(xq, 16) || ldxq % 16 || ldxq < k)) return NQT_ERR_ARG;
   if (!aligned(w, 16) || ldw % 16 || ldw < k || ldy < cols || !aligned(y, 2)) return NQT_ERR_ARG;
   return NQT_OK;
 }
@@ -963,7 +965,7 @@ extern "C" int nqt_int8_quantize_rows(const void* x, int64_t ldx, int m, int k, 
 extern "C" int nqt_gemm_int8(const void* xq, int64_t ldxq, const float* xscale, const void* w, int64_t ldw,
                              const float* wscale, const void* bias, void* y, int64_t ldy, int m, int n, int cols,
                              int k, int epilogue, int32_t* status, void* stream) {
-  const int rc = check_gemm(xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue);
+  const int rc = check_gemm(true, xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue);
   if (rc != NQT_OK) return rc;
   if (m == 0) return NQT_OK;
   if (takes_gemv(m, k))
@@ -973,10 +975,13 @@ extern "C" int nqt_gemm_int8(const void* xq, int64_t ldxq, const float* xscale, 
                   as_stream(stream));
 }
 
+extern "C" int nqt_linear_int8_launches(int m, int k) { return m < 1 || k < 1 ? 0 : (takes_gemv(m, k) ? 1 : 2); }
+
 extern "C" int nqt_linear_int8(const void* x, int64_t ldx, void* xq, int64_t ldxq, float* xscale, const void* w,
                                int64_t ldw, const float* wscale, const void* bias, void* y, int64_t ldy, int m, int n,
                                int cols, int k, int epilogue, int32_t* status, void* stream) {
-  const int rc = check_gemm(xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n, cols, k, epilogue);
+  const int rc = check_gemm(nqt_linear_int8_launches(m, k) == 2, xq, ldxq, xscale, w, ldw, wscale, bias, y, ldy, m, n,
+                            cols, k, epilogue);
   if (rc != NQT_OK) return rc;
   if (!x || ldx < k || !aligned(x, 2)) return NQT_ERR_ARG;
   if (m == 0) return NQT_OK;

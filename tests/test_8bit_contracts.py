@@ -1,0 +1,37 @@
+"""CPU: contracts of the 8-bit operators that need no launch: scratch and launches of the integer projection, sizes that
+32-bit indices cannot hold, calls without rows, and when the C++ binding is compiled again."""
+
+from __future__ import annotations
+
+import importlib
+import math
+
+import pytest
+
+ARG = -1
+A = 1 << 20  # an aligned address that is never read: every call here is refused first
+
+
+def _lib():
+    return importlib.import_module("nari-qwen3-tts_b200._lib").lib()
+
+
+def test_linear_launches():
+    """One launch for up to 8 tokens whose codes, in 1, 2, 4 or 8 rows of k rounded up to 16, fit 96 KB."""
+
+    f = _lib().nqt_linear_int8_launches
+    for m in range(1, 20):
+        slots = next((s for s in (1, 2, 4, 8) if s >= m), None)
+        for k in (1, 16, 2048, 12288, 12289, 24576, 24577, 49152, 49153, 98304, 98305, 131072):
+            one = slots is not None and slots * math.ceil(k / 16) * 16 <= 96 * 1024
+            assert f(m, k) == (1 if one else 2)
+    assert f(0, 64) == 0
+
+
+@pytest.mark.parametrize(("m", "k"), [(9, 64), (64, 2048), (8, 12304), (3, 24592), (1, 98320)])
+def test_linear_refuses_missing_scratch_where_it_is_used(m, k):
+    def call(xq, ldxq, xscale):
+        return _lib().nqt_linear_int8(A, k, xq, ldxq, xscale, A, k, A, None, A, 4, m, 4, 4, k, 0, A, None)
+
+    for args in ((None, k, A), (A, k, None), (A + 8, k, A), (A, k - 16, A), (A, k + 8, A)):
+        assert call(*args) == ARG

@@ -141,3 +141,28 @@ def test_prefill_shows_nan_scales_to_those_who_see_them(nqt, cuda, kind, what, h
         assert out[seen:200, first:].isnan().all()
         assert torch.equal(out[:seen], clean[:seen]) and torch.equal(out[200:], clean[200:])
         assert torch.equal(out[:, :first], clean[:, :first])
+
+
+# ------------------------------------------------------------------------------------------------ launches and scratch
+def test_linear_launches_as_it_says(nqt, cuda):
+    """One launch or two by nqt_linear_int8_launches, in the count of launches too; one needs no scratch."""
+
+    lib = nqt._lib.lib()
+    for m, k in ((1, 64), (8, 2048), (8, 12288), (8, 12304), (5, 16384), (4, 24592), (3, 24576), (9, 64), (64, 2048)):
+        g = torch.Generator().manual_seed(m + k)
+        x = torch.randn(m, k, generator=g).to(torch.bfloat16).to(cuda)
+        weight = nqt.kernels.Int8Weight(torch.randn(48, k, generator=g).to(torch.bfloat16).to(cuda))
+        codes, scale = nqt.kernels.int8_quantize_rows(x)
+        nqt._lib.reset_launch_count()
+        y = nqt.kernels.linear_int8(x, weight)
+        assert nqt._lib.launch_count() == lib.nqt_linear_int8_launches(m, k)
+        assert torch.equal(y, nqt.kernels.linear_int8(codes, weight, xscale=scale))
+        pitch = (k + 15) // 16 * 16
+        out = torch.empty_like(y)
+        scratch = torch.full((m * (pitch + 4),), 7, dtype=torch.uint8, device=cuda)
+        one = lib.nqt_linear_int8_launches(m, k) == 1
+        nqt._lib.call("nqt_linear_int8", x.data_ptr(), k, None if one else scratch.data_ptr(), pitch,
+                      None if one else scratch.data_ptr() + m * pitch, weight.data.data_ptr(), weight.data.stride(0),
+                      weight.data_scale.data_ptr(), None, out.data_ptr(), 48, m, 48, 48, k, 0,
+                      nqt.kernels.device_status(cuda).data_ptr(), nqt._lib.stream_handle(cuda))
+        assert torch.equal(out, y)
