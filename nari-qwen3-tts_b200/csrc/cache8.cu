@@ -139,7 +139,8 @@ __device__ __forceinline__ void store_half(__nv_bfloat16* p, int vec, const floa
   }
 }
 
-// Codes of x times 1 / s, E in a row at r.
+// Codes of x / s, E in a row at r, as x times the rounded 1 / s: within 2^-23 of the quotient, relative, so a code is not
+// the quotient's only where that lies within 2^-16 steps of the middle between two codes.
 template <int D, bool E4M3>
 __device__ __forceinline__ void store_codes(uint8_t* r, const float (&x)[D / 16], float s, float inv) {
   constexpr int E = D / 16;
@@ -149,8 +150,11 @@ __device__ __forceinline__ void store_codes(uint8_t* r, const float (&x)[D / 16]
     float v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      // 1 / s overflows for subnormal scales only; s = 0 stands for a block of zeros
-      v[j] = inv <= FLT_MAX ? x[4 * i + j] * inv : (s > 0.f ? __fdiv_rn(x[4 * i + j], s) : 0.f);
+      // 1 / s overflows for subnormal scales only; s = 0 stands for a block of zeros (and of what is NaN: 0 x)
+      v[j] = x[4 * i + j] * (inv <= FLT_MAX ? inv : 0.f);
+    if (inv > FLT_MAX && s > 0.f)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __fdiv_rn(x[4 * i + j], s);
     w[i] = codes_of_pair<E4M3>(v[0], v[1]) | static_cast<uint32_t>(codes_of_pair<E4M3>(v[2], v[3])) << 16;
   }
   if constexpr (E == 8) *reinterpret_cast<uint2*>(r) = make_uint2(w[0], w[E / 4 - 1]);

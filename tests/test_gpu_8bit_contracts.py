@@ -6,9 +6,12 @@ from __future__ import annotations
 import pytest
 import torch
 
+from oracle import cache8 as oc8
 from tests._cache8 import make_cache8
 
 pytestmark = pytest.mark.gpu
+
+EPS, THETA = 1e-6, 1.0e6
 
 
 def _q(rows, hq, d, seed):
@@ -166,3 +169,40 @@ def test_linear_launches_as_it_says(nqt, cuda):
                       weight.data_scale.data_ptr(), None, out.data_ptr(), 48, m, 48, 48, k, 0,
                       nqt.kernels.device_status(cuda).data_ptr(), nqt._lib.stream_handle(cuda))
         assert torch.equal(out, y)
+
+
+# ------------------------------------------------------------------------------------------------ special values
+def _write_one(nqt, cuda, dc, ds, k, v, offset, hq=2):
+    d = k.shape[-1]
+    w = torch.ones(d, dtype=torch.bfloat16, device=cuda)
+    q = torch.zeros(len(k), hq, d, dtype=torch.bfloat16, device=cuda)
+    at = (torch.arange(len(k)) + offset).to(cuda)
+    nqt.paired_qk_norm_rope_paged_cache8(q, k.to(cuda), v.to(cuda), w, w, at, EPS, THETA, dc, ds, torch.zeros_like(at), at)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_write_nan_tokens(nqt, cuda, kind, d):
+    """A NaN is code 0 (int8) or the NaN code (e4m3), also where the block holds nothing else: a NaN key element makes
+    its whole row NaN, so the first token of a block leaves the scale 0."""
+
+    def expect(row, nan):
+        raw = row.view(torch.uint8).flatten()
+        return ((raw & 0x7F) == 0x7F).all() if nan and kind == "e4m3" else (raw & 0x7F == 0).all()
+
+    ones = torch.ones(1, 1, d, dtype=torch.bfloat16)
+    dc = torch.full((1, 2, 16, 1, d), 3).to(oc8.DTYPE[kind]).to(cuda)
+    ds = torch.ones(1, 2, 1, 1, device=cuda)
+    bad = ones.clone()
+    bad[0, 0, 5] = float("nan")
+    _write_one(nqt, cuda, dc, ds, bad, ones * float("nan"), 0)
+    assert (ds == 0).all() and expect(dc[0, 0, 0, 0], True) and expect(dc[0, 1, 0, 0], True)
+    # a later token sets the scale; what was NaN stays so
+    _write_one(nqt, cuda, dc, ds, ones, 2 * ones, 1)
+    assert (ds > 0).all() and expect(dc[0, 0, 0, 0], True) and expect(dc[0, 1, 0, 0], True)
+    back = nqt.read_paged_cache8(dc, ds, torch.tensor([0], device=cuda))
+    assert (back[0, 1, 1, 0] == 2).all() and back[0, 0, 1].isfinite().all()
+    # and a row of zeros beside a NaN row
+    _write_one(nqt, cuda, dc, ds, torch.cat([0 * ones, bad]), torch.cat([0 * ones, bad * 0]), 0)
+    assert (ds == 0).all() and expect(dc[0, 0, 0, 0], False) and expect(dc[0, 0, 1, 0], True)
+    assert expect(dc[0, 1, 0, 0], False) and expect(dc[0, 1, 1, 0, 5:6], True) and expect(dc[0, 1, 1, 0, :5], False)
