@@ -573,9 +573,12 @@ int nqt_step_finish(const int32_t* row_slot, int rows, int slots, const int64_t*
  * need), and then the codes at lower offsets are rounded again to code * s / s'.
  * Codes behind the group are left as they are.  A call's tokens of one block
  * must form one group: two groups of one block in a call race on its scale.
- * Infinities count as the largest finite number, NaN becomes code 0 (NQT_I8) or
- * the NaN code (NQT_E4M3).  A page or offset outside the pool sets
- * NQT_DEV_BAD_PAGE and writes nothing.
+ * NaN becomes code 0 (NQT_I8) or the NaN code (NQT_E4M3) and does not count for
+ * the scale.  An infinite element of V counts as the largest finite number.  One
+ * of K makes the row's RMS infinite: it and its partner in the rotation become NaN,
+ * the rest of that key 0.  A NaN element of K makes the whole key NaN.  q fares as
+ * K does, in bf16.  A page or offset outside the pool sets NQT_DEV_BAD_PAGE and
+ * writes nothing.
  *
  * nqt_read_paged_cache8: pages i64 [count] of a layer as bf16
  * [count, 2, page_size, num_kv_heads, head_dim] (out 16-byte aligned, contiguous).

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import cache8 as oc8
-from tests._cache8 import make_cache8
+from tests._cache8 import make_cache8, numbers
 
 pytestmark = pytest.mark.gpu
 
@@ -206,3 +206,41 @@ def test_write_nan_tokens(nqt, cuda, kind, d):
     _write_one(nqt, cuda, dc, ds, torch.cat([0 * ones, bad]), torch.cat([0 * ones, bad * 0]), 0)
     assert (ds == 0).all() and expect(dc[0, 0, 0, 0], False) and expect(dc[0, 0, 1, 0], True)
     assert expect(dc[0, 1, 0, 0], False) and expect(dc[0, 1, 1, 0, 5:6], True) and expect(dc[0, 1, 1, 0, :5], False)
+
+
+# ------------------------------------------------------------------------------------------------ infinities
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_write_infinite_keys_and_values(nqt, cuda, kind):
+    """An infinite V is the largest code.  An infinite element of K makes the row's RMS infinite: it and its partner in
+    the rotation become NaN, the row's other elements zero; other tokens of the block are not touched."""
+
+    d, top = 128, oc8.TOP[kind]
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(4, 1, d, generator=g).to(torch.bfloat16) for _ in range(2))
+    pair = torch.zeros(d, dtype=torch.bool)
+    pair[[6, 70]] = True
+    dc = [torch.zeros(1, 2, 16, 1, d, dtype=oc8.DTYPE[kind], device=cuda) for _ in range(2)]
+    ds = [torch.zeros(1, 2, 1, 1, device=cuda) for _ in range(2)]
+    k2 = k.clone()
+    k2[2, 0, 70] = float("inf")
+    _write_one(nqt, cuda, dc[0], ds[0], k2, v, 0)
+    got = dc[0][0, 0, 2, 0].cpu()
+    raw = got.view(torch.uint8) & 0x7F
+    assert (raw[~pair] == 0).all() and (raw[pair] == (0 if kind == "int8" else 0x7F)).all()
+    k2[2] = 0  # contributes nothing to the block's scale, as the infinite row does
+    _write_one(nqt, cuda, dc[1], ds[1], k2, v, 0)
+    others = torch.tensor([0, 1, 3])
+    assert torch.equal(ds[0], ds[1])
+    assert torch.equal(dc[0][0, 0].view(torch.uint8)[others.to(cuda)], dc[1][0, 0].view(torch.uint8)[others.to(cuda)])
+    v[1, 0, 9], v[1, 0, 10] = float("inf"), -float("inf")
+    _write_one(nqt, cuda, dc[0], ds[0], k, v, 0)
+    assert numbers(dc[0].cpu())[0, 1, 1, 0, 9:11].tolist() == [top, -top] and ds[0].isfinite().all()
+    # a query fares as a key does, in bf16
+    q, w = torch.ones(4, 2, d, dtype=torch.bfloat16), torch.ones(d, dtype=torch.bfloat16)
+    q[2, 1, 70] = float("inf")
+    at = torch.arange(4)
+    rot = nqt.paired_qk_norm_rope_paged_cache8(*(t.to(cuda) for t in (q, k, v, w, w, at)), EPS, THETA, dc[0], ds[0],
+                                               torch.zeros_like(at).to(cuda), at.to(cuda)).cpu()
+    assert rot[2, 1, pair].isnan().all() and (rot[2, 1, ~pair] == 0).all()
+    rot[2, 1] = 1
+    assert rot.isfinite().all()
