@@ -956,9 +956,9 @@ using namespace nqt;
 
 extern "C" int nqt_int8_quantize_rows(const void* x, int64_t ldx, int m, int k, void* q, int64_t ldq, float* scale,
                                       void* stream) {
-  if (!x || !q || !scale || m < 0 || k < 1 || ldx < k || ldq < k || !aligned(x, 2) || !aligned(scale, 4))
-    return NQT_ERR_ARG;
-  if (m == 0) return NQT_OK;
+  if (m < 0 || k < 1 || ldx < k || ldq < k) return NQT_ERR_ARG;
+  if (m == 0) return NQT_OK;  // tensors without elements have no address
+  if (!x || !q || !scale || !aligned(x, 2) || !aligned(scale, 4)) return NQT_ERR_ARG;
   return run_quantize(x, ldx, m, k, q, ldq, scale, as_stream(stream));
 }
 

@@ -35,3 +35,9 @@ def test_linear_refuses_missing_scratch_where_it_is_used(m, k):
 
     for args in ((None, k, A), (A, k, None), (A + 8, k, A), (A, k - 16, A), (A, k + 8, A)):
         assert call(*args) == ARG
+
+
+def test_quantize_no_rows():
+    assert _lib().nqt_int8_quantize_rows(None, 8, 0, 8, None, 16, None, None) == 0
+    assert _lib().nqt_int8_quantize_rows(None, 8, -1, 8, None, 16, None, None) == ARG
+    assert _lib().nqt_int8_quantize_rows(None, 8, 0, 0, None, 16, None, None) == ARG

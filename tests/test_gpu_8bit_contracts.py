@@ -244,3 +244,9 @@ def test_write_infinite_keys_and_values(nqt, cuda, kind):
     assert rot[2, 1, pair].isnan().all() and (rot[2, 1, ~pair] == 0).all()
     rot[2, 1] = 1
     assert rot.isfinite().all()
+
+
+# ------------------------------------------------------------------------------------------------ empty rows
+def test_quantize_no_rows(nqt, cuda):
+    q, s = nqt.kernels.int8_quantize_rows(torch.zeros(0, 40, dtype=torch.bfloat16, device=cuda))
+    assert q.shape == (0, 40) and s.shape == (0,)
