@@ -279,7 +279,7 @@ PyObject* read8(PyObject* const* a) {
 
 // Row stride of a matrix in elements; a single row's stride says nothing.
 int64_t pitch_of(const at::Tensor& t) {
-  return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), (t.size(1) + 15) / 16 * 16);
+  return t.size(0) > 1 ? t.stride(0) : (t.size(1) + 15) / 16 * 16;
 }
 
 // (x, data, data_scale, k, cols, gate_up, bias, xscale, out): data int8 [rows, >= k] as Int8Weight lays it out

@@ -678,7 +678,7 @@ def int8_quantize_rows(x: torch.Tensor, *, out: torch.Tensor | None = None,
 def _row_pitch(t: torch.Tensor) -> int:
     """Row stride of a matrix in elements; a single row's stride says nothing."""
 
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), (t.shape[1] + 15) // 16 * 16)
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
 class Int8Weight:

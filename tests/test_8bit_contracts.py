@@ -7,6 +7,7 @@ import importlib
 import math
 
 import pytest
+import torch
 
 ARG = -1
 A = 1 << 20  # an aligned address that is never read: every call here is refused first
@@ -41,3 +42,17 @@ def test_quantize_no_rows():
     assert _lib().nqt_int8_quantize_rows(None, 8, 0, 8, None, 16, None, None) == 0
     assert _lib().nqt_int8_quantize_rows(None, 8, -1, 8, None, 16, None, None) == ARG
     assert _lib().nqt_int8_quantize_rows(None, 8, 0, 0, None, 16, None, None) == ARG
+
+
+def test_one_row_of_codes_with_any_pitch(nqt):
+    """Only the missing GPU stops a single row of codes whose stride is odd."""
+
+    weight = nqt.kernels.Int8Weight.__new__(nqt.kernels.Int8Weight)
+    weight._lay_out(torch.zeros(6, 33, dtype=torch.int8), torch.ones(6), False)
+    base = torch.zeros(4, 101, dtype=torch.int8)
+    with pytest.raises(ValueError, match="CUDA"):
+        nqt.kernels.linear_int8(base[:1, :33], weight, xscale=torch.ones(1))
+    with pytest.raises(ValueError, match="16-byte"):
+        nqt.kernels.linear_int8(base[:2, :33], weight, xscale=torch.ones(2))
+    with pytest.raises(ValueError, match="16-byte"):
+        nqt.kernels.linear_int8(base[1:2, :33], weight, xscale=torch.ones(1))

@@ -250,3 +250,18 @@ def test_write_infinite_keys_and_values(nqt, cuda, kind):
 def test_quantize_no_rows(nqt, cuda):
     q, s = nqt.kernels.int8_quantize_rows(torch.zeros(0, 40, dtype=torch.bfloat16, device=cuda))
     assert q.shape == (0, 40) and s.shape == (0,)
+
+
+# ------------------------------------------------------------------------------------------------ single rows
+def test_one_row_of_codes_with_any_pitch(nqt, cuda):
+    """The pitch of a single row says nothing: a row cut out of a matrix of odd width is taken."""
+
+    g = torch.Generator().manual_seed(4)
+    base = torch.randint(-127, 128, (16, 101), generator=g, dtype=torch.int8)
+    weight = nqt.kernels.Int8Weight.from_quantized(torch.randint(-127, 128, (20, 33), generator=g, dtype=torch.int8).to(cuda),
+                                                   torch.ones(20, device=cuda))
+    xs = torch.ones(1, device=cuda)
+    x = base.to(cuda)[:1, :33]
+    assert x.stride(0) == 101
+    want = (base[0, :33].double() @ weight.q.cpu().double().t()).to(torch.float32).to(torch.bfloat16)
+    assert torch.equal(nqt.kernels.linear_int8(x, weight, xscale=xs).cpu()[0], want)
