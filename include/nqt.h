@@ -641,7 +641,7 @@ int nqt_prefill_attention8(
  * W8A8 integer projection.  nqt_int8_quantize_rows: per row of bf16 x [m, k],
  * scale = amax / 127 and q = round(x * 127 / amax) (a row of zeros has scale 0; a
  * NaN or an infinity makes the row's scale NaN or infinite).  It serves tokens
- * and, over a weight [n, k], output channels.  Any alignment and any k.
+ * and, over a weight [n, k], output channels.  Any alignment, k <= 2^31 - 8.
  *
  * nqt_gemm_int8: y[t, j] = (xq[t] . w[j]) * xscale[t] * wscale[j], int32 sums:
  *   epilogue 0  y = bf16(.)          [m, cols], cols == n
@@ -649,8 +649,9 @@ int nqt_prefill_attention8(
  *   epilogue 2  w's rows in groups [16 gate | 16 up] (n a multiple of 32):
  *               y[t, 16 g + i] = bf16(silu(gate) * up), the first cols <= n / 2
  *               columns of it.
- * Any m, n >= 1 and 1 <= k <= 131072; xq and w 16-byte aligned with row pitches
- * (bytes) that are multiples of 16; y any row pitch.  No workspace.
+ * Any m <= 2^31 - 128, 1 <= n <= 2^31 - 256 and 1 <= k <= 131072; xq and w 16-byte
+ * aligned with row pitches (bytes) that are multiples of 16; y any row pitch.  No
+ * workspace.
  *
  * nqt_linear_int8: both for bf16 x.  Where nqt_linear_int8_launches(m, k) is 1
  * (up to 8 rows of a k that their launch can hold) xq and xscale are not used and

@@ -311,7 +311,7 @@ PyObject* linear8(PyObject* const* a) {
   } else if (xscale) {
     value_error("xscale belongs to int8 codes");
   }
-  if (m > 0x7fffffff) value_error("linear_int8 takes up to 2^31 - 1 rows");
+  if (m > 0x7fffffff - 127) value_error("linear_int8 takes up to 2^31 - 128 rows");
   Device dev;
   dev.add(x);
   dev.add(w);

@@ -880,6 +880,7 @@ int check_gemm(bool codes, const void* xq, int64_t ldxq, const float* xscale, co
   if (epilogue == kBias && !bias) return NQT_ERR_ARG;
   if (epilogue == kSiluMul ? (n % 32 != 0 || cols > n / 2) : cols != n) return NQT_ERR_ARG;
   if (k > 131072) return NQT_ERR_UNSUPPORTED;  // the int32 sums could overflow
+  if (m > INT32_MAX - (kTileM - 1) || n > INT32_MAX - (kMaxTN - 1)) return NQT_ERR_UNSUPPORTED;  // whole tiles of them
   if (codes && (!xq || !xscale || !aligned(xq, 16) || ldxq % 16 || ldxq < k)) return NQT_ERR_ARG;
   if (!aligned(w, 16) || ldw % 16 || ldw < k || ldy < cols || !aligned(y, 2)) return NQT_ERR_ARG;
   return NQT_OK;
@@ -957,6 +958,7 @@ using namespace nqt;
 extern "C" int nqt_int8_quantize_rows(const void* x, int64_t ldx, int m, int k, void* q, int64_t ldq, float* scale,
                                       void* stream) {
   if (m < 0 || k < 1 || ldx < k || ldq < k) return NQT_ERR_ARG;
+  if (k > INT32_MAX - 7) return NQT_ERR_UNSUPPORTED;  // whole vectors of 8
   if (m == 0) return NQT_OK;  // tensors without elements have no address
   if (!x || !q || !scale || !aligned(x, 2) || !aligned(scale, 4)) return NQT_ERR_ARG;
   return run_quantize(x, ldx, m, k, q, ldq, scale, as_stream(stream));

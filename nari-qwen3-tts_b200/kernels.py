@@ -659,8 +659,8 @@ def int8_quantize_rows(x: torch.Tensor, *, out: torch.Tensor | None = None,
     if x.dim() != 2 or x.dtype != torch.bfloat16 or (x.stride(1) != 1 and x.shape[1] > 1):
         raise ValueError("int8_quantize_rows takes bf16 [m, k] with unit stride along k")
     m, k = x.shape
-    if k < 1:
-        raise ValueError("int8_quantize_rows needs k >= 1")
+    if not 1 <= k <= 2**31 - 8 or m >= 2**31:
+        raise ValueError("int8_quantize_rows takes 1 <= k <= 2^31 - 8 and up to 2^31 - 1 rows")
     if out is not None and (out.shape != (m, k) or out.dtype != torch.int8 or out.stride(1) != 1):
         raise ValueError("int8_quantize_rows output must be int8 [m, k] with unit column stride")
     if scale is not None and (scale.shape != (m,) or scale.dtype != torch.float32 or not scale.is_contiguous()):
@@ -708,6 +708,8 @@ class Int8Weight:
         n, k = q.shape
         if n < 1 or not 1 <= k <= 131072:
             raise ValueError("int8 weights need n >= 1 and 1 <= k <= 131072 (int32 sums)")
+        if n > 2**31 - 256:
+            raise ValueError("int8 weights have up to 2^31 - 256 rows")
         if gate_up and n % 2:
             raise ValueError("a gate_up weight has an even number of rows")
         self.q, self.scale = q, scale

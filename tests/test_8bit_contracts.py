@@ -5,12 +5,16 @@ from __future__ import annotations
 
 import importlib
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
 
-ARG = -1
+ARG, UNSUPPORTED = -1, -4
 A = 1 << 20  # an aligned address that is never read: every call here is refused first
+ROOT = Path(__file__).resolve().parents[1]
 
 
 def _lib():
@@ -36,6 +40,35 @@ def test_linear_refuses_missing_scratch_where_it_is_used(m, k):
 
     for args in ((None, k, A), (A, k, None), (A + 8, k, A), (A, k - 16, A), (A, k + 8, A)):
         assert call(*args) == ARG
+
+
+@pytest.mark.parametrize(("m", "n"), [(2**31 - 1, 4), (2**31 - 127, 4), (4, 2**31 - 1), (4, 2**31 - 255)])
+def test_sizes_behind_32_bit_indices_are_refused(m, n):
+    """Rows and columns are rounded up to whole tiles in 32 bits.  In a process of its own: a product that went on with
+    them would not come back."""
+
+    code = f"""
+import importlib
+lib = importlib.import_module("nari-qwen3-tts_b200._lib").lib()
+print(lib.nqt_gemm_int8({A}, 16, {A}, {A}, 16, {A}, None, {A}, {n}, {m}, {n}, {n}, 16, 0, {A}, None))
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and int(r.stdout) == UNSUPPORTED
+
+
+def test_rows_behind_32_bit_indices_are_refused(nqt):
+    """The same limits at the functions, which would cut the counts to 32 bits."""
+
+    weight = nqt.kernels.Int8Weight.__new__(nqt.kernels.Int8Weight)
+    weight._lay_out(torch.zeros(6, 16, dtype=torch.int8), torch.ones(6), False)
+    row = torch.zeros(1, 16, dtype=torch.bfloat16)
+    for rows in (2**31 - 127, 2**32 + 5):
+        with pytest.raises(ValueError, match="rows"):
+            nqt.kernels.linear_int8(row.expand(rows, 16), weight)
+    for rows in (2**31 - 254, 2**32 + 2):
+        for gate_up in (False, True):
+            with pytest.raises(ValueError, match="rows"):
+                weight._lay_out(torch.zeros(1, 16, dtype=torch.int8).expand(rows, 16), torch.ones(1).expand(rows), gate_up)
 
 
 def test_quantize_no_rows():
