@@ -14,6 +14,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cfloat>
 #include <cmath>
 #include <optional>
 
@@ -234,7 +235,8 @@ PyObject* write8(PyObject* const* a) {
   if (out && (out->sizes() != q.sizes() || out->scalar_type() != at::kBFloat16 || out->stride(2) != 1))
     value_error("the rotated query must be bf16 of the query's shape, contiguous per head");
   const double eps = number(a[6]), theta = number(a[7]);
-  if (!(theta > 0)) value_error("rope_theta must be positive");
+  // as the float32 that the call takes
+  if (!(std::abs(theta) <= FLT_MAX) || !(static_cast<float>(theta) > 0)) value_error("rope_theta must be a positive float32");
   Device dev;
   for (int i : {0, 1, 2, 3, 4, 5, 8, 9, 10, 11}) dev.add(tensor(a[i]));
   dev.add(out);

@@ -427,7 +427,7 @@ extern "C" int nqt_qk_norm_rope_paged_cache8(
   if (rc != NQT_OK) return rc;
   if (!q || !k || !v || !q_weight || !k_weight || !position_ids || !write_pages || !write_offsets || !q_out)
     return NQT_ERR_ARG;
-  if (tokens < 0 || num_qo_heads < 1 || !(rope_theta > 0.f)) return NQT_ERR_ARG;
+  if (tokens < 0 || num_qo_heads < 1 || !(rope_theta > 0.f && rope_theta <= FLT_MAX)) return NQT_ERR_ARG;
   if (tokens == 0) return NQT_OK;
   const int units = num_qo_heads + 2 * num_kv_heads;
   if ((units + kWarps8 - 1) / kWarps8 > 65535) return NQT_ERR_UNSUPPORTED;

@@ -65,6 +65,10 @@ def test_rows_behind_32_bit_indices_are_refused(nqt):
     for rows in (2**31 - 127, 2**32 + 5):
         with pytest.raises(ValueError, match="rows"):
             nqt.kernels.linear_int8(row.expand(rows, 16), weight)
+    for shape in ((1, 2**31 - 7), (1, 2**32 + 5), (2**32 + 5, 1)):
+        with pytest.raises(ValueError, match="rows"):
+            nqt.kernels.int8_quantize_rows(torch.empty(shape, dtype=torch.bfloat16, device="meta"))
+    assert _lib().nqt_int8_quantize_rows(A, 2**31, 1, 2**31 - 7, A, 2**31, A, None) == UNSUPPORTED
     for rows in (2**31 - 254, 2**32 + 2):
         for gate_up in (False, True):
             with pytest.raises(ValueError, match="rows"):
@@ -89,3 +93,16 @@ def test_one_row_of_codes_with_any_pitch(nqt):
         nqt.kernels.linear_int8(base[:2, :33], weight, xscale=torch.ones(2))
     with pytest.raises(ValueError, match="16-byte"):
         nqt.kernels.linear_int8(base[1:2, :33], weight, xscale=torch.ones(1))
+
+
+@pytest.mark.parametrize("theta", [math.inf, 1e300, 1e-60, -1.0])
+def test_rope_theta_has_to_be_a_positive_float32(nqt, theta):
+    q, k = torch.zeros(2, 16, 128, dtype=torch.bfloat16), torch.zeros(2, 8, 128, dtype=torch.bfloat16)
+    w, i = torch.ones(128, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.long)
+    cache, scales = torch.zeros(4, 2, 16, 8, 128, dtype=torch.int8), torch.ones(4, 2, 1, 8)
+    with pytest.raises(ValueError, match="rope_theta"):
+        nqt.paired_qk_norm_rope_paged_cache8(q, k, k, w, w, i, 1e-6, theta, cache, scales, i, i)
+    if abs(theta) < 1e30 or theta == math.inf:
+        args = [A, 4096, 128, A, 4096, 128, A, 4096, 128, A, A, A, A, A, A, 2048, 128, A, A, 64, 16, 3, 16, 8, 128, 1e-6,
+                theta, 3, A, None]
+        assert _lib().nqt_qk_norm_rope_paged_cache8(*args) == ARG
