@@ -6,7 +6,8 @@ objects are linked into ``libnqt.so`` next to this file (in-tree, so the
 library travels with the source tree).  Objects go to ``_build/``.
 ``csrc/bind.cpp`` is compiled with the host compiler against the running
 Python and torch.  A rebuild happens only when a source or header is newer
-than the libraries.
+than the libraries, or when the binding was compiled against another Python
+or torch.
 """
 
 from __future__ import annotations
@@ -61,8 +62,25 @@ def up_to_date() -> bool:
     return _newer(LIB_PATH, _inputs()) and _bind_up_to_date()
 
 
+def _bind_key() -> str:
+    """What the binding was compiled against, besides its sources."""
+
+    import torch
+
+    return f"{sysconfig.get_config_var('SOABI')} torch {torch.__version__}"
+
+
+def _bind_stamp() -> Path:
+    return BUILD_DIR / "bind.txt"
+
+
+def _mark_bind() -> None:
+    _bind_stamp().write_text(_bind_key())
+
+
 def _bind_up_to_date() -> bool:
-    return _newer(BIND_PATH, [CSRC / "bind.cpp", *(REPO_DIR / "include").glob("*.h")])
+    return (_newer(BIND_PATH, [CSRC / "bind.cpp", *(REPO_DIR / "include").glob("*.h")]) and _bind_stamp().exists()
+            and _bind_stamp().read_text() == _bind_key())
 
 
 def _cuda_include() -> Path:
@@ -88,6 +106,8 @@ def build_bind() -> Path:
     if proc.returncode != 0:
         raise RuntimeError(f"compiling bind.cpp failed:\n{proc.stderr}")
     os.replace(tmp, BIND_PATH)
+    BUILD_DIR.mkdir(exist_ok=True)
+    _mark_bind()
     return BIND_PATH
 
 

@@ -106,3 +106,18 @@ def test_rope_theta_has_to_be_a_positive_float32(nqt, theta):
         args = [A, 4096, 128, A, 4096, 128, A, 4096, 128, A, A, A, A, A, A, 2048, 128, A, A, 64, 16, 3, 16, 8, 128, 1e-6,
                 theta, 3, A, None]
         assert _lib().nqt_qk_norm_rope_paged_cache8(*args) == ARG
+
+
+def test_binding_is_compiled_again_for_another_torch(monkeypatch, tmp_path):
+    """The binding belongs to the torch and the Python that it was compiled against, whatever its age."""
+
+    build = importlib.import_module("nari-qwen3-tts_b200.build")
+    for path in ("BUILD_DIR", "BIND_PATH"):
+        monkeypatch.setattr(build, path, tmp_path / path)
+    build.BUILD_DIR.mkdir()
+    build.BIND_PATH.write_bytes(b"")
+    assert not build._bind_up_to_date()  # nothing says what it was compiled against
+    build._mark_bind()
+    assert build._bind_up_to_date()
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    assert not build._bind_up_to_date()
