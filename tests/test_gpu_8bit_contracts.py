@@ -265,3 +265,105 @@ def test_one_row_of_codes_with_any_pitch(nqt, cuda):
     assert x.stride(0) == 101
     want = (base[0, :33].double() @ weight.q.cpu().double().t()).to(torch.float32).to(torch.bfloat16)
     assert torch.equal(nqt.kernels.linear_int8(x, weight, xscale=xs).cpu()[0], want)
+
+
+# ------------------------------------------------------------------------------------------------ stricter checks
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize(("lens", "chunks"), [([1, 16, 17, 40, 33], [1, 1, 1, 1, 1]), ([37, 300, 16, 129], [37, 45, 16, 1]),
+                                              ([20, 30, 64, 700], [3, 15, 50, 640])])
+def test_write_each_code(nqt, cuda, kind, lens, chunks):
+    """Every code that the call writes or rounds again, by itself: equal to the exact one, or one step beside it where
+    the exact quotient lies within fp32's error of the middle between two codes."""
+
+    hq, hkv, d = 16, 8, 128
+    codes, scales, indptr, indices, _ = make_cache8(lens, kind=kind, hkv=hkv, d=d, seed=21)
+    g = torch.Generator().manual_seed(22)
+    pos = torch.cat([torch.arange(n - c, n) for n, c in zip(lens, chunks, strict=True)])
+    row = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(chunks))
+    pages = indices.long()[indptr.long()[row] + pos // 16]
+    offs = pos % 16
+    t = len(pos)
+    qkv = (torch.randn(t, hq + 2 * hkv, d, generator=g) * torch.exp(torch.randn(t, 1, 1, generator=g))).to(torch.bfloat16)
+    qw, kw = ((1 + 0.2 * torch.randn(d, generator=g)).to(torch.bfloat16) for _ in range(2))
+    k, v = qkv[:, hq:hq + hkv], qkv[:, hq + hkv:]
+    dq, dc, ds = qkv.to(cuda), codes.to(cuda), scales.to(cuda)
+    nqt.paired_qk_norm_rope_paged_cache8(dq[:, :hq], dq[:, hq:hq + hkv], dq[:, hq + hkv:], qw.to(cuda), kw.to(cuda),
+                                         pos.to(cuda), EPS, THETA, dc, ds, pages.to(cuda), offs.to(cuda))
+    new = torch.stack([oc8.norm_rope(k, kw, pos, EPS, THETA), v.double()], 1)  # [t, 2, hkv, d]
+    wc, ws = numbers(codes), scales.double()
+    oc8.write(wc, ws, new, pages.tolist(), offs.tolist(), kind)
+    gc, gs = numbers(dc.cpu()), ds.cpu().double()
+
+    written = torch.zeros(codes.shape[:3], dtype=torch.bool)
+    written[pages, :, offs] = True
+    # codes that a growing scale rounded again, and all that the call left: a power of two is exact
+    assert torch.equal(gc[~written], wc[~written])
+    # A rotated key: 2^-20 of the two elements that it is made of (cos and sin 2^-22; the norm 2^-22 of rsqrt and as much
+    # of its sum; four roundings).  The block's largest is at least half of such a pair, so the scale is off by 2^-19.  The
+    # scale's division and the quotient's two roundings: 2^-22 in all, for V too.
+    plain = torch.sqrt(k.double().square().mean(-1, keepdim=True) + EPS)
+    plain = (k.double() / plain * kw.double()).abs()
+    pair = plain + plain.roll(d // 2, -1)
+    err = torch.stack([2.0**-20 * pair, torch.zeros_like(pair)], 1)
+    s = ws[pages, :, offs // 16][..., None]
+    x = torch.where(s > 0, new / s.clamp_min(1e-300), 0.0)
+    err = err / s.clamp_min(1e-300) + x.abs() * torch.tensor([2.0**-19 + 2.0**-22, 2.0**-22]).view(1, 2, 1, 1).double()
+    want, got = oc8.nearest_code(x, kind), gc[pages, :, offs]
+    low, high = oc8.nearest_code(x - err, kind), oc8.nearest_code(x + err, kind)
+    assert torch.equal(want, wc[pages, :, offs])
+    assert ((got >= low) & (got <= high)).all()
+    assert ((gs - ws).abs() <= 2.0**-19 * ws).all()
+
+
+def _step(nqt, case, ws, overlap):
+    q, k, v, w, pos, cache, scales, pages, offs, table = case
+    rot = nqt.paired_qk_norm_rope_paged_cache8(q, k, v, w, w, pos, EPS, THETA, cache, scales, pages, offs)
+    return nqt.batch_decode_paged8(rot, cache, scales, *table, ws, overlap_kv_write=overlap)
+
+
+def _step_case(cuda, lens, kind, seed):
+    codes, scales, indptr, indices, last = make_cache8(lens, kind=kind, seed=seed)
+    qkv = _q(len(lens), 32, 128, seed + 1).to(cuda)
+    pos = torch.tensor(lens) - 1
+    pages = indices.long()[indptr.long()[:-1] + pos // 16]
+    w = torch.ones(128, dtype=torch.bfloat16, device=cuda)
+    return [qkv[:, :16], qkv[:, 16:24], qkv[:, 24:], w, pos.to(cuda), codes.to(cuda), scales.to(cuda), pages.to(cuda),
+            (pos % 16).to(cuda), [t.to(cuda) for t in (indptr, indices, last)]]
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_streams_at_once_each_with_its_own_cache(nqt, cuda, kind):
+    """Two captured steps on two streams and eager ones on a third, each with a cache and a workspace of its own: every
+    result on every round is the one that it gives alone."""
+
+    cases = [_step_case(cuda, lens, kind, s) for s, lens in ((31, [3000, 5, 77, 640]), (33, [64, 4100]), (35, [1900, 9, 48]))]
+    start = [(c[5].clone(), c[6].clone()) for c in cases]
+    spaces = [nqt.decode_paged8_workspace(len(c[4]), 16, 128, cuda) for c in cases]
+
+    def reset():
+        for c, (cache, scales) in zip(cases, start, strict=True):
+            c[5].copy_(cache)
+            c[6].copy_(scales)
+        torch.cuda.synchronize()
+
+    want = []
+    for c, ws in zip(cases, spaces, strict=True):
+        reset()
+        want.append(_step(nqt, c, ws, False))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for c, ws in zip(cases[:2], spaces, strict=False):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_step(nqt, c, ws, True))
+        graphs.append(graph)
+    for _ in range(10):
+        reset()
+        for s, graph in zip(streams, graphs, strict=False):
+            with torch.cuda.stream(s):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = _step(nqt, cases[2], spaces[2], True)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[2])
