@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import cache8 as oc8
-from tests._cache8 import make_cache8, numbers
+from tests._cache8 import attention_tolerance, make_cache8, numbers
 
 pytestmark = pytest.mark.gpu
 
@@ -367,3 +367,59 @@ def test_streams_at_once_each_with_its_own_cache(nqt, cuda, kind):
             eager = _step(nqt, cases[2], spaces[2], True)
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[2])
+
+
+# ------------------------------------------------------------------------------------------------ page sizes and many rows
+def _close(got, want, mag):
+    over = (got.cpu().double() - want).abs() - attention_tolerance(want, mag)
+    assert torch.isfinite(got).all() and over.max() <= 0, f"off by {float(over.max()):.3g} above the tolerance"
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("page_size", [48, 80, 112, 240])
+def test_page_sizes_that_are_no_power_of_two(nqt, cuda, kind, page_size):
+    lens, chunks = [700, 95, 48, 1], [150, 95, 1, 1]
+    codes, scales, indptr, indices, last = make_cache8(lens, kind=kind, page_size=page_size, hkv=2, d=64, seed=page_size)
+    qo = torch.tensor([0, *torch.tensor(chunks).cumsum(0).tolist()], dtype=torch.int32)
+    q = _q(sum(chunks), 6, 64, 3)
+    table = [t.to(cuda) for t in (indptr, indices, last)]
+    dev = [t.to(cuda) for t in (codes, scales)]
+    exact = (numbers(codes), scales.double(), indptr, indices, last)
+    nqt.kernels.clear_status(cuda)
+    _close(nqt.batch_prefill_paged8(q.to(cuda), *dev, qo.to(cuda), *table), *oc8.attention(q, *exact, qo))
+    ends = (qo[1:] - 1).long()
+    ws = nqt.decode_paged8_workspace(4, 6, 64, cuda)
+    _close(nqt.batch_decode_paged8(q[ends].to(cuda), *dev, *table, ws), *oc8.attention(q[ends], *exact))
+    # the write: block by block what it is in pages of 16
+    pos = torch.cat([torch.arange(n - c, n) for n, c in zip(lens, chunks, strict=True)])
+    row = torch.repeat_interleave(torch.arange(4), torch.tensor(chunks))
+    pages, offs = indices.long()[indptr.long()[row] + pos // page_size], pos % page_size
+    per = page_size // 16
+    small = [codes.view(-1, 2, per, 16, 2, 64).transpose(1, 2).reshape(-1, 2, 16, 2, 64).contiguous().to(cuda),
+             scales.transpose(1, 2).reshape(-1, 2, 1, 2).contiguous().to(cuda)]
+    k, v = (_q(len(pos), 2, 64, s).to(cuda) for s in (4, 5))
+    w = torch.ones(64, dtype=torch.bfloat16, device=cuda)
+    for cache, page, off in ((dev, pages, offs), (small, pages * per + offs // 16, offs % 16)):
+        nqt.paired_qk_norm_rope_paged_cache8(q.to(cuda), k, v, w, w, pos.to(cuda), EPS, THETA, *cache, page.to(cuda),
+                                             off.to(cuda))
+    big = dev[0].view(-1, 2, per, 16, 2, 64).transpose(1, 2).reshape(-1, 2, 16, 2, 64)
+    assert torch.equal(big.view(torch.uint8), small[0].view(torch.uint8))
+    assert torch.equal(dev[1].transpose(1, 2).reshape(-1, 2, 1, 2), small[1])
+    got = [nqt.read_paged_cache8(*c, torch.arange(len(c[0]), device=cuda)) for c in (dev, small)]
+    assert torch.equal(got[0].view(-1, 2, per, 16, 2, 64).transpose(1, 2).reshape(-1, 2, 16, 2, 64), got[1])
+    assert nqt.kernels.read_status(cuda) == 0
+
+
+def test_decode_as_many_rows_as_a_launch_takes(nqt, cuda):
+    lens = torch.randint(0, 24, (8192,), generator=torch.Generator().manual_seed(1)).tolist()
+    lens[77] = 3000
+    codes, scales, indptr, indices, last = make_cache8(lens, hkv=1, d=64, seed=2)
+    q = _q(8192, 2, 64, 3)
+    dev = [t.to(cuda) for t in (q, codes, scales, indptr, indices, last)]
+    ws = nqt.decode_paged8_workspace(8192, 2, 64, cuda)
+    first = nqt.batch_decode_paged8(*dev, ws)
+    assert torch.equal(first, nqt.batch_decode_paged8(*dev, ws))
+    _close(first, *oc8.attention(q, numbers(codes), scales.double(), indptr, indices, last))
+    with pytest.raises(nqt._lib.NqtError):
+        nqt.batch_decode_paged8(dev[0].repeat(2, 1, 1), *dev[1:3], torch.zeros(16385, dtype=torch.int32, device=cuda),
+                                dev[4], torch.ones(16384, dtype=torch.int32, device=cuda), ws)
