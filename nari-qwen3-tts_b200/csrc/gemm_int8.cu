@@ -65,7 +65,8 @@ struct RowRule {
   __device__ __forceinline__ explicit RowRule(uint32_t mx) {
     amax = __uint_as_float(mx << 16);
     s = __fdiv_rn(amax, 127.f);
-    f = amax == 0.f ? 0.f : __fdiv_ru(127.f, amax);
+    f = amax == 0.f ? 0.f : __fdiv_rn(127.f, amax);
+    if (fmaf(f, amax, -127.f) < 0.f) f = __uint_as_float(__float_as_uint(f) + 1u);  // up
     plain = f <= 3.0e38f && mx < 0x7f80u;
   }
   __device__ __forceinline__ uint32_t odd(uint32_t bf16_bits) const {
