@@ -28,7 +28,8 @@
 // and V are read twice, once for the maximum and once (from L1) to be rounded; between the two only the rows' norms
 // are kept.  Few tokens: windows of one token and up to one unit per warp, for latency.  Many: windows of 16, the
 // groups of an aligned prefill.  Bound by latency for a decode step, by instruction issue for a prefill.  One B200, 16
-// query and 8 KV heads of 128: 200 tokens 9 us, 4893 tokens 31 us (70 MB), 16384 tokens 89 us (2.6 TB/s).
+// query and 8 KV heads of 128, captured graphs: 200 tokens 9.6 us, 4893 tokens 31 us (70 MB), 16384 tokens 87 us (2.7
+// TB/s).  The page read: 307 pages 8.1 us, 1025 pages 22 us (4.6 TB/s).
 #include "cache8.cuh"
 
 #include <float.h>

@@ -44,10 +44,11 @@
 // P goes from the accumulator layout to the B layout with movmatrix.
 //
 // Bound by HBM for large batches and by a chain of dependent trips (row lengths,
-// page ids, TMA, tickets: about 6 us) for small ones.  One B200, captured graphs:
-// 1 row of 300 tokens 9.0 us; 64 rows of 64 to 2048 tokens (16 query and 8 KV
-// heads of 128) 35 us, 144 MB; 240 rows of 32 to 4096 172 to 177 us, 6.1 TB/s; five
-// rows of 20001 to 98765 tokens (14 and 2 heads of 64) 30 us, 81 MB.
+// page ids, TMA, tickets: about 6 us) for small ones.  One B200, one call among others
+// and in a captured graph: 1 row of 300 tokens 9.4 and 9.1 us; 64 rows of 64 to 2048
+// tokens (16 query and 8 KV heads of 128) 35.9 and 35.5, 144 MB; 240 rows of 32 to 4096
+// 176 to 191 and 172 to 176, 5.6 to 6.2 TB/s; five rows of 20001 to 98765 tokens (14 and
+// 2 heads of 64) 30 and 30, 81 MB.
 #include "cache8.cuh"
 
 namespace nqt {

@@ -32,10 +32,11 @@
 // its first weights already on their way, and a warp takes two weight rows at a
 // time (gate and up of one column) with dp4a.
 //
-// One B200, captured graphs, weights from HBM, with the quantiser: 1 x 2048 x 2048
-// with bias 3.9 us; 64 x 12288 x 2048 with SwiGLU 7.8; 64 x 2048 x 6144 9.1;
-// 4613 x 2048 x 6144 56.5, of which the product 42 (2.8 POP/s, tensor pipe 66 %
-// busy).
+// One B200, captured graphs, bf16 tokens, weights from HBM (from L2): 1 x 2048 x 2048 with
+// bias 4.2 us (4.0); 64 x 12288 x 2048 with SwiGLU 10.4 (8.0), of codes 7.9; 64 x 2048 x
+// 6144 9.1 (7.9), of codes 7.1; 4613 x 2048 x 6144 56, of which the product 40 (2.9 POP/s,
+// tensor pipe 66 % busy).  One call among others, weights from L2: 5.0, 8.9 and 65 us for
+// the first, second and last.
 #include <algorithm>
 #include <cstdint>
 #include <mutex>
@@ -51,8 +52,8 @@ using namespace gemm_detail;
 
 // ------------------------------------------------------------------ quantiser
 // The rule of a row whose largest |bf16| bits are `mx`: scale, factor and the codes of its values.  A value times the
-// factor plus 1.5 2^23 is the rounded code in the sum's low bits: one rounding, no conversion (1024 x 6144: 5.0 -> 3.8
-// us).
+// factor plus 1.5 2^23 is the rounded code in the sum's low bits: one rounding, no conversion (1024 x 6144
+// from L2: 3.6 us; with a rounding and a conversion each 5.0).
 //
 // The codes are exactly round(x 127 / amax), ties to even, because the factor 127 / amax is rounded up.  Write x and amax
 // as 8-bit integers times powers of two: a quotient q that is no tie is q / (254 255) or more away from one, and the factor
@@ -796,9 +797,10 @@ int boxes_per_stage(int rows, int tn) { return 3 * 2 * (rows + tn) * kBlockK <= 
 // Weight rows per tile, and the CTAs that share a tile's K.  The times of a wave's tiles in ns, fitted to a sweep over
 // 16 to 4613 tokens and five weights on one B200.  A box of K costs its barriers and the issue of its products, about
 // 120 with two boxes a stage and 270 with one, and wide tiles what they bring into shared memory.  So tiles are as
-// narrow as one wave allows (64 tokens x 12288 x 2048: width 96, 7.8 us, against 128, 8.5, and 192, 10.0), and K is
-// shared where that saves more boxes than the cluster's two barriers and the exchange of rows x tn sums cost
-// (128 tokens x 2048 x 6144: 7.6 us, against 8.7 undivided; 64 x 2048 x 2048: 5.5 against 4.7, so undivided).
+// narrow as one wave allows (products of codes, weights from HBM: 64 tokens x 12288 x 2048: width 96, 7.8 us, against 128,
+// 8.5, and 192, 10.0), and K is shared where that saves more boxes than the cluster's two barriers and the exchange of
+// rows x tn sums cost (128 tokens x 2048 x 6144: 7.7 us, against 8.7 undivided; 64 x 2048 x 2048: 5.5 against 4.7, so
+// undivided).
 struct Tiling {
   int tn, split;
 };
@@ -936,9 +938,9 @@ int run_quantize(const void* x, int64_t ldx, int m, int k, void* q, int64_t ldq,
   const bool vec = aligned(x, 16) && ldx % 8 == 0 && k % 8 == 0 && aligned(q, 8) && ldq % 8 == 0;
   const __nv_bfloat16* xp = static_cast<const __nv_bfloat16*>(x);
   int8_t* qp = static_cast<int8_t*>(q);
-  // A warp per row where its lanes hold the row (k <= 1024: 4613 x 1024 on one B200 3.4 us, against 7.2 with four warps),
-  // and up to 2048 when there are rows enough for the GPU (4613 x 2048: 7.0 us, against 9.2); else four warps, which hold
-  // 6144 elements (4613 x 6144: 14.4 us, 5.9 TB/s, against 16.1 with eight warps).
+  // A warp per row where its lanes hold the row (k <= 1024: 4613 x 1024 from HBM on one B200 4.0 us, against 7.7 with four
+  // warps), and up to 2048 when there are rows enough for the GPU (4613 x 2048: 7.1 us, against 9.3); else four warps,
+  // which hold 6144 elements (4613 x 6144: 14.5 us, 5.9 TB/s, against 15.9 with eight warps).
   const bool warp_rows = k <= 1024 || (k <= 2048 && m >= 8 * num_sms());
   auto kernel = warp_rows ? (vec ? int8_quantize_rows_kernel<32, true> : int8_quantize_rows_kernel<32, false>)
                           : (vec ? int8_quantize_rows_kernel<128, true> : int8_quantize_rows_kernel<128, false>);

@@ -30,9 +30,11 @@
 // walking over a part of its keys; the parts are joined in the cluster's shared memory in CTA order, so there is no
 // workspace and nothing depends on timing.
 //
-// Bound by the softmax warps' instructions: a block costs about 2150 clocks, of which the tensor pipe and MUFU each
-// need about 1024.  On one B200 (16 query and 8 KV heads of 128, captured graphs): eight prompts of 2048 tokens 187 us,
-// eight first chunks of 128 to 1024 53 us, two chunks of 301 to 515 behind 9000 to 16001 tokens 166 us.
+// Bound by the softmax warps: for a block the tensor pipe and MUFU each need about 1024 clocks and are busy 35 to 42 % of
+// the time; 54 % of the issue slots are used, and the warps wait for TMEM loads, fixed latencies and one another.  On one
+// B200 (16 query and 8 KV heads of 128), one call among others and in a captured graph: eight prompts of 2048 tokens 201
+// and 186 us, eight first chunks of 128 to 1024 55 and 53, two chunks of 301 to 515 behind 9000 to 16001 tokens 172 and
+// 166.
 #include "cache8.cuh"
 #include "gemm_common.cuh"
 #include "tcgen05.cuh"
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(p8::kThreads, 1)
         }
         const bool last = item.row < 0 && !more;
         if (more && ok) {
-          // One item ahead: asked for when this one's queries are on their way.  (Eight prompts of 2048: 187 us, against
+          // One item ahead: asked for when this one's queries are on their way.  (Eight prompts of 2048: 186 us, against
           // 212 when it is asked for with this one's last keys, and 245 with one item per CTA.)
           if (lane == 0) {
             mbar_arrive_expect_tx(steal_bar, 16);
